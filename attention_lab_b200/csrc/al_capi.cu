@@ -10,7 +10,7 @@
 #include "al_context.cuh"
 #include "al_index.cuh"
 #include "al_prefill.cuh"
-#include "../../include/attention_lab_b200.h"
+#include "al_host.h"
 
 namespace al {
 __device__ unsigned g_al_error;   // kernel error bits (see kErr*)
@@ -19,8 +19,13 @@ __device__ unsigned g_al_error;   // kernel error bits (see kErr*)
 using namespace al;
 
 namespace {
-
 thread_local char g_msg[1024] = "";
+std::mutex g_mu;
+DeviceInfo g_dev[64];
+std::unordered_map<unsigned long long, int> g_smem_set;   // (kernel, device) -> dynamic smem bytes allowed
+}  // namespace
+
+namespace al {
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -33,18 +38,6 @@ int fail(int code, const char* fmt, ...) {
 int cuda_fail(cudaError_t e, const char* where) {
   return fail(AL_ECUDA, "%s: %s", where, cudaGetErrorString(e));
 }
-
-constexpr int kMaxRanks = 64;   // ranks of one exchange (the flag array of a channel holds one word each)
-
-struct DeviceInfo {
-  int sms = 0;
-  int max_smem_optin = 0;
-  unsigned* err = nullptr;
-};
-
-std::mutex g_mu;
-DeviceInfo g_dev[64];
-std::unordered_map<unsigned long long, int> g_smem_set;   // (kernel, device) -> dynamic smem bytes allowed
 
 int device_info(DeviceInfo** out) {
   int dev = 0;
@@ -66,12 +59,10 @@ int device_info(DeviceInfo** out) {
   return AL_OK;
 }
 
-template <typename K>
-int prepare_kernel(K kernel, size_t smem, int cs) {
+int prepare_kernel_ptr(const void* kernel, size_t smem) {
   int dev = 0;
   cudaGetDevice(&dev);
-  const unsigned long long key = (reinterpret_cast<unsigned long long>(reinterpret_cast<const void*>(kernel)) << 6) ^
-                                 (unsigned long long)dev;
+  const unsigned long long key = (reinterpret_cast<unsigned long long>(kernel) << 6) ^ (unsigned long long)dev;
   std::lock_guard<std::mutex> lk(g_mu);
   auto it = g_smem_set.find(key);
   if (it == g_smem_set.end() || it->second < (int)smem) {
@@ -83,15 +74,20 @@ int prepare_kernel(K kernel, size_t smem, int cs) {
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared memory carve-out)");
     g_smem_set[key] = (int)smem;
   }
-  (void)cs;
   return AL_OK;
 }
+
+}  // namespace al
+
+namespace {
+
+constexpr int kMaxRanks = 64;   // ranks of one exchange (the flag array of a channel holds one word each)
 
 std::unordered_map<unsigned long long, int> g_cluster_ok;   // (kernel, cs, smem, device) -> schedulable
 
 template <typename K, typename... P>
 int launch(K kernel, dim3 grid, int cs, size_t smem, void* stream, const P&... p) {
-  int rc = prepare_kernel(kernel, smem, cs);
+  int rc = prepare_kernel(kernel, smem);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -131,14 +127,6 @@ int launch(K kernel, dim3 grid, int cs, size_t smem, void* stream, const P&... p
   return AL_OK;
 }
 
-int plain_launch_check(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, what);
-  return AL_OK;
-}
-
-bool dtype_ok(int t) { return t == AL_F32 || t == AL_BF16; }
-int esize(int t) { return t == AL_F32 ? 4 : 2; }
 int pad_heads(int h) { return h <= 1 ? 1 : (h <= 2 ? 2 : 4); }
 size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
@@ -285,8 +273,6 @@ int dispatch_attend(const AttendParams& p, int kv_dtype, int hp, dim3 grid, int 
     default: return launch(attend_kernel<float, 4>, grid, cs, smem, stream, p);
   }
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Shared validation + launch of the fused kernel (decode step or select-only).
 int run_fused(DecodeParams p, int kv_dtype, int idx_dtype, int d, int cluster, void* stream, bool attend) {
@@ -930,7 +916,7 @@ int al_prefill_score_topk(const void* u, long long u_sh, long long u_st, const v
   if (rc) return rc;
   CUtensorMap zmap;
   if (!pf_tensor_map(zT, H, C, z_sh, z_ld, &zmap)) return fail(AL_ECUDA, "cuTensorMapEncodeTiled refused the zT layout");
-  rc = prepare_kernel(prefill_topk_kernel, kPfSmem, 1);
+  rc = prepare_kernel(prefill_topk_kernel, kPfSmem);
   if (rc) return rc;
   PrefillParams p{};
   p.u = static_cast<const __nv_bfloat16*>(u); p.u_sh = u_sh; p.u_st = u_st;

@@ -28,7 +28,7 @@
 #pragma once
 #include <climits>
 #include <cuda.h>
-#include "al_common.cuh"
+#include "al_tcgen05.cuh"
 
 namespace al {
 
@@ -64,14 +64,7 @@ struct PrefillParams {
   unsigned* err;
 };
 
-// ------------------------------------------------------------------------------------------------ tcgen05 helpers
-// Shared-memory matrix descriptor (sm_100): start address, leading and stride byte offsets (all >> 4), version 1,
-// layout type in bits 61..63 (0 = no swizzle, 2 = 128-byte swizzle).
-__device__ __forceinline__ uint64_t pf_sdesc(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint32_t layout) {
-  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)((lbo >> 4) & 0x3fffu) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3fffu) << 32) | (1ull << 46) | ((uint64_t)layout << 61);
-}
-
+// ------------------------------------------------------------------------------------------------ MMA and copies
 // Instruction descriptor of kind::f16: fp32 accumulator, bf16 A and B, A K-major, B N-major, M = 128, N = 128.
 constexpr uint32_t kPfIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(kPfTile >> 3) << 17) |
                               ((uint32_t)(kPfRows >> 4) << 24);
@@ -81,38 +74,12 @@ __device__ __forceinline__ void pf_mma(uint32_t tmem_d, uint64_t adesc, uint64_t
                " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
                ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(kPfIdesc), "r"(accumulate) : "memory");
 }
-// Arrive once on `bar` when every MMA this thread issued so far has completed.
-__device__ __forceinline__ void pf_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
-               ::"r"((uint32_t)__cvta_generic_to_shared(bar)) : "memory");
-}
-__device__ __forceinline__ void pf_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"((uint32_t)__cvta_generic_to_shared(bar)) : "memory");
-}
 // 3-D tiled bulk copy (x = column, y = index row, z = head) completing on `bar`; x * 2 bytes is a multiple of 128.
 __device__ __forceinline__ void pf_tma3(uint32_t dst, const void* map, int x, int y, int z, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z),
                "r"((uint32_t)__cvta_generic_to_shared(bar)) : "memory");
 }
-// 32 consecutive TMEM columns of the thread's lane; the values are defined after pf_tmem_wait.
-__device__ __forceinline__ void pf_tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-                 "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-                 "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-               : "r"(taddr) : "memory");
-}
-// Wait for this thread's TMEM loads; the empty statements tie every loaded register to the wait so no use of them
-// is scheduled before it.
-__device__ __forceinline__ void pf_tmem_wait(uint32_t (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-#pragma unroll
-  for (int j = 0; j < 32; ++j) asm volatile("" : "+r"(v[j]));
-}
-
 // ------------------------------------------------------------------------------------------------ keys
 // Canonical key (signed order): NaN above +inf, -0 = +0, negative scores below every non-negative one. On positive
 // finite scores it equals the raw bit pattern, which is what rows in the fast mode use.
@@ -296,15 +263,6 @@ __device__ __forceinline__ void pf_anchor(float m, PfRow& r) {
     r.sum = 0.0f;
   } else {
     pf_restart_canonical(r);
-  }
-}
-
-// Bounded wait; after the first wait that gives up, the CTA stops waiting (its results are invalid and flagged).
-__device__ __forceinline__ void pf_wait(uint64_t* bar, unsigned parity, volatile int* abort_flag, unsigned* err) {
-  if (*abort_flag) return;
-  if (!mbar_wait(bar, parity)) {
-    *abort_flag = 1;
-    atomicOr(err, kErrWaitLimit);
   }
 }
 
