@@ -1,0 +1,288 @@
+// C ABI of the 8-bit cache: validation, launch-shape choice and dispatch.
+// Declarations and contracts: include/attention_lab_b200.h.
+#include <algorithm>
+
+#include "al_host.h"
+#include "al_q8_prompt.cuh"
+
+using namespace al;
+
+namespace {
+
+bool rows_aligned(const void* p, const int64_t* strides, int n, int dtype) {
+  const int64_t unit = 16 / esize(dtype);
+  if (!aligned16(p)) return false;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % unit) return false;
+  return true;
+}
+
+int rot_table(const float* table, int rows, int rot, int layout, int d, RotTable* out) {
+  if (!table) return fail(AL_EINVAL, "null rotary table");
+  if (rows < 1) return fail(AL_EINVAL, "the rotary table needs at least one row");
+  if (rot < 2 || rot % 2 || rot > d) return fail(AL_EINVAL, "rotary_dim must be even and in [2, head_dim=%d], got %d", d, rot);
+  if (layout != AL_ROT_HALF && layout != AL_ROT_INTERLEAVED) return fail(AL_EINVAL, "unknown rotary layout %d", layout);
+  if (!aligned16(table)) return fail(AL_EUNSUPPORTED, "the rotary table must start on a 16-byte boundary");
+  out->table = table; out->rows = rows; out->rot = rot; out->layout = layout;
+  return AL_OK;
+}
+
+// Shape checks every 8-bit cache entry shares.
+int q8_shape(int B, int G, int C, int d, const void* kc, const void* vc, const void* ke, const void* ve) {
+  if (B < 0 || G <= 0 || C <= 0) return fail(AL_EINVAL, "G and C must be positive and B not negative");
+  if (d != kHeadDim) return fail(AL_EUNSUPPORTED, "head_dim must be %d, got %d", kHeadDim, d);
+  if (B * (long long)G > 65535) return fail(AL_EUNSUPPORTED, "B*G = %lld exceeds 65535", B * (long long)G);
+  if (B == 0) return AL_OK;
+  if (!kc || !vc || !ke || !ve) return fail(AL_EINVAL, "null cache pointer");
+  if (!aligned16(kc) || !aligned16(vc)) return fail(AL_EUNSUPPORTED, "the codes must start on a 16-byte boundary");
+  return AL_OK;
+}
+
+int q8_blocks(int C) { return (C + kQ8Block - 1) / kQ8Block; }
+
+// The attend's kernel, and how it splits its work.
+struct Q8Plan {
+  bool token;                       // the few-column kernel (mma.sync); else the prompt kernel (tcgen05)
+  int cs;                           // token: CTAs per cluster
+  int row_tiles, nsplit;            // prompt: tiles of 256 rows, key splits
+  size_t ml_off, bytes;             // prompt with nsplit > 1: workspace layout
+};
+
+int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_length, int sms, Q8Plan* out) {
+  Q8Plan pl = {};
+  const long long R = (long long)h * T, segs = (long long)B * G;
+  int len = max_length > 0 ? std::min(max_length, C) : C;
+  // tokens a query tile can see, as far as the host knows
+  const long long span = window > 0 ? std::min<long long>(len, (long long)window + sinks) : len;
+  if (R <= kQ8TokenCols) {
+    pl.token = true;
+    const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
+    pl.cs = 1;
+    while (pl.cs < kMaxCluster && units * pl.cs < 2LL * sms && span > (long long)pl.cs * 2 * kQdWarps * kQdStep) pl.cs <<= 1;
+  } else {
+    pl.row_tiles = (int)((R + 2 * kQpRows - 1) / (2 * kQpRows));
+    const long long ctas = segs * pl.row_tiles;
+    const long long tiles = (span + T + kQpKeys - 1) / kQpKeys + 1;
+    pl.nsplit = 1;
+    if (ctas < sms) pl.nsplit = (int)std::max<long long>(1, std::min<long long>(sms / ctas, tiles / 4));
+    if (pl.nsplit > 1) {
+      const size_t rows = (size_t)segs * (size_t)R;
+      pl.ml_off = (size_t)pl.nsplit * rows * kHeadDim * sizeof(float);
+      pl.bytes = pl.ml_off + (size_t)pl.nsplit * rows * 2 * sizeof(float);
+    }
+  }
+  *out = pl;
+  return AL_OK;
+}
+
+int q8_attend_check(int B, int G, int h, int T, int C, int window, int sinks) {
+  if (h < 1 || T < 0) return fail(AL_EINVAL, "h must be positive and T not negative, got h=%d T=%d", h, T);
+  if (window < 0 || sinks < 0) return fail(AL_EINVAL, "window and sinks must not be negative, got %d and %d", window, sinks);
+  if ((long long)h * T > (1 << 28)) return fail(AL_EUNSUPPORTED, "h*T = %lld exceeds 2^28 query rows per group", (long long)h * T);
+  if (B * (long long)G * (((long long)h * T + 255) / 256) > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query tiles");
+  (void)C;
+  return AL_OK;
+}
+
+template <typename T>
+int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long R = (long long)p.h * p.T;
+  int rc;
+  if (pl.token) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)pl.cs, (unsigned)(p.B * p.G), (unsigned)((R + kQdCols - 1) / kQdCols));
+    cfg.blockDim = dim3(kQdThreads, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)pl.cs;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (pl.cs > 8 && (rc = prepare_kernel(q8_decode_kernel<T>, 0))) return rc;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, q8_decode_kernel<T>, p);
+    return e == cudaSuccess ? AL_OK : cuda_fail(e, "q8_decode_kernel");
+  }
+  if ((rc = prepare_kernel(q8_prompt_kernel<T>, kQpSmem))) return rc;
+  const dim3 grid((unsigned)(p.B * p.G * pl.row_tiles), (unsigned)pl.nsplit);
+  q8_prompt_kernel<T><<<grid, kQpThreads, kQpSmem, st>>>(p);
+  if ((rc = plain_launch_check("q8_prompt_kernel"))) return rc;
+  if (pl.nsplit > 1) {
+    const long long rows = (long long)p.B * p.G * R;
+    q8_merge_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
+    return plain_launch_check("q8_merge_kernel");
+  }
+  return AL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int al_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, const int64_t* k_strides, int Hk, int dtype,
+              const float* table, int table_rows, int rot, int layout, const int64_t* positions,
+              const int64_t* pos_strides, int64_t start, int B, int T, int d, int inverse, void* q_out, void* k_out,
+              void* stream) {
+  if (!dtype_ok(dtype)) return fail(AL_EINVAL, "unknown dtype code");
+  if (B < 0 || T < 0 || Hq < 1 || Hk < 0) return fail(AL_EINVAL, "need B, T >= 0, Hq >= 1 and Hk >= 0");
+  if (d < 8 || d % 8 || d > 1024) return fail(AL_EUNSUPPORTED, "head_dim must be a multiple of 8 in [8, 1024], got %d", d);
+  RotaryParams p = {};
+  int rc = rot_table(table, table_rows, rot, layout, d, &p.rt);
+  if (rc) return rc;
+  if (B == 0 || T == 0) return AL_OK;
+  if (!q || !q_strides || !q_out || (Hk > 0 && (!k || !k_strides || !k_out))) return fail(AL_EINVAL, "null pointer argument");
+  if (positions && !pos_strides) return fail(AL_EINVAL, "positions given without strides");
+  if (!rows_aligned(q, q_strides, 3, dtype) || !aligned16(q_out) ||
+      (Hk > 0 && (!rows_aligned(k, k_strides, 3, dtype) || !aligned16(k_out))))
+    return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
+  DeviceInfo* di = nullptr;
+  if ((rc = device_info(&di))) return rc;
+  p.q.x = q; p.q.sb = q_strides[0]; p.q.sh = q_strides[1]; p.q.st = q_strides[2]; p.q.H = Hq; p.q.out = q_out;
+  if (Hk > 0) { p.k.x = k; p.k.sb = k_strides[0]; p.k.sh = k_strides[1]; p.k.st = k_strides[2]; p.k.H = Hk; p.k.out = k_out; }
+  if (positions) {
+    p.pos = reinterpret_cast<const long long*>(positions);
+    p.pos_sb = pos_strides[0]; p.pos_st = pos_strides[1];
+  }
+  p.start = start; p.B = B; p.T = T; p.d = d; p.sgn = inverse ? -1.0f : 1.0f; p.err = di->err;
+  const long long threads = (long long)B * T * (d / 8), heads = Hq + Hk;
+  const long long blocks = (threads + 255) / 256;
+  if (blocks > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many tokens");
+  // heads per thread: one while the launch does not fill the GPU, then as many as keep it filled (up to 8)
+  p.hpt = 1;
+  while (p.hpt < 8 && blocks * ((heads + 2 * p.hpt - 1) / (2 * p.hpt)) >= 8LL * di->sms) p.hpt *= 2;
+  const dim3 grid((unsigned)blocks, (unsigned)((heads + p.hpt - 1) / p.hpt));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == AL_F32) rotary_kernel<float><<<grid, 256, 0, st>>>(p);
+  else rotary_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  return plain_launch_check("rotary_kernel");
+}
+
+int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const int* lengths, int length,
+                 const void* k_new, const int64_t* k_strides, const void* v_new, const int64_t* v_strides, int dtype,
+                 const float* table, int table_rows, int rot, int layout, const void* q, const int64_t* q_strides, int h,
+                 void* q_out, int B, int G, int T, int C, int d, void* stream) {
+  if (!dtype_ok(dtype)) return fail(AL_EINVAL, "unknown dtype code");
+  int rc = q8_shape(B, G, C, d, k_codes, v_codes, k_exp, v_exp);
+  if (rc) return rc;
+  if (T < 0) return fail(AL_EINVAL, "T must not be negative, got %d", T);
+  if (!lengths && (length < T || length > C))
+    return fail(AL_EINVAL, "positions [%d, %d) do not fit capacity %d", length - T, length, C);
+  Q8AppendParams p = {};
+  if (table || q) {
+    if ((rc = rot_table(table, table_rows, rot, layout, d, &p.rt))) return rc;
+    if (!lengths && length > table_rows)
+      return fail(AL_EINVAL, "positions up to %d exceed the rotary table's %d rows", length - 1, table_rows);
+  }
+  if (B == 0 || T == 0) return AL_OK;
+  if (!k_new || !v_new || !k_strides || !v_strides) return fail(AL_EINVAL, "null pointer argument");
+  if (!rows_aligned(k_new, k_strides, 3, dtype) || !rows_aligned(v_new, v_strides, 3, dtype))
+    return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
+  if (q) {
+    if (h < 1 || !q_strides || !q_out) return fail(AL_EINVAL, "q given without heads, strides or an output");
+    if (!rows_aligned(q, q_strides, 4, dtype) || !aligned16(q_out)) return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
+    if ((long long)G * h * T > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query rows per request");
+  }
+  DeviceInfo* di = nullptr;
+  if ((rc = device_info(&di))) return rc;
+  p.codes[0] = static_cast<uint8_t*>(k_codes); p.codes[1] = static_cast<uint8_t*>(v_codes);
+  p.exps[0] = static_cast<signed char*>(k_exp); p.exps[1] = static_cast<signed char*>(v_exp);
+  p.x[0] = k_new; p.x[1] = v_new;
+  p.sb[0] = k_strides[0]; p.sg[0] = k_strides[1]; p.st[0] = k_strides[2];
+  p.sb[1] = v_strides[0]; p.sg[1] = v_strides[1]; p.st[1] = v_strides[2];
+  p.len.per_batch = lengths; p.len.all = length;
+  p.B = B; p.G = G; p.T = T; p.C = C; p.NB = q8_blocks(C);
+  p.touched = std::min((T + kQ8Block - 2) / kQ8Block + 1, p.NB);
+  p.err = di->err;
+  const long long kv = 2LL * B * G * p.touched;
+  long long qc = 0;
+  if (q) {
+    p.q = q; p.q_sb = q_strides[0]; p.q_sg = q_strides[1]; p.q_sh = q_strides[2]; p.q_st = q_strides[3];
+    p.h = h; p.q_out = q_out;
+    qc = ((long long)B * G * h * T * 16 + kQ8AppendThreads - 1) / kQ8AppendThreads;
+  }
+  if (kv + qc > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many rows for one call");
+  p.kv_ctas = (int)kv;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)(kv + qc);
+  if (dtype == AL_F32) q8_append_kernel<float><<<grid, kQ8AppendThreads, 0, st>>>(p);
+  else q8_append_kernel<__nv_bfloat16><<<grid, kQ8AppendThreads, 0, st>>>(p);
+  return plain_launch_check("q8_append_kernel");
+}
+
+int al_read_q8(const void* k_codes, const void* v_codes, const void* k_exp, const void* v_exp, int B, int G, int C, int d,
+               int lo, int hi, int out_dtype, void* k_out, void* v_out, void* stream) {
+  if (!dtype_ok(out_dtype)) return fail(AL_EINVAL, "unknown dtype code");
+  int rc = q8_shape(B, G, C, d, k_codes, v_codes, k_exp, v_exp);
+  if (rc) return rc;
+  if (!(0 <= lo && lo <= hi && hi <= C)) return fail(AL_EINVAL, "need 0 <= lo <= hi <= C, got lo=%d hi=%d C=%d", lo, hi, C);
+  if (B == 0 || lo == hi) return AL_OK;
+  if (!k_out || !v_out) return fail(AL_EINVAL, "null output pointer");
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(AL_EUNSUPPORTED, "outputs must start on 16-byte boundaries");
+  Q8ReadParams p = {};
+  p.codes[0] = static_cast<const uint8_t*>(k_codes); p.codes[1] = static_cast<const uint8_t*>(v_codes);
+  p.exps[0] = static_cast<const signed char*>(k_exp); p.exps[1] = static_cast<const signed char*>(v_exp);
+  p.out[0] = k_out; p.out[1] = v_out;
+  p.C = C; p.NB = q8_blocks(C); p.lo = lo; p.n = hi - lo; p.rows = (long long)B * G * p.n;
+  const long long blocks = (p.rows * (kHeadDim / (16 / esize(out_dtype))) + 255) / 256;
+  if (blocks > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many rows for one call");
+  const dim3 grid((unsigned)blocks, 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (out_dtype == AL_F32) q8_read_kernel<float><<<grid, 256, 0, st>>>(p);
+  else q8_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  return plain_launch_check("q8_read_kernel");
+}
+
+int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int sinks, int max_length, size_t* bytes) {
+  if (!bytes) return fail(AL_EINVAL, "null bytes");
+  *bytes = 0;
+  if (B < 0 || G <= 0 || C <= 0) return fail(AL_EINVAL, "G and C must be positive and B not negative");
+  int rc = q8_attend_check(B, G, h, T, C, window, sinks);
+  if (rc) return rc;
+  if (B == 0 || T == 0) return AL_OK;
+  DeviceInfo* di = nullptr;
+  if ((rc = device_info(&di))) return rc;
+  Q8Plan pl;
+  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, di->sms, &pl))) return rc;
+  *bytes = pl.bytes;
+  return AL_OK;
+}
+
+int al_attend_q8(const void* q, const int64_t* q_strides, int dtype, const void* k_codes, const void* v_codes,
+                 const void* k_exp, const void* v_exp, const int* lengths, int length, int B, int G, int h, int T, int C,
+                 int d, int window, int sinks, float scale, int max_length, void* out, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  if (!dtype_ok(dtype)) return fail(AL_EINVAL, "unknown dtype code");
+  int rc = q8_shape(B, G, C, d, k_codes, v_codes, k_exp, v_exp);
+  if (rc) return rc;
+  if ((rc = q8_attend_check(B, G, h, T, C, window, sinks))) return rc;
+  if (!lengths && (length < 0 || length > C)) return fail(AL_EINVAL, "length=%d must be in [0, capacity=%d]", length, C);
+  if (!(scale == scale) || scale > 3.0e38f || scale < -3.0e38f) return fail(AL_EINVAL, "scale must be finite");
+  if (B == 0 || T == 0) return AL_OK;
+  if (!q || !q_strides || !out) return fail(AL_EINVAL, "null pointer argument");
+  if (!rows_aligned(q, q_strides, 4, dtype) || !aligned16(out)) return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
+  DeviceInfo* di = nullptr;
+  if ((rc = device_info(&di))) return rc;
+  Q8Plan pl;
+  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, di->sms, &pl))) return rc;
+  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)))
+    return fail(AL_EINVAL, "this call needs a 16-byte aligned workspace of %zu bytes, got %zu", pl.bytes, workspace_bytes);
+  Q8AttendParams p = {};
+  p.q = q; p.q_sb = q_strides[0]; p.q_sg = q_strides[1]; p.q_sh = q_strides[2]; p.q_st = q_strides[3];
+  p.kc = static_cast<const uint8_t*>(k_codes); p.vc = static_cast<const uint8_t*>(v_codes);
+  p.ke = static_cast<const signed char*>(k_exp); p.ve = static_cast<const signed char*>(v_exp);
+  p.len.per_batch = lengths; p.len.all = length;
+  p.B = B; p.G = G; p.h = h; p.T = T; p.C = C; p.NB = q8_blocks(C);
+  p.window = window; p.sinks = window > 0 ? sinks : 0;
+  p.scale = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
+  p.qsign = scale < 0 ? -1.0f : 1.0f;
+  p.out = out; p.nsplit = pl.nsplit; p.row_tiles = pl.row_tiles; p.err = di->err;
+  if (pl.bytes > 0) {
+    p.part = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.ml_off);
+  }
+  return dtype == AL_F32 ? q8_launch_attend<float>(p, pl, stream) : q8_launch_attend<__nv_bfloat16>(p, pl, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,419 @@
+// Attention of a few query columns (a decode step: T * h columns per KV group, T usually 1) over the 8-bit cache, with
+// an optional sliding window and first tokens (sinks) that stay visible.
+//
+// A query at position p sees the tokens j <= p with window = 0, or j > p - window, or j < sinks. A CTA holds 8 columns
+// (query, head) of one (batch, group); its warps walk steps of 32 tokens and every warp keeps its own online softmax,
+// so no warp waits for another until the end. Per step a warp reads the 32 rows of K and V straight from global memory
+// into the registers of the tensor-core fragments (each row is 128 bytes, read as full lines): both contractions may
+// permute their summed index freely, so a thread's 16 contiguous bytes serve as the operand without a pass through
+// shared memory. K and V codes become f16 exactly; q and the softmax weights are split into two f16 terms that occupy
+// the two halves of the MMA's 16 rows (rows 0-7 high, 8-15 low), so 8 columns with about 21 bits each cost the same
+// MMAs as 16 columns with 11. The block's exponents enter as 2^(ek) on the scores and as an addend ev inside the
+// weights' exponent: weights are w = 2^(s + ev - m) with the running maximum m over s + ev, the output sums w * code,
+// and the denominator sums w * 2^-ev.
+//
+// Bound: HBM reads of 256 bytes per visible token and group. The work of a segment is split over a cluster of CTAs
+// whose partial (m, l, O) are merged through distributed shared memory, so one launch does the whole step.
+#pragma once
+#include <cuda_fp16.h>
+#include "al_q8.cuh"
+
+namespace al {
+
+constexpr int kQdWarps = 4;
+constexpr int kQdThreads = 32 * kQdWarps;
+constexpr int kQdCols = 8;                 // columns (query, head) per CTA
+constexpr int kQ8TokenCols = 16;          // up to this many columns per group take this kernel, more the prompt kernel
+constexpr int kQdStep = 32;                // tokens per warp step (half a block: one exponent each for K and V)
+constexpr float kQdBias = 10.0f;           // weights run up to 2^10, so f16's normal range starts 2^-24 below the largest
+
+struct Q8AttendParams {
+  const void* q;                           // [B,G,h,T,128] (strides)
+  long long q_sb, q_sg, q_sh, q_st;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const signed char* ke;
+  const signed char* ve;
+  Q8Lengths len;
+  int B, G, h, T, C, NB;
+  int window, sinks;                       // window 0: every earlier token; sinks counts only with a window
+  float scale;                             // |softmax scale| * log2 e; its sign is folded into q
+  float qsign;
+  void* out;                               // [B,G,h,T,128] contiguous
+  // tensor-core kernel for prompts: split of the key tiles and its partial results
+  int nsplit, row_tiles;
+  float* part;                             // [nsplit][B*G][R][128] unnormalised O, R = T * h
+  float* part_ml;                          // [nsplit][B*G][R][2]
+  unsigned* err;
+};
+
+// What rows with positions [plo, phi] can see, as steps of `unit` tokens: `ns` steps from token 0 (the sinks), then
+// steps from `first` to the one that holds phi.
+struct Q8Range {
+  int ns, first, total;
+};
+__device__ __forceinline__ Q8Range q8_range(int plo, int phi, int window, int sinks, int unit) {
+  Q8Range r = {0, 0, 0};
+  if (phi < 0) return r;
+  if (window > 0) {
+    const int w0 = max(plo - window + 1, 0);
+    r.ns = (min(sinks, w0) + unit - 1) / unit;
+    r.first = max(w0 / unit, r.ns);
+  }
+  r.total = r.ns + max(phi / unit + 1 - r.first, 0);
+  return r;
+}
+__device__ __forceinline__ bool q8_sees(int p, int j, int window, int sinks) {
+  return j <= p && (window == 0 || j > p - window || j < sinks);
+}
+
+__device__ __forceinline__ float q8_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t q8_pack_half2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// D += A (16x16 f16, row) * B (16x8 f16, col) with fp32 accumulate.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Any e4m3 NaN code (0x7f or 0xff) among the 4 bytes of w: non-zero.
+__device__ __forceinline__ uint32_t q8_nan_mask(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// The codes of w with NaN replaced by zero.
+__device__ __forceinline__ uint32_t q8_drop_nan(uint32_t w) { return w & ~((q8_nan_mask(w) >> 7) * 0xffu); }
+
+// Power of two that brings a row's largest magnitude (its bits, finite) into [2^13, 2^14): the exponent eq with
+// q = (q 2^-eq) 2^eq. A maximum that is zero,
+// subnormal or non-finite gives 0 (a NaN or infinity then makes the row's output NaN).
+__device__ __forceinline__ int q8_row_exponent(uint32_t amax_bits) {
+  const int E = (int)(amax_bits >> 23);
+  return E == 0 || E == 255 ? 0 : max(E - 127 - 13, -126);
+}
+
+// The weights of a block whose V exponent lies far below others can leave fp32's range although the block counts in the
+// denominator (w = 2^(s + ev - m) with m set by a loud block): beyond this distance the denominator's terms 2^(s - m)
+// are taken by their own exponentials. At 90 the terms that fast sums lose are below 2^-36 of the denominator.
+constexpr int kQ8FarExp = 90;
+// x * 2^d for d <= 0, in two steps: 2^d alone may underflow where the product does not. d = -inf gives 0 (x finite).
+__device__ __forceinline__ float q8_rescale(float x, float d) {
+  const float a = q8_ex2(0.5f * d);
+  return x * a * a;
+}
+
+// Merging partials (m, l, O): the weight of one with maximum m under the common maximum M, and its share of the
+// denominator. An empty partial has m = -inf and l = 0; one whose every score was NaN has m = -inf and l NaN.
+__device__ __forceinline__ float q8_merge_weight(float l, float m, float M) {
+  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : q8_ex2(m - M);
+}
+__device__ __forceinline__ float q8_merge_l(float l, float m, float M) { return m == -INFINITY ? l : q8_rescale(l, m - M); }
+
+// Raw score -> log2 units for a block: a row's factor times 2^ek, kept positive and finite so that a hidden score
+// (-inf) stays -inf.
+__device__ __forceinline__ float q8_factor(float f_row, int ek) {
+  return fminf(fmaxf(f_row * q8_exp2i(ek), 1.17549435e-38f), 3.0e38f);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8AttendParams p) {
+  __shared__ __align__(16) float s_o[kQdWarps][kQdCols][kHeadDim];
+  __shared__ float s_m[kQdWarps][kQdCols], s_l[kQdWarps][kQdCols];
+  __shared__ float s_cm[kQdCols], s_cl[kQdCols];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+  const int bg = blockIdx.y, b = bg / p.G, g = bg - b * p.G;
+  const int cs = gridDim.x, rank = blockIdx.x;
+  const int R = p.h * p.T;
+  int n = q8_length(p.len, b);
+  if (n < 0 || n > p.C) {
+    if (tid == 0) atomicOr(p.err, kErrQ8Range);
+    n = max(0, min(n, p.C));
+  }
+  const int col0 = blockIdx.z * kQdCols;
+  const int col_last = min(col0 + kQdCols, R) - 1;
+  const int mycol = min(col0 + g8, R - 1);               // columns past the end repeat the last one and are not stored
+  const int myp = n - p.T + mycol / p.h;                 // this thread's column: position
+  const int plo = n - p.T + col0 / p.h, phi = n - p.T + col_last / p.h;
+  const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQdStep);
+
+  // q fragments: k-slots (2t, 2t+1 | 2t+8, 2t+9) of MMA ks hold dimensions 4 ks .. 4 ks + 3 of the thread's 16-byte
+  // pieces [16 t, 16 t + 16) (ks < 4) and [64 + 16 t, ...) (ks >= 4)
+  uint32_t qa[8][4];
+  float f_row;                                           // 2^eq * scale: raw score -> log2 units (before 2^ek)
+  {
+    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + (mycol % p.h) * p.q_sh + (mycol / p.h) * p.q_st;
+    float x[32];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float y[8];
+        q8_load8(src + 64 * half + 16 * t4 + 8 * i, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[16 * half + 8 * i + j] = y[j] * p.qsign;
+      }
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int eq = q8_row_exponent(amax);
+    const float inv = q8_exp2i(-eq);
+    f_row = p.scale * q8_exp2i(eq);
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      float hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float y = x[4 * ks + j] * inv;
+        hi[j] = __half2float(__float2half_rn(y));
+        lo[j] = y - hi[j];
+      }
+      qa[ks][0] = q8_pack_half2(hi[0], hi[1]); qa[ks][2] = q8_pack_half2(hi[2], hi[3]);
+      qa[ks][1] = q8_pack_half2(lo[0], lo[1]); qa[ks][3] = q8_pack_half2(lo[2], lo[3]);
+    }
+  }
+
+  float o[16][4];                                        // O: rows g8 (high weights) and g8 + 8 (low), n-tile j
+#pragma unroll
+  for (int j = 0; j < 16; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f; }
+  float m = -INFINITY, l = 0.0f;
+  int ev_top = -128;                                     // largest V exponent met so far
+
+  const uint8_t* kbase = p.kc + (long long)bg * p.C * kHeadDim;
+  const uint8_t* vbase = p.vc + (long long)bg * p.C * kHeadDim;
+  const signed char* keb = p.ke + (long long)bg * p.NB;
+  const signed char* veb = p.ve + (long long)bg * p.NB;
+
+  const int W = cs * kQdWarps;
+  int step = rank * kQdWarps + warp;
+  uint4 kr[8], vr[8];
+  int ek = 0, ev = 0;
+  auto step_token = [&](int s) { return (s < rg.ns ? s : rg.first + (s - rg.ns)) * kQdStep; };
+  auto load_k = [&](int j0) {
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt) {
+      const int j = j0 + 8 * nt + g8;
+      const uint8_t* r = kbase + (long long)j * kHeadDim + 16 * t4;
+      if (j < n) {
+        kr[2 * nt] = ldg_stream16(r);
+        kr[2 * nt + 1] = ldg_stream16(r + 64);
+      } else {
+        kr[2 * nt] = kr[2 * nt + 1] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  auto load_v = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = j0 + 16 * (i >> 2) + 8 * ((i >> 1) & 1) + 2 * t4 + (i & 1);
+      vr[i] = j < n ? ldg_stream16(vbase + (long long)j * kHeadDim + 16 * g8) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  int j0 = 0;
+  if (step < rg.total) {
+    j0 = step_token(step);
+    load_k(j0);
+    load_v(j0);
+    ek = keb[j0 / kQ8Block];
+    ev = veb[j0 / kQ8Block];
+  }
+#pragma unroll 1
+  for (; step < rg.total; step += W) {
+    const int nxt = step + W;
+    const bool more = nxt < rg.total;
+    const int j1 = more ? step_token(nxt) : 0;
+    // scores: 4 n-tiles of 8 tokens
+    float s[8];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt) {
+      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint32_t w[8] = {kr[2 * nt].x, kr[2 * nt].y, kr[2 * nt].z, kr[2 * nt].w,
+                             kr[2 * nt + 1].x, kr[2 * nt + 1].y, kr[2 * nt + 1].z, kr[2 * nt + 1].w};
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+        mma_f16_16816(acc, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], q8_decode_lo(w[ks]), q8_decode_hi(w[ks]));
+      s[2 * nt] = acc[0] + acc[2];
+      s[2 * nt + 1] = acc[1] + acc[3];
+    }
+    const float f = q8_factor(f_row, ek), fev = (float)ev, inv_ev = q8_exp2i(-ev);
+    const int ev_now = ev;
+    if (more) {
+      load_k(j1);
+      ek = keb[j1 / kQ8Block];
+      ev = veb[j1 / kQ8Block];
+    }
+    // a step is whole when every column sees all of it
+    const bool whole = j0 + kQdStep - 1 <= plo && (p.window == 0 || j0 > phi - p.window || j0 + kQdStep <= p.sinks);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] *= f;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + 8 * (i >> 1) + 2 * t4 + (i & 1);
+        if (!q8_sees(myp, j, p.window, p.sinks)) s[i] = -INFINITY;
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float mn = fmaxf(m, mx + fev);
+    if (__any_sync(0xffffffffu, mn > m)) {
+      const float alpha = mn > m ? q8_ex2(m - mn) : 1.0f;   // m = -inf: 0
+      l = mn > m ? q8_rescale(l, m - mn) : l;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) { o[j][0] *= alpha; o[j][1] *= alpha; o[j][2] *= alpha; o[j][3] *= alpha; }
+      m = mn;
+    }
+    const float ref = (m == -INFINITY ? 0.0f : m) - kQdBias - fev;
+    float sum = 0.0f;
+    uint32_t pa[2][4];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {                         // n-tile 2 ks + u: k-slots 2t, 2t+1 (u = 0) or 2t+8, 2t+9
+        const float w0 = q8_ex2(s[4 * ks + 2 * u] - ref), w1 = q8_ex2(s[4 * ks + 2 * u + 1] - ref);
+        sum += w0 + w1;
+        const float h0 = __half2float(__float2half_rn(w0)), h1 = __half2float(__float2half_rn(w1));
+        pa[ks][2 * u] = q8_pack_half2(h0, h1);
+        pa[ks][2 * u + 1] = q8_pack_half2(w0 - h0, w1 - h1);
+      }
+    ev_top = max(ev_top, ev_now);
+    if (ev_top - ev_now > kQ8FarExp) {
+      sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += q8_ex2(s[i] - (ref + fev));
+      l += sum;
+    } else {
+      l += sum * inv_ev;
+    }
+    // O += P V. Rows that no column sees become zero codes. A NaN code in a row that only some columns see must not
+    // reach the others (0 * NaN): such codes become zero too, and the columns that see them get their NaN here.
+    if (!whole) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + 16 * (i >> 2) + 8 * ((i >> 1) & 1) + 2 * t4 + (i & 1);
+        const bool none = j > phi || (p.window > 0 && j <= plo - p.window && j >= p.sinks);
+        if (none) vr[i] = make_uint4(0, 0, 0, 0);
+        bad |= q8_nan_mask(vr[i].x) | q8_nan_mask(vr[i].y) | q8_nan_mask(vr[i].z) | q8_nan_mask(vr[i].w);
+      }
+      if (plo != phi && __any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          vr[i].x = q8_drop_nan(vr[i].x); vr[i].y = q8_drop_nan(vr[i].y);
+          vr[i].z = q8_drop_nan(vr[i].z); vr[i].w = q8_drop_nan(vr[i].w);
+        }
+#pragma unroll 1
+        for (int j = j0; j < min(j0 + kQdStep, n); ++j) {
+          if (!q8_sees(myp, j, p.window, p.sinks)) continue;
+          const uint8_t* v = vbase + (long long)j * kHeadDim + 32 * t4;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            if ((v[d] & 0x7f) == 0x7f) o[d][0] = __uint_as_float(0x7fffffffu);
+            if ((v[16 + d] & 0x7f) == 0x7f) o[d][1] = __uint_as_float(0x7fffffffu);
+          }
+        }
+        __syncwarp();
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const uint4 a0 = vr[4 * ks], a1 = vr[4 * ks + 1], b0 = vr[4 * ks + 2], b1 = vr[4 * ks + 3];
+      const uint32_t x0[4] = {a0.x, a0.y, a0.z, a0.w}, x1[4] = {a1.x, a1.y, a1.z, a1.w};
+      const uint32_t y0[4] = {b0.x, b0.y, b0.z, b0.w}, y1[4] = {b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t xl = __byte_perm(x0[w], x1[w], 0x5140), xh = __byte_perm(x0[w], x1[w], 0x7362);
+        const uint32_t yl = __byte_perm(y0[w], y1[w], 0x5140), yh = __byte_perm(y0[w], y1[w], 0x7362);
+        mma_f16_16816(o[4 * w], pa[ks][0], pa[ks][1], pa[ks][2], pa[ks][3], q8_decode_lo(xl), q8_decode_lo(yl));
+        mma_f16_16816(o[4 * w + 1], pa[ks][0], pa[ks][1], pa[ks][2], pa[ks][3], q8_decode_hi(xl), q8_decode_hi(yl));
+        mma_f16_16816(o[4 * w + 2], pa[ks][0], pa[ks][1], pa[ks][2], pa[ks][3], q8_decode_lo(xh), q8_decode_lo(yh));
+        mma_f16_16816(o[4 * w + 3], pa[ks][0], pa[ks][1], pa[ks][2], pa[ks][3], q8_decode_hi(xh), q8_decode_hi(yh));
+      }
+    }
+    if (more) load_v(j1);
+    j0 = j1;
+  }
+
+  // the CTA's partial: thread holds column g8, dimensions 32 t + j (o[j][0] + o[j][2]) and 32 t + 16 + j
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+  for (int j = 0; j < 16; j += 4) {
+    *reinterpret_cast<float4*>(&s_o[warp][g8][32 * t4 + j]) =
+        make_float4(o[j][0] + o[j][2], o[j + 1][0] + o[j + 1][2], o[j + 2][0] + o[j + 2][2], o[j + 3][0] + o[j + 3][2]);
+    *reinterpret_cast<float4*>(&s_o[warp][g8][32 * t4 + 16 + j]) =
+        make_float4(o[j][1] + o[j][3], o[j + 1][1] + o[j + 1][3], o[j + 2][1] + o[j + 2][3], o[j + 3][1] + o[j + 3][3]);
+  }
+  if (t4 == 0) { s_m[warp][g8] = m; s_l[warp][g8] = l; }
+  __syncthreads();
+  // merge the warps into s_o[0]: thread d (0..127) takes dimension d of every column
+  {
+    float acc[kQdCols];
+#pragma unroll
+    for (int c = 0; c < kQdCols; ++c) {
+      float M = s_m[0][c];
+#pragma unroll
+      for (int w = 1; w < kQdWarps; ++w) M = fmaxf(M, s_m[w][c]);
+      float a = 0.0f, L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kQdWarps; ++w) {
+        const float e = q8_merge_weight(s_l[w][c], s_m[w][c], M);
+        a += e != 0.0f ? e * s_o[w][c][tid] : 0.0f;
+        L += q8_merge_l(s_l[w][c], s_m[w][c], M);
+      }
+      acc[c] = a;
+      if (tid == c) { s_cm[c] = M; s_cl[c] = L; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kQdCols; ++c) s_o[0][c][tid] = acc[c];
+  }
+  const int ncol = col_last - col0 + 1;
+  if (cs > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // rank r merges every cs-th (column, 4 dimensions) piece over the CTAs
+    for (int i = rank * kQdThreads + tid; i < ncol * (kHeadDim / 4); i += cs * kQdThreads) {
+      const int c = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4));
+      float M = -INFINITY;
+      for (int r = 0; r < cs; ++r) M = fmaxf(M, *cluster.map_shared_rank(&s_cm[c], r));
+      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float L = 0.0f;
+      for (int r = 0; r < cs; ++r) {
+        const float mr = *cluster.map_shared_rank(&s_cm[c], r), lr = *cluster.map_shared_rank(&s_cl[c], r);
+        const float e = q8_merge_weight(lr, mr, M);
+        L += q8_merge_l(lr, mr, M);
+        if (e == 0.0f) continue;
+        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s_o[0][c][d], r));
+        a.x += e * v.x; a.y += e * v.y; a.z += e * v.z; a.w += e * v.w;
+      }
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      const int cc = col0 + c, hd = cc % p.h, t = cc / p.h;
+      T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + hd) * p.T + t) * kHeadDim + d;
+      if (L == 0.0f) a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      dst[0] = fromf<T>(a.x * inv); dst[1] = fromf<T>(a.y * inv); dst[2] = fromf<T>(a.z * inv); dst[3] = fromf<T>(a.w * inv);
+    }
+    cluster.sync();                                       // peers' shared memory stays until every rank has read it
+  } else {
+    __syncthreads();
+    for (int i = tid; i < ncol * kHeadDim; i += kQdThreads) {
+      const int c = i / kHeadDim, d = i % kHeadDim;
+      const float L = s_cl[c];
+      const int cc = col0 + c, hd = cc % p.h, t = cc / p.h;
+      static_cast<T*>(p.out)[(((long long)bg * p.h + hd) * p.T + t) * kHeadDim + d] =
+          fromf<T>(L == 0.0f ? 0.0f : s_o[0][c][d] / L);
+    }
+  }
+}
+
+}  // namespace al

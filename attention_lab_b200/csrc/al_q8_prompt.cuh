@@ -1,0 +1,500 @@
+// Attention of a prompt chunk over the 8-bit cache on the fifth-generation tensor cores, causal, with an optional
+// sliding window and sinks (the rule of al_q8_decode.cuh).
+//
+// The T x h query rows of a KV group are one list (row r = t * h + head), so all heads of a group share every key tile.
+// A CTA takes 256 of them as two tiles of 128 rows (TMEM lanes) and walks the key tiles (128 tokens) that any of its
+// rows can see. Per key tile and query tile: S = Q K^T (tcgen05.mma, f16 operands from shared memory, fp32 in TMEM),
+// the softmax weights P go back into S's columns as f16, and O += P V (P from TMEM, V from shared memory). The two
+// query tiles alternate, so the tensor cores multiply for one while the other's weights are computed.
+//   warps 0-3, 4-7  one thread per query row: scores -> running maximum, weights, denominator; O is rescaled only when
+//                   a row's maximum grew by more than 2^8 (weights up to 2^14 fit f16)
+//   warps 8-11      read the codes from global memory, convert them to f16 (exact) and store them in the 128-byte
+//                   swizzled layout both contractions read; the next tile's codes are in registers meanwhile
+//   warp 12         issues the MMAs
+// 16-bit queries are one f16 operand (scaled by a power of two per row, exact). 32-bit queries and their weights are
+// split into two f16 terms (SPLIT): twice the MMAs, about 21 bits, single-buffered key tiles.
+//
+// V codes that are NaN would reach rows that do not see them (0 * NaN in the MMA): they are replaced by zero on the way
+// in, their tokens noted, and rows that do see one get their NaN in the epilogue.
+#pragma once
+#include "al_tcgen05.cuh"
+#include "al_q8_decode.cuh"
+
+namespace al {
+
+constexpr int kQpRows = 128;                           // query rows per tile
+constexpr int kQpKeys = 128;                           // tokens per key tile: two blocks of the cache
+constexpr int kQpThreads = 512;
+constexpr uint32_t kQpTile = kQpKeys * kHeadDim * 2;   // 32 KB: a tile of 128 x 128 f16, two 64-wide halves of 16 KB
+constexpr uint32_t kQpHalf = kQpTile / 2;
+constexpr size_t kQpSmem = 1024 + 6 * kQpTile;         // 2 Q + 2 K + 2 V tiles, or 4 Q (high, low) + K + V
+constexpr int kQpNanList = 64;
+constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8)
+// Registers a thread after the split: 2 x 128 softmax threads, 128 converting threads, the MMA warp's group.
+// 184 + 184 + 104 + 40 = 512 = 4 x the 128 of the launch.
+constexpr int kQpRegsSoftmax = 184, kQpRegsConvert = 104, kQpRegsMma = 40;
+
+// Instruction descriptors (kind::f16): fp32 accumulator, f16 operands, M = N = 128; Q K^T has both operands K-major,
+// P V has V N-major.
+constexpr uint32_t kQpIdescQK = (1u << 4) | ((uint32_t)(kQpKeys >> 3) << 17) | ((uint32_t)(kQpRows >> 4) << 24);
+constexpr uint32_t kQpIdescPV = kQpIdescQK | (1u << 16);
+
+__device__ __forceinline__ void qp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(kQpIdescQK), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void qp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(b), "r"(kQpIdescPV), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void qp_tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                 "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
+                 "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+                 "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+               : "memory");
+}
+__device__ __forceinline__ void qp_st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void qp_fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+// 16-byte chunk c (0..15, 8 f16 each) of row r in a 128-byte swizzled tile of two 64-wide halves.
+__device__ __forceinline__ uint32_t qp_chunk(uint32_t tile, int r, int c) {
+  return tile + (uint32_t)(c >> 3) * kQpHalf + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8AttendParams p) {
+  constexpr bool SPLIT = sizeof(T) == 4;
+  constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
+  constexpr int QP = SPLIT ? 2 : 1;                    // f16 terms per query row
+  extern __shared__ __align__(1024) unsigned char qp_raw[];
+  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2], s_pfull[2], s_ofull[2];
+  __shared__ uint32_t s_taddr;
+  __shared__ int s_nan_count, s_nan[kQpNanList];
+  __shared__ volatile int s_abort;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_addr(qp_raw) + 1023u) & ~1023u;
+  const uint32_t s_q = base, s_k = base + 2 * QP * kQpTile, s_v = s_k + NS * kQpTile;
+
+  // the longest row tiles first; all (batch, group) pairs of a row tile together
+  const int BG = p.B * p.G, R = p.h * p.T;
+  const int split = blockIdx.y;
+  const int tile = p.row_tiles - 1 - (int)(blockIdx.x / BG), bg = (int)(blockIdx.x % BG);
+  const int b = bg / p.G, g = bg - b * p.G;
+  int n = q8_length(p.len, b);
+  if (n < 0 || n > p.C) {
+    if (tid == 0) atomicOr(p.err, kErrQ8Range);
+    n = max(0, min(n, p.C));
+  }
+  const int r0 = tile * 2 * kQpRows;
+  const int ntile = r0 + kQpRows < R ? 2 : 1;
+  const int pbase = n - p.T;
+  const int plo = pbase + r0 / p.h, phi = pbase + min(r0 + 2 * kQpRows - 1, R - 1) / p.h;
+  const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQpKeys);
+  const int it0 = (int)((long long)rg.total * split / p.nsplit), it1 = (int)((long long)rg.total * (split + 1) / p.nsplit);
+  const int nt = it1 - it0;
+  auto tile_token = [&](int it) { return (it < rg.ns ? it : rg.first + (it - rg.ns)) * kQpKeys; };
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_qfull[i], kQpRows);
+      mbar_init(&s_sfull[i], 1);
+      mbar_init(&s_pfull[i], kQpRows);
+      mbar_init(&s_ofull[i], 1);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&s_kfull[i], 128); mbar_init(&s_kempty[i], 1);
+      mbar_init(&s_vfull[i], 128); mbar_init(&s_vempty[i], 1);
+    }
+    mbar_init_fence();
+    s_nan_count = 0;
+    s_abort = 0;
+  }
+  if (warp == 12) { tmem_alloc(&s_taddr, 512); tmem_relinquish(); }
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  const uint32_t tm = s_taddr;                          // S0 | S1 | O0 | O1, 128 columns each
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------------------------------------- query rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kQpRegsSoftmax));
+    const int qt = warp >> 2, row = tid & 127;
+    if (qt < ntile && nt > 0) {
+      const int r = min(r0 + qt * kQpRows + row, R - 1);
+      const int t = r / p.h, head = r - t * p.h, pos = pbase + t;
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t tS = tm + lanes + (uint32_t)qt * 128u, tO = tm + lanes + 256u + (uint32_t)qt * 128u;
+      float f_row;
+      {
+        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t * p.q_st;
+        uint32_t amax = 0;
+#pragma unroll 4
+        for (int c = 0; c < 16; ++c) {
+          float y[8];
+          q8_load8(src + 8 * c, y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(y[i]) & 0x7fffffffu);
+        }
+        const int eq = q8_row_exponent(amax);
+        const float inv = q8_exp2i(-eq) * p.qsign;
+        f_row = p.scale * q8_exp2i(eq);
+        const uint32_t qtile = s_q + (uint32_t)(qt * QP) * kQpTile;
+#pragma unroll 4
+        for (int c = 0; c < 16; ++c) {
+          float y[8];
+          q8_load8(src + 8 * c, y);
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float a = y[2 * i] * inv, d = y[2 * i + 1] * inv;
+            hi[i] = q8_pack_half2(a, d);
+            const float2 x = q8_half2_floats(hi[i]);
+            lo[i] = q8_pack_half2(a - x.x, d - x.y);
+          }
+          qp_st_shared16(qp_chunk(qtile, row, c), hi[0], hi[1], hi[2], hi[3]);
+          if (SPLIT) qp_st_shared16(qp_chunk(qtile + kQpTile, row, c), lo[0], lo[1], lo[2], lo[3]);
+        }
+        qp_fence_async();
+        pf_arrive(&s_qfull[qt]);
+      }
+      // positions of the warp's rows, for the test that a tile needs no mask
+      const int rw0 = r0 + qt * kQpRows + (warp & 3) * 32;
+      const int wlo = pbase + min(rw0, R - 1) / p.h, whi = pbase + min(rw0 + 31, R - 1) / p.h;
+      const signed char* keb = p.ke + (long long)bg * p.NB;
+      const signed char* veb = p.ve + (long long)bg * p.NB;
+      float m = -INFINITY, l = 0.0f;
+      int ev_top = -128;                               // largest V exponent met so far
+#pragma unroll 1
+      for (int it = 0; it < nt; ++it) {
+        const int j0 = tile_token(it0 + it), blk = j0 / kQ8Block, blk1 = min(blk + 1, p.NB - 1);
+        const int ek0 = keb[blk], ek1 = keb[blk1], ev0 = veb[blk], ev1 = veb[blk1];
+        pf_wait(&s_sfull[qt], (uint32_t)it & 1u, &s_abort, p.err);
+        tmem_fence_after_sync();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) pf_tmem_ld32(tS + 32u * (uint32_t)c, s[c]);
+        pf_tmem_wait(s[0]);
+#pragma unroll
+        for (int c = 1; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(s[c][i]));
+        const bool whole = j0 + kQpKeys - 1 <= wlo &&
+                           (p.window == 0 || j0 > whi - p.window || j0 + kQpKeys <= p.sinks);
+        if (!whole) {
+          const int last = pos - j0, left = p.window > 0 ? last - p.window : -1, sink = p.window > 0 ? p.sinks - j0 : 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int x = 32 * c + i;
+              if (!(x <= last && (x > left || x < sink))) s[c][i] = 0xff800000u;
+            }
+        }
+        const float f0 = q8_factor(f_row, ek0), f1 = q8_factor(f_row, ek1);
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float a = __uint_as_float(s[c][0]), d = __uint_as_float(s[c][1]);
+#pragma unroll
+          for (int i = 2; i < 32; i += 2) {
+            a = fmaxf(a, __uint_as_float(s[c][i]));
+            d = fmaxf(d, __uint_as_float(s[c][i + 1]));
+          }
+          mx[c] = fmaxf(a, d);
+        }
+        const float cand = fmaxf(fmaxf(mx[0], mx[1]) * f0 + (float)ev0, fmaxf(mx[2], mx[3]) * f1 + (float)ev1);
+        const bool grow = cand > m + kQpLazy;            // m = -inf: any visible score
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? q8_ex2(m - cand) : 1.0f;
+          if (grow) {
+            l = q8_rescale(l, m - cand);
+            m = cand;
+          }
+          if (it > 0) {
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tO + 16u * (uint32_t)c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                asm volatile("" : "+r"(o[i]));
+                o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              }
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) tmem_st2(tO + 16u * (uint32_t)c + (uint32_t)i, o[i], o[i + 1]);
+            }
+            tmem_wait_st();
+          }
+        }
+        const float mref = (m == -INFINITY ? 0.0f : m) - kQpBias;
+        ev_top = max(ev_top, max(ev0, ev1));
+        float sum[2];
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb) {                 // the tile's two blocks
+          const int ev = hb ? ev1 : ev0;
+          const float f = hb ? f1 : f0, add = (float)ev - mref;
+          float a0 = 0.0f, a1 = 0.0f, far = 0.0f;
+          if (ev_top - ev > kQ8FarExp) {                 // the denominator's terms on their own (see kQ8FarExp)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) far += q8_ex2(fmaf(__uint_as_float(s[2 * hb + c][i]), f, -mref));
+          }
+          uint32_t w[32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float x = q8_ex2(fmaf(__uint_as_float(s[2 * hb + c][i]), f, add));
+              const float y = q8_ex2(fmaf(__uint_as_float(s[2 * hb + c][i + 1]), f, add));
+              a0 += x;
+              a1 += y;
+              const uint32_t hw = q8_pack_half2(x, y);
+              w[16 * c + i / 2] = hw;
+              if (SPLIT) {
+                const float2 z = q8_half2_floats(hw);
+                s[2 * hb + c][i / 2] = q8_pack_half2(x - z.x, y - z.y);
+              }
+            }
+          sum[hb] = ev_top - ev > kQ8FarExp ? far : (a0 + a1) * q8_exp2i(-ev);
+          qp_tmem_st32(tS + 32u * (uint32_t)hb, w);
+          if (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { w[i] = s[2 * hb][i]; w[16 + i] = s[2 * hb + 1][i]; }
+            qp_tmem_st32(tS + 64u + 32u * (uint32_t)hb, w);
+          }
+        }
+        l += sum[0] + sum[1];
+        tmem_wait_st();
+        tmem_fence_before_sync();
+        pf_arrive(&s_pfull[qt]);
+      }
+      pf_wait(&s_ofull[qt], 0, &s_abort, p.err);
+      tmem_fence_after_sync();
+      const int rr = r0 + qt * kQpRows + row;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int bad = s_nan_count;
+      float* part = p.part ? p.part + (((long long)split * BG + bg) * R + rr) * kHeadDim : nullptr;
+      T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim;
+      const uint8_t* vbase = p.vc + (long long)bg * p.C * kHeadDim;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        pf_tmem_ld32(tO + 32u * (uint32_t)c, o);
+        pf_tmem_wait(o);
+        if (bad > 0) {
+          // tokens with a NaN code in V: the listed ones, or all of this CTA's when the list ran over
+          const int cnt = bad <= kQpNanList ? bad : nt * kQpKeys;
+          for (int i = 0; i < cnt; ++i) {
+            const int j = bad <= kQpNanList ? s_nan[i] : tile_token(it0 + i / kQpKeys) + i % kQpKeys;
+            if (j >= n || !q8_sees(pos, j, p.window, p.sinks)) continue;
+            const uint8_t* v = vbase + (long long)j * kHeadDim + 32 * c;
+#pragma unroll
+            for (int d = 0; d < 32; ++d)
+              if ((v[d] & 0x7f) == 0x7f) o[d] = 0x7fffffffu;
+          }
+        }
+        if (rr < R && part) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(part + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else if (rr < R) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = l == 0.0f ? 0.0f : __uint_as_float(o[i + k]) * inv;
+            q8_store8(dst + 32 * c + i, y);
+          }
+        }
+        __syncwarp();
+      }
+      if (part && rr < R) {
+        float* ml = p.part_ml + (((long long)split * BG + bg) * R + rr) * 2;
+        ml[0] = m;
+        ml[1] = l;
+      }
+    } else if (nt == 0) {
+      // nothing to see for any row of this CTA: zeros, or an empty partial
+      const int rr = r0 + qt * kQpRows + row;
+      if (rr < R) {
+        if (p.part) {
+          float* ml = p.part_ml + (((long long)split * BG + bg) * R + rr) * 2;
+          ml[0] = -INFINITY;
+          ml[1] = 0.0f;
+        } else {
+          const int t = rr / p.h, head = rr - t * p.h;
+          T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim;
+          const float z[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+          for (int c = 0; c < 16; ++c) q8_store8(dst + 8 * c, z);
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------------------------------------- codes -> f16 tiles
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsConvert));
+    const int rw = (warp - 8) * 4 + (lane >> 3), c8 = lane & 7;     // row within a group of 16, 16-code piece of the row
+    const long long off = (long long)bg * p.C * kHeadDim + 16 * c8;
+    uint4 kr[8], vr[8];
+    auto load = [&](const uint8_t* codes, int it, uint4 (&x)[8]) {
+      const int j0 = tile_token(it0 + it);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + 16 * i + rw;
+        x[i] = j < n ? __ldg(reinterpret_cast<const uint4*>(codes + off + (long long)j * kHeadDim)) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto store = [&](uint32_t dst, const uint4 (&x)[8]) {
+      // pieces 4-7 of a row (the second half) write their two chunks in the other order: no two lanes of a quarter
+      // warp share a bank
+      const int first = c8 >> 2;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 16 * i + rw;
+        const uint32_t lo[4] = {q8_decode_lo(x[i].x), q8_decode_hi(x[i].x), q8_decode_lo(x[i].y), q8_decode_hi(x[i].y)};
+        const uint32_t hi[4] = {q8_decode_lo(x[i].z), q8_decode_hi(x[i].z), q8_decode_lo(x[i].w), q8_decode_hi(x[i].w)};
+        const uint32_t a0 = qp_chunk(dst, r, 2 * c8), a1 = qp_chunk(dst, r, 2 * c8 + 1);
+        if (first) {
+          qp_st_shared16(a1, hi[0], hi[1], hi[2], hi[3]);
+          qp_st_shared16(a0, lo[0], lo[1], lo[2], lo[3]);
+        } else {
+          qp_st_shared16(a0, lo[0], lo[1], lo[2], lo[3]);
+          qp_st_shared16(a1, hi[0], hi[1], hi[2], hi[3]);
+        }
+      }
+    };
+    if (nt > 0) { load(p.kc, 0, kr); load(p.vc, 0, vr); }
+#pragma unroll 1
+    for (int it = 0; it < nt; ++it) {
+      const int st = it % NS;
+      const uint32_t par = (uint32_t)(it / NS) & 1u;
+      pf_wait(&s_kempty[st], par ^ 1u, &s_abort, p.err);
+      store(s_k + (uint32_t)st * kQpTile, kr);
+      qp_fence_async();
+      pf_arrive(&s_kfull[st]);
+      if (it + 1 < nt) load(p.kc, it + 1, kr);
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bad |= q8_nan_mask(vr[i].x) | q8_nan_mask(vr[i].y) | q8_nan_mask(vr[i].z) | q8_nan_mask(vr[i].w);
+      if (bad) {
+        const int j0 = tile_token(it0 + it);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+          uint32_t any = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            any |= q8_nan_mask(w[k]);
+            w[k] = q8_drop_nan(w[k]);
+          }
+          vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          if (any) {
+            const int at = atomicAdd(&s_nan_count, 1);
+            if (at < kQpNanList) s_nan[at] = j0 + 16 * i + rw;
+          }
+        }
+      }
+      pf_wait(&s_vempty[st], par ^ 1u, &s_abort, p.err);
+      store(s_v + (uint32_t)st * kQpTile, vr);
+      qp_fence_async();
+      pf_arrive(&s_vfull[st]);
+      if (it + 1 < nt) load(p.vc, it + 1, vr);
+    }
+  } else {
+    // ---------------------------------------------------------------------------------------------- MMAs
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsMma));
+    if (warp == 12 && lane == 0 && nt > 0) {
+      auto scores = [&](int qt, int st) {               // S = Q K^T
+#pragma unroll
+        for (int term = 0; term < QP; ++term)
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t o = (uint32_t)(ks >> 2) * kQpHalf + (uint32_t)(ks & 3) * 32u;
+            qp_mma_ss(tm + (uint32_t)qt * 128u, pf_sdesc(s_q + (uint32_t)(qt * QP + term) * kQpTile + o, 16, 1024, 2),
+                      pf_sdesc(s_k + (uint32_t)st * kQpTile + o, 16, 1024, 2), (term | ks) > 0 ? 1u : 0u);
+          }
+      };
+      auto values = [&](int qt, int st, bool first) {   // O += P V
+#pragma unroll
+        for (int term = 0; term < QP; ++term)
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            qp_mma_ts(tm + 256u + (uint32_t)qt * 128u, tm + (uint32_t)qt * 128u + (uint32_t)term * 64u + (uint32_t)ks * 8u,
+                      pf_sdesc(s_v + (uint32_t)st * kQpTile + (uint32_t)ks * 2048u, kQpHalf, 1024, 2),
+                      (first && term == 0 && ks == 0) ? 0u : 1u);
+      };
+      pf_wait(&s_kfull[0], 0, &s_abort, p.err);
+      for (int qt = 0; qt < ntile; ++qt) {
+        pf_wait(&s_qfull[qt], 0, &s_abort, p.err);
+        tmem_fence_after_sync();
+        scores(qt, 0);
+        pf_commit(&s_sfull[qt]);
+      }
+      pf_commit(&s_kempty[0]);
+#pragma unroll 1
+      for (int it = 0; it < nt; ++it) {
+        const int st = it % NS, st1 = (it + 1) % NS;
+        const bool more = it + 1 < nt;
+        pf_wait(&s_vfull[st], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
+        for (int qt = 0; qt < ntile; ++qt) {
+          pf_wait(&s_pfull[qt], (uint32_t)it & 1u, &s_abort, p.err);
+          tmem_fence_after_sync();
+          values(qt, st, it == 0);
+          if (qt == ntile - 1) pf_commit(&s_vempty[st]);
+          if (more) {
+            // S's columns hold P until the P V above has read them: MMAs of one thread run in order
+            if (qt == 0) pf_wait(&s_kfull[st1], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
+            tmem_fence_after_sync();
+            scores(qt, st1);
+            pf_commit(&s_sfull[qt]);
+            if (qt == ntile - 1) pf_commit(&s_kempty[st1]);
+          } else {
+            pf_commit(&s_ofull[qt]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  if (warp == 12) tmem_dealloc(tm, 512);
+}
+
+// Merge of the key splits: one warp per row, a lane per 4 dimensions.
+template <typename T>
+__global__ void __launch_bounds__(256) q8_merge_kernel(const Q8AttendParams p) {
+  const int BG = p.B * p.G, R = p.h * p.T;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (long long)BG * R;
+  if (row >= rows) return;
+  const int d = 4 * (threadIdx.x & 31);
+  float M = -INFINITY;
+  for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, p.part_ml[((long long)s * rows + row) * 2]);
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float L = 0.0f;
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((long long)s * rows + row) * 2);
+    const float e = q8_merge_weight(ml.y, ml.x, M);
+    L += q8_merge_l(ml.y, ml.x, M);
+    if (e == 0.0f) continue;
+    const float4 v = *reinterpret_cast<const float4*>(p.part + ((long long)s * rows + row) * kHeadDim + d);
+    a.x += e * v.x; a.y += e * v.y; a.z += e * v.z; a.w += e * v.w;
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  const int bg = (int)(row / R), r = (int)(row - (long long)bg * R), t = r / p.h, head = r - t * p.h;
+  T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim + d;
+  const float y[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dst[i] = fromf<T>(y[i]);
+}
+
+}  // namespace al

@@ -38,7 +38,9 @@ const char* al_last_error(void);
 int al_version(void);
 
 /* Synchronises the current device, then returns (and clears) the error bits kernels raised since the last call:
- * 1 = a row id outside [0, B*G*C) was skipped (the row is not read). */
+ * 1 = a row id outside [0, B*G*C) was skipped (the row is not read), 2 = a bounded wait gave up (that launch's results
+ * are invalid), 4 = an 8-bit cache call met a length outside [0, C] (clamped) or a position past its rotary table (that
+ * row is written as zeros). */
 int al_device_status(unsigned* error_bits);
 
 /* a8: one layer's sparse decode step, fused into one launch (replaces attention-lab
@@ -201,6 +203,49 @@ int al_context_threshold_noalloc(const uint64_t* const* rank_keys, int world, in
 int al_prefill_score_topk(const void* u, long long u_sh, long long u_st, const void* zT, long long z_sh, long long z_ld,
                           int H, int T, int C, int r, int q_pos0, int k, int kcap, int* idx_out, float* scores_out,
                           void* stream);
+
+/* ---- 8-bit cache (no reference counterpart): K and V of one layer as e4m3 codes [B,G,C,128] (contiguous) and one int8
+ * exponent per block of 64 tokens of each (batch, group), [B,G,ceil(C/64)] (contiguous): value = code * 2^exponent.
+ * Lengths count the tokens of a request after the step's T rows: row t of T sits at position length - T + t, and rows at
+ * negative positions are padding. `lengths` [B] int32 on the device gives one per request; when NULL, `length` is every
+ * request's. A device length outside [0, C] is clamped and sets error bit 4. Row starts (pointer and strides) must be
+ * 16-byte aligned. */
+#define AL_ROT_HALF 0          /* pairs (i, i + rot/2) */
+#define AL_ROT_INTERLEAVED 1   /* pairs (2i, 2i + 1) */
+
+/* Rotary positions: q [B,Hq,T,d] and, with Hk > 0, k [B,Hk,T,d] (strides for B, H, T) to contiguous q_out, k_out of the
+ *   same dtype. table [table_rows, rot] fp32: cos then sin of every pair, scaled as the caller likes; the pair (a, b)
+ *   becomes (a c - b s, b c + a s), with -s when `inverse` (the gradient); dimensions from rot on are copied.
+ *   positions [B,T] int64 (strides for B, T) or NULL: start + t. A negative position gives zeros; one past the table gives
+ *   zeros and error bit 4. */
+int al_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, const int64_t* k_strides, int Hk, int dtype,
+              const float* table, int table_rows, int rot, int layout, const int64_t* positions,
+              const int64_t* pos_strides, int64_t start, int B, int T, int d, int inverse, void* q_out, void* k_out,
+              void* stream);
+
+/* Quantising append: k_new, v_new [B,G,T,128] (strides for B, G, T; dtype) become codes at their positions. A block's
+ *   exponent is the smallest with amax <= 448 * 2^e over its finite values (in [-100, 120]); a block that keeps earlier
+ *   rows keeps at least its exponent, and where that grows the kept codes are rounded again. NaN and infinities become the
+ *   NaN code. With a table, k_new is rotated first (in fp32), and q [B,G,h,T,128] (strides for B, G, h, T), when given, is
+ *   rotated to the contiguous q_out. */
+int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const int* lengths, int length,
+                 const void* k_new, const int64_t* k_strides, const void* v_new, const int64_t* v_strides, int dtype,
+                 const float* table, int table_rows, int rot, int layout, const void* q, const int64_t* q_strides, int h,
+                 void* q_out, int B, int G, int T, int C, int d, void* stream);
+
+/* Read-back: positions [lo, hi) as values in out_dtype, k_out and v_out [B,G,hi-lo,128] contiguous. */
+int al_read_q8(const void* k_codes, const void* v_codes, const void* k_exp, const void* v_exp, int B, int G, int C, int d,
+               int lo, int hi, int out_dtype, void* k_out, void* v_out, void* stream);
+
+/* Attention of q [B,G,h,T,128] (strides for B, G, h, T) over the cache: the query at position p sees tokens j <= p with
+ *   window = 0, or j > p - window, or j < sinks. out [B,G,h,T,128] (dtype, contiguous); a row that sees nothing is zero.
+ *   max_length (0 = C) is what the caller knows of the largest length; it only chooses how the work is split. The
+ *   workspace (al_attend_q8_workspace bytes, 16-byte aligned; NULL when that is 0) holds partial results of the call. */
+int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int sinks, int max_length, size_t* bytes);
+int al_attend_q8(const void* q, const int64_t* q_strides, int dtype, const void* k_codes, const void* v_codes,
+                 const void* k_exp, const void* v_exp, const int* lengths, int length, int B, int G, int h, int T, int C,
+                 int d, int window, int sinks, float scale, int max_length, void* out, void* workspace,
+                 size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
