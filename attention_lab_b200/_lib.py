@@ -80,20 +80,24 @@ SIGNATURES = {
                                      c_void_p, c_void_p],
     "al_prefill_score_topk": [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
                               c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
-    "al_rotary": [c_void_p, P64, c_int, c_void_p, P64, c_int, c_int,
-                  c_void_p, c_int, c_int, c_int, c_void_p, P64, c_int64,
+    "al_rotary": [c_void_p, c_int64, c_int64, c_int64, c_int,
+                  c_void_p, c_int64, c_int64, c_int64, c_int, c_int,
+                  c_void_p, c_int, c_int, c_int,
+                  c_void_p, c_int64, c_int64, c_int64,
                   c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "al_append_q8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                     c_void_p, P64, c_void_p, P64, c_int,
-                     c_void_p, c_int, c_int, c_int, c_void_p, P64, c_int,
-                     c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
+                     c_void_p, c_int64, c_int64, c_int64,
+                     c_void_p, c_int64, c_int64, c_int64, c_int,
+                     c_void_p, c_int, c_int, c_int,
+                     c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,
+                     c_int, c_int, c_int, c_int, c_int, c_void_p],
     "al_read_q8": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                    c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "al_attend_q8_workspace": [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, POINTER(ctypes.c_size_t)],
-    "al_attend_q8": [c_void_p, P64, c_int, c_void_p, c_void_p,
-                     c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
-                     c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p,
-                     ctypes.c_size_t, c_void_p],
+    "al_attend_q8": [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int,
+                     c_void_p, c_void_p, c_void_p, c_void_p,
+                     c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                     c_float, c_int, c_void_p, c_void_p, ctypes.c_size_t, c_void_p],
 }
 
 _lib = None

@@ -9,12 +9,8 @@ using namespace al;
 
 namespace {
 
-bool rows_aligned(const void* p, const int64_t* strides, int n, int dtype) {
-  const int64_t unit = 16 / esize(dtype);
-  if (!aligned16(p)) return false;
-  for (int i = 0; i < n; ++i)
-    if (strides[i] % unit) return false;
-  return true;
+bool rows_aligned(const void* p, int dtype, int64_t s0, int64_t s1, int64_t s2, int64_t s3 = 0) {
+  return aligned16(p) && ((s0 | s1 | s2 | s3) & (16 / esize(dtype) - 1)) == 0;
 }
 
 int rot_table(const float* table, int rows, int rot, int layout, int d, RotTable* out) {
@@ -54,7 +50,7 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
   int len = max_length > 0 ? std::min(max_length, C) : C;
   // tokens a query tile can see, as far as the host knows
   const long long span = window > 0 ? std::min<long long>(len, (long long)window + sinks) : len;
-  if (R <= kQ8TokenCols) {
+  if (R <= AL_Q8_TOKEN_COLS) {
     pl.token = true;
     const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
     pl.cs = 1;
@@ -121,10 +117,11 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
 
 extern "C" {
 
-int al_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, const int64_t* k_strides, int Hk, int dtype,
-              const float* table, int table_rows, int rot, int layout, const int64_t* positions,
-              const int64_t* pos_strides, int64_t start, int B, int T, int d, int inverse, void* q_out, void* k_out,
-              void* stream) {
+int al_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, int Hq,
+              const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, int Hk, int dtype,
+              const float* table, int table_rows, int rot, int layout,
+              const int64_t* positions, int64_t pos_sb, int64_t pos_st, int64_t start,
+              int B, int T, int d, int inverse, void* q_out, void* k_out, void* stream) {
   if (!dtype_ok(dtype)) return fail(AL_EINVAL, "unknown dtype code");
   if (B < 0 || T < 0 || Hq < 1 || Hk < 0) return fail(AL_EINVAL, "need B, T >= 0, Hq >= 1 and Hk >= 0");
   if (d < 8 || d % 8 || d > 1024) return fail(AL_EUNSUPPORTED, "head_dim must be a multiple of 8 in [8, 1024], got %d", d);
@@ -132,18 +129,17 @@ int al_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, co
   int rc = rot_table(table, table_rows, rot, layout, d, &p.rt);
   if (rc) return rc;
   if (B == 0 || T == 0) return AL_OK;
-  if (!q || !q_strides || !q_out || (Hk > 0 && (!k || !k_strides || !k_out))) return fail(AL_EINVAL, "null pointer argument");
-  if (positions && !pos_strides) return fail(AL_EINVAL, "positions given without strides");
-  if (!rows_aligned(q, q_strides, 3, dtype) || !aligned16(q_out) ||
-      (Hk > 0 && (!rows_aligned(k, k_strides, 3, dtype) || !aligned16(k_out))))
+  if (!q || !q_out || (Hk > 0 && (!k || !k_out))) return fail(AL_EINVAL, "null pointer argument");
+  if (!rows_aligned(q, dtype, q_sb, q_sh, q_st) || !aligned16(q_out) ||
+      (Hk > 0 && (!rows_aligned(k, dtype, k_sb, k_sh, k_st) || !aligned16(k_out))))
     return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
   DeviceInfo* di = nullptr;
   if ((rc = device_info(&di))) return rc;
-  p.q.x = q; p.q.sb = q_strides[0]; p.q.sh = q_strides[1]; p.q.st = q_strides[2]; p.q.H = Hq; p.q.out = q_out;
-  if (Hk > 0) { p.k.x = k; p.k.sb = k_strides[0]; p.k.sh = k_strides[1]; p.k.st = k_strides[2]; p.k.H = Hk; p.k.out = k_out; }
+  p.q.x = q; p.q.sb = q_sb; p.q.sh = q_sh; p.q.st = q_st; p.q.H = Hq; p.q.out = q_out;
+  if (Hk > 0) { p.k.x = k; p.k.sb = k_sb; p.k.sh = k_sh; p.k.st = k_st; p.k.H = Hk; p.k.out = k_out; }
   if (positions) {
     p.pos = reinterpret_cast<const long long*>(positions);
-    p.pos_sb = pos_strides[0]; p.pos_st = pos_strides[1];
+    p.pos_sb = pos_sb; p.pos_st = pos_st;
   }
   p.start = start; p.B = B; p.T = T; p.d = d; p.sgn = inverse ? -1.0f : 1.0f; p.err = di->err;
   const long long threads = (long long)B * T * (d / 8), heads = Hq + Hk;
@@ -160,9 +156,11 @@ int al_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, co
 }
 
 int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const int* lengths, int length,
-                 const void* k_new, const int64_t* k_strides, const void* v_new, const int64_t* v_strides, int dtype,
-                 const float* table, int table_rows, int rot, int layout, const void* q, const int64_t* q_strides, int h,
-                 void* q_out, int B, int G, int T, int C, int d, void* stream) {
+                 const void* k_new, int64_t k_sb, int64_t k_sg, int64_t k_st,
+                 const void* v_new, int64_t v_sb, int64_t v_sg, int64_t v_st, int dtype,
+                 const float* table, int table_rows, int rot, int layout,
+                 const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t q_st, int h, void* q_out,
+                 int B, int G, int T, int C, int d, void* stream) {
   if (!dtype_ok(dtype)) return fail(AL_EINVAL, "unknown dtype code");
   int rc = q8_shape(B, G, C, d, k_codes, v_codes, k_exp, v_exp);
   if (rc) return rc;
@@ -176,12 +174,12 @@ int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const i
       return fail(AL_EINVAL, "positions up to %d exceed the rotary table's %d rows", length - 1, table_rows);
   }
   if (B == 0 || T == 0) return AL_OK;
-  if (!k_new || !v_new || !k_strides || !v_strides) return fail(AL_EINVAL, "null pointer argument");
-  if (!rows_aligned(k_new, k_strides, 3, dtype) || !rows_aligned(v_new, v_strides, 3, dtype))
+  if (!k_new || !v_new) return fail(AL_EINVAL, "null pointer argument");
+  if (!rows_aligned(k_new, dtype, k_sb, k_sg, k_st) || !rows_aligned(v_new, dtype, v_sb, v_sg, v_st))
     return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
   if (q) {
-    if (h < 1 || !q_strides || !q_out) return fail(AL_EINVAL, "q given without heads, strides or an output");
-    if (!rows_aligned(q, q_strides, 4, dtype) || !aligned16(q_out)) return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
+    if (h < 1 || !q_out) return fail(AL_EINVAL, "q given without heads or an output");
+    if (!rows_aligned(q, dtype, q_sb, q_sg, q_sh, q_st) || !aligned16(q_out)) return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
     if ((long long)G * h * T > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query rows per request");
   }
   DeviceInfo* di = nullptr;
@@ -189,8 +187,8 @@ int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const i
   p.codes[0] = static_cast<uint8_t*>(k_codes); p.codes[1] = static_cast<uint8_t*>(v_codes);
   p.exps[0] = static_cast<signed char*>(k_exp); p.exps[1] = static_cast<signed char*>(v_exp);
   p.x[0] = k_new; p.x[1] = v_new;
-  p.sb[0] = k_strides[0]; p.sg[0] = k_strides[1]; p.st[0] = k_strides[2];
-  p.sb[1] = v_strides[0]; p.sg[1] = v_strides[1]; p.st[1] = v_strides[2];
+  p.sb[0] = k_sb; p.sg[0] = k_sg; p.st[0] = k_st;
+  p.sb[1] = v_sb; p.sg[1] = v_sg; p.st[1] = v_st;
   p.len.per_batch = lengths; p.len.all = length;
   p.B = B; p.G = G; p.T = T; p.C = C; p.NB = q8_blocks(C);
   p.touched = std::min((T + kQ8Block - 2) / kQ8Block + 1, p.NB);
@@ -198,7 +196,7 @@ int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const i
   const long long kv = 2LL * B * G * p.touched;
   long long qc = 0;
   if (q) {
-    p.q = q; p.q_sb = q_strides[0]; p.q_sg = q_strides[1]; p.q_sh = q_strides[2]; p.q_st = q_strides[3];
+    p.q = q; p.q_sb = q_sb; p.q_sg = q_sg; p.q_sh = q_sh; p.q_st = q_st;
     p.h = h; p.q_out = q_out;
     qc = ((long long)B * G * h * T * 16 + kQ8AppendThreads - 1) / kQ8AppendThreads;
   }
@@ -249,10 +247,10 @@ int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int si
   return AL_OK;
 }
 
-int al_attend_q8(const void* q, const int64_t* q_strides, int dtype, const void* k_codes, const void* v_codes,
-                 const void* k_exp, const void* v_exp, const int* lengths, int length, int B, int G, int h, int T, int C,
-                 int d, int window, int sinks, float scale, int max_length, void* out, void* workspace,
-                 size_t workspace_bytes, void* stream) {
+int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t q_st, int dtype,
+                 const void* k_codes, const void* v_codes, const void* k_exp, const void* v_exp,
+                 const int* lengths, int length, int B, int G, int h, int T, int C, int d, int window, int sinks,
+                 float scale, int max_length, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   if (!dtype_ok(dtype)) return fail(AL_EINVAL, "unknown dtype code");
   int rc = q8_shape(B, G, C, d, k_codes, v_codes, k_exp, v_exp);
   if (rc) return rc;
@@ -260,8 +258,8 @@ int al_attend_q8(const void* q, const int64_t* q_strides, int dtype, const void*
   if (!lengths && (length < 0 || length > C)) return fail(AL_EINVAL, "length=%d must be in [0, capacity=%d]", length, C);
   if (!(scale == scale) || scale > 3.0e38f || scale < -3.0e38f) return fail(AL_EINVAL, "scale must be finite");
   if (B == 0 || T == 0) return AL_OK;
-  if (!q || !q_strides || !out) return fail(AL_EINVAL, "null pointer argument");
-  if (!rows_aligned(q, q_strides, 4, dtype) || !aligned16(out)) return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
+  if (!q || !out) return fail(AL_EINVAL, "null pointer argument");
+  if (!rows_aligned(q, dtype, q_sb, q_sg, q_sh, q_st) || !aligned16(out)) return fail(AL_EUNSUPPORTED, "rows must start on 16-byte boundaries");
   DeviceInfo* di = nullptr;
   if ((rc = device_info(&di))) return rc;
   Q8Plan pl;
@@ -269,7 +267,7 @@ int al_attend_q8(const void* q, const int64_t* q_strides, int dtype, const void*
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)))
     return fail(AL_EINVAL, "this call needs a 16-byte aligned workspace of %zu bytes, got %zu", pl.bytes, workspace_bytes);
   Q8AttendParams p = {};
-  p.q = q; p.q_sb = q_strides[0]; p.q_sg = q_strides[1]; p.q_sh = q_strides[2]; p.q_st = q_strides[3];
+  p.q = q; p.q_sb = q_sb; p.q_sg = q_sg; p.q_sh = q_sh; p.q_st = q_st;
   p.kc = static_cast<const uint8_t*>(k_codes); p.vc = static_cast<const uint8_t*>(v_codes);
   p.ke = static_cast<const signed char*>(k_exp); p.ve = static_cast<const signed char*>(v_exp);
   p.len.per_batch = lengths; p.len.all = length;

@@ -23,7 +23,6 @@ namespace al {
 constexpr int kQdWarps = 4;
 constexpr int kQdThreads = 32 * kQdWarps;
 constexpr int kQdCols = 8;                 // columns (query, head) per CTA
-constexpr int kQ8TokenCols = 16;          // up to this many columns per group take this kernel, more the prompt kernel
 constexpr int kQdStep = 32;                // tokens per warp step (half a block: one exponent each for K and V)
 constexpr float kQdBias = 10.0f;           // weights run up to 2^10, so f16's normal range starts 2^-24 below the largest
 

@@ -27,12 +27,18 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .ops import _code, _cuda, _scale, _stream
 
 BLOCK = 64                     # tokens that share one exponent
 HEAD_DIM = 128
 LAYOUTS = {"half": 0, "interleaved": 1}
+TOKEN_ROWS = 16                # up to this many query rows per group attention needs no workspace (AL_Q8_TOKEN_COLS)
 _CODES = torch.float8_e4m3fn
+_DTYPES = {torch.float32: _lib.AL_F32, torch.bfloat16: _lib.AL_BF16}
+
+# These operators also serve calls of a few microseconds (a decode step of one request), where the wrapper's own time
+# counts: tensors are compared by device ordinal, the stream handle is taken without building a Stream object, and the
+# device is switched only when it is not the current one.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class Q8Cache(NamedTuple):
@@ -53,25 +59,63 @@ class Q8Cache(NamedTuple):
                    torch.zeros(nb, dtype=torch.int8, device=device), torch.zeros(nb, dtype=torch.int8, device=device))
 
 
+def _call_on(dev: int, entry, *args) -> None:
+    """entry(*args) with device `dev` current."""
+    if torch.cuda.current_device() == dev:
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args)
+    if rc:
+        _lib.check(rc)
+
+
+def _call(dev: int, entry, *args) -> None:
+    """entry(*args, stream) on device `dev`, on its current stream."""
+    _call_on(dev, entry, *args, _raw_stream(dev))
+
+
+def _same_device(dev: int, *ts) -> None:
+    if dev < 0:
+        raise ValueError("every tensor must live on a CUDA device (the CUDA path has no CPU fallback)")
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            if not t.is_cuda:
+                raise ValueError("every tensor must live on a CUDA device (the CUDA path has no CPU fallback)")
+            raise ValueError("all inputs must live on the same device")
+
+
+def _code(dtype, what: str) -> int:
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32 or bfloat16, got {dtype}")
+    return code
+
+
 def _check_q8(cache):
+    """(codes and exponents as given, their shape, device ordinal)"""
     k, v, ke, ve = cache
-    if k.dim() != 4 or k.shape != v.shape:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError(f"the codes must be [B,G,C,d] of one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != _CODES or v.dtype != _CODES:
         raise ValueError(f"the codes must be float8_e4m3fn, got {k.dtype} and {v.dtype}")
-    B, G, C, d = k.shape
+    B, G, C, d = shape
     if ke.shape != (B, G, -(-C // BLOCK)) or ve.shape != ke.shape or ke.dtype != torch.int8 or ve.dtype != torch.int8:
         raise ValueError("the exponents must be int8 [B,G,ceil(C/64)]")
     if not (k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()):
         raise ValueError("codes and exponents must be contiguous")
-    return B, G, C, d
+    dev = k.get_device()
+    _same_device(dev, v, ke, ve)
+    return B, G, C, d, dev
 
 
-def _check_lengths(lengths, B: int, what: str, least: int, most: int):
+def _check_lengths(lengths, B: int, dev: int, what: str, least: int, most: int):
     """(device pointer or None, int)"""
     if isinstance(lengths, torch.Tensor):
         if lengths.dtype != torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous():
             raise ValueError("lengths must be an int or a contiguous int32 tensor [B]")
+        _same_device(dev, lengths)
         return lengths.data_ptr(), 0
     n = int(lengths)
     if not least <= n <= most:
@@ -79,18 +123,18 @@ def _check_lengths(lengths, B: int, what: str, least: int, most: int):
     return None, n
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x itself when its rows can be read in 16-byte pieces, else a contiguous copy."""
-    unit = 16 // x.element_size()
-    s = x.stride()
-    if s[-1] == 1 and x.data_ptr() % 16 == 0:
-        for i in s[:-1]:
-            if i % unit:
-                break
-        else:
-            return x
-    x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
+def _rows(x: torch.Tensor):
+    """(x, its address, its strides); a contiguous copy of x when its rows cannot be read in 16-byte pieces."""
+    s, p = x.stride(), x.data_ptr()
+    bits = 0
+    for i in s[:-1]:
+        bits |= i
+    if s[-1] != 1 or p & 15 or bits & (16 // x.element_size() - 1):
+        x = x.contiguous()
+        if x.data_ptr() & 15:
+            x = x.clone()
+        s, p = x.stride(), x.data_ptr()
+    return x, p, s
 
 
 def _check_table(table: torch.Tensor, layout: str) -> int:
@@ -152,38 +196,40 @@ def rotary_embed(q: torch.Tensor, k, table: torch.Tensor, positions, *, layout: 
     (a c - b s, b c + a s) in float32, rounded once; dimensions past the table's rotary_dim are copied. `positions` is
     an int (row t at positions + t) or int64 [B,T] (or [T]); negative ones are padding (zeros), one past the table gives
     zeros and error bit 4. `inverse` rotates back: the gradient of the forward rotation. Returns (q', k')."""
-    dev = _cuda(q, k, table, positions if isinstance(positions, torch.Tensor) else None)
     lay = _check_table(table, layout)
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError(f"q must be [B,H,T,d], got {tuple(q.shape)}")
-    B, H, T, d = q.shape
-    code = _code(q, "q")
-    q = _rows(q)
-    Hk, kp, ks, ko, k_out = 0, None, None, None, None
+    B, H, T, d = shape
+    dev, dtype = q.get_device(), q.dtype
+    code = _code(dtype, "q")
+    _same_device(dev, table, k)
+    q, qp, qs = _rows(q)
+    Hk, kp, ks, ko, k_out = 0, None, (0, 0, 0), None, None
     if k is not None:
-        if k.dim() != 4 or k.shape[0] != B or k.shape[2] != T or k.shape[3] != d or k.dtype != q.dtype:
+        Hk = k.shape[1] if k.dim() == 4 else 0
+        if k.shape != (B, Hk, T, d) or k.dtype != dtype:
             raise ValueError("k must be [B,G,T,d] of q's dtype")
-        k = _rows(k)
-        Hk, kp, ks = k.shape[1], k.data_ptr(), _lib.strides(k, 3)
-        k_out = torch.empty((B, Hk, T, d), dtype=q.dtype, device=dev)
+        k, kp, ks = _rows(k)
+        k_out = q.new_empty((B, Hk, T, d))
         ko = k_out.data_ptr()
-    pp, pst, start = None, None, 0
+    pp, pst, start = None, (0, 0), 0
     if isinstance(positions, torch.Tensor):
         if positions.dtype != torch.int64:
             raise ValueError("positions must be int64")
-        pos = positions.expand(B, T) if positions.dim() < 2 or positions.shape[0] == 1 else positions
-        if tuple(pos.shape) != (B, T):
+        _same_device(dev, positions)
+        if positions.dim() < 2 or positions.shape[0] == 1:
+            positions = positions.expand(B, T)
+        if positions.shape != (B, T):
             raise ValueError(f"positions must be [B,T] = [{B},{T}], got {tuple(positions.shape)}")
-        pp, pst = pos.data_ptr(), _lib.strides(pos, 2)
+        pp, pst = positions.data_ptr(), positions.stride()
     else:
         start = int(positions)
         if start < 0 or start + T > table.shape[0]:
             raise ValueError(f"positions [{start}, {start + T}) outside the table's {table.shape[0]} rows")
-    out = torch.empty((B, H, T, d), dtype=q.dtype, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().al_rotary(
-            q.data_ptr(), _lib.strides(q, 3), H, kp, ks, Hk, code, table.data_ptr(), table.shape[0], table.shape[1], lay,
-            pp, pst, start, B, T, d, int(bool(inverse)), out.data_ptr(), ko, _stream(dev)))
+    out = q.new_empty(shape)
+    _call(dev, _lib.load().al_rotary, qp, qs[0], qs[1], qs[2], H, kp, ks[0], ks[1], ks[2], Hk, code, table.data_ptr(),
+          table.shape[0], table.shape[1], lay, pp, pst[0], pst[1], start, B, T, d, int(bool(inverse)), out.data_ptr(), ko)
     return out, k_out
 
 
@@ -192,51 +238,50 @@ def append_q8(cache, lengths, k_new: torch.Tensor, v_new: torch.Tensor, *, q=Non
     rotated to its positions first (in float32, then rounded to codes once), and q [B,G,h,T,d], when given, is returned
     rotated ([B,G,h,T,d] contiguous, zeros in padding rows); without a table q must be None. One launch."""
     k, v, ke, ve = cache
-    dev = _cuda(k, v, ke, ve, k_new, v_new, q, table, lengths if isinstance(lengths, torch.Tensor) else None)
-    B, G, C, d = _check_q8(cache)
-    if k_new.dim() != 4 or k_new.shape[0] != B or k_new.shape[1] != G or k_new.shape[3] != d or v_new.shape != k_new.shape:
+    B, G, C, d, dev = _check_q8(cache)
+    shape, dtype = k_new.shape, k_new.dtype
+    if len(shape) != 4 or shape[0] != B or shape[1] != G or shape[3] != d or v_new.shape != shape:
         raise ValueError("k_new and v_new must be [B,G,T,d] matching the cache")
-    if v_new.dtype != k_new.dtype:
+    if v_new.dtype != dtype:
         raise ValueError("k_new and v_new must share one dtype")
-    T, code = k_new.shape[2], _code(k_new, "k_new")
-    lp, length = _check_lengths(lengths, B, "append", T, C)
+    _same_device(dev, k_new, v_new, table, q)
+    T, code = shape[2], _code(dtype, "k_new")
+    lp, length = _check_lengths(lengths, B, dev, "append", T, C)
     tp, trows, rot, lay = None, 0, 0, 0
     if table is not None:
         lay = _check_table(table, layout)
-        tp, trows, rot = table.data_ptr(), table.shape[0], table.shape[1]
-    qp, qst, h, q_out, qo = None, None, 0, None, None
+        tp, (trows, rot) = table.data_ptr(), table.shape
+    qp, qs, h, q_out, qo = None, (0, 0, 0, 0), 0, None, None
     if q is not None:
         if table is None:
             raise ValueError("q is rotated: it needs a table")
-        if q.dim() != 5 or q.shape[0] != B or q.shape[1] != G or q.shape[3] != T or q.shape[4] != d or q.dtype != k_new.dtype:
+        h = q.shape[2] if q.dim() == 5 else 0
+        if q.shape != (B, G, h, T, d) or q.dtype != dtype:
             raise ValueError("q must be [B,G,h,T,d] of k_new's dtype")
-        q = _rows(q)
-        h = q.shape[2]
-        q_out = torch.empty((B, G, h, T, d), dtype=q.dtype, device=dev)
-        qp, qst, qo = q.data_ptr(), _lib.strides(q, 4), q_out.data_ptr()
-    k_new, v_new = _rows(k_new), _rows(v_new)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().al_append_q8(
-            k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), lp, length, k_new.data_ptr(),
-            _lib.strides(k_new, 3), v_new.data_ptr(), _lib.strides(v_new, 3), code, tp, trows, rot, lay, qp, qst, h, qo,
-            B, G, T, C, d, _stream(dev)))
+        q, qp, qs = _rows(q)
+        q_out = q.new_empty((B, G, h, T, d))
+        qo = q_out.data_ptr()
+    k_new, kp, ks = _rows(k_new)
+    v_new, vp, vs = _rows(v_new)
+    _call(dev, _lib.load().al_append_q8, k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), lp, length,
+          kp, ks[0], ks[1], ks[2], vp, vs[0], vs[1], vs[2], code, tp, trows, rot, lay,
+          qp, qs[0], qs[1], qs[2], qs[3], h, qo, B, G, T, C, d)
     return q_out
 
 
 def read_q8(cache, lo: int, hi: int, *, dtype=torch.bfloat16):
     """Positions [lo, hi) of the cache as values: (k, v), each [B,G,hi-lo,d] of dtype."""
     k, v, ke, ve = cache
-    dev = _cuda(k, v, ke, ve)
-    B, G, C, d = _check_q8(cache)
+    B, G, C, d, dev = _check_q8(cache)
     lo, hi = int(lo), int(hi)
     if not 0 <= lo <= hi <= C:
         raise ValueError(f"need 0 <= lo <= hi <= capacity {C}, got lo={lo} hi={hi}")
-    ko, vo = (torch.empty((B, G, hi - lo, d), dtype=dtype, device=dev) for _ in range(2))
-    code = _code(ko, "dtype")
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().al_read_q8(k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), B, G, C, d, lo, hi,
-                                          code, ko.data_ptr(), vo.data_ptr(), _stream(dev)))
-    return ko, vo
+    code = _code(dtype, "dtype")
+    k_out = torch.empty((B, G, hi - lo, d), dtype=dtype, device=k.device)
+    v_out = torch.empty_like(k_out)
+    _call(dev, _lib.load().al_read_q8, k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), B, G, C, d, lo, hi, code,
+          k_out.data_ptr(), v_out.data_ptr())
+    return k_out, v_out
 
 
 def attend_q8(q: torch.Tensor, cache, lengths, *, window: int = 0, sinks: int = 0, scale=None, max_length=None):
@@ -245,26 +290,30 @@ def attend_q8(q: torch.Tensor, cache, lengths, *, window: int = 0, sinks: int = 
     capacity) is what the caller knows of the largest length; it chooses how the work is split, never the result's rows.
     Returns [B,G,h,T,d] of q's dtype."""
     k, v, ke, ve = cache
-    dev = _cuda(q, k, v, ke, ve, lengths if isinstance(lengths, torch.Tensor) else None)
-    B, G, C, d = _check_q8(cache)
-    if q.dim() != 5 or q.shape[0] != B or q.shape[1] != G or q.shape[4] != d:
+    B, G, C, d, dev = _check_q8(cache)
+    shape = q.shape
+    if len(shape) != 5 or shape[0] != B or shape[1] != G or shape[4] != d:
         raise ValueError(f"q must be [B,G,h,T,d] matching the cache, got {tuple(q.shape)}")
-    _, _, h, T, _ = q.shape
-    code = _code(q, "q")
+    _same_device(dev, q)
+    h, T = shape[2], shape[3]
+    code = _code(q.dtype, "q")
     window, sinks = int(window), int(sinks)
     if window < 0 or sinks < 0:
         raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
-    lp, length = _check_lengths(lengths, B, "attend", 0, C)
+    lp, length = _check_lengths(lengths, B, dev, "attend", 0, C)
     most = length if lp is None else (C if max_length is None else int(max_length))
-    q = _rows(q)
-    out = torch.empty((B, G, h, T, d), dtype=q.dtype, device=dev)
+    q, qp, qs = _rows(q)
+    out = q.new_empty(shape)
     lib = _lib.load()
-    need = ctypes.c_size_t(0)
-    with torch.cuda.device(dev):
-        _lib.check(lib.al_attend_q8_workspace(B, G, h, T, C, window, sinks, most, ctypes.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        _lib.check(lib.al_attend_q8(
-            q.data_ptr(), _lib.strides(q, 4), code, k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), lp, length,
-            B, G, h, T, C, d, window, sinks, _scale(d, scale), most, out.data_ptr(),
-            None if work is None else work.data_ptr(), need.value, _stream(dev)))
+    work, wp, wn = None, None, 0
+    if h * T > TOKEN_ROWS:
+        need = ctypes.c_size_t(0)
+        _call_on(dev, lib.al_attend_q8_workspace, B, G, h, T, C, window, sinks, most, ctypes.byref(need))
+        wn = need.value
+        if wn:
+            work = torch.empty(wn, dtype=torch.uint8, device=q.device)
+            wp = work.data_ptr()
+    _call(dev, lib.al_attend_q8, qp, qs[0], qs[1], qs[2], qs[3], code, k.data_ptr(), v.data_ptr(), ke.data_ptr(),
+          ve.data_ptr(), lp, length, B, G, h, T, C, d, window, sinks, 1.0 / math.sqrt(d) if scale is None else float(scale),
+          most, out.data_ptr(), wp, wn)
     return out

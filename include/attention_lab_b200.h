@@ -218,10 +218,11 @@ int al_prefill_score_topk(const void* u, long long u_sh, long long u_st, const v
  *   becomes (a c - b s, b c + a s), with -s when `inverse` (the gradient); dimensions from rot on are copied.
  *   positions [B,T] int64 (strides for B, T) or NULL: start + t. A negative position gives zeros; one past the table gives
  *   zeros and error bit 4. */
-int al_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, const int64_t* k_strides, int Hk, int dtype,
-              const float* table, int table_rows, int rot, int layout, const int64_t* positions,
-              const int64_t* pos_strides, int64_t start, int B, int T, int d, int inverse, void* q_out, void* k_out,
-              void* stream);
+int al_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, int Hq,
+              const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, int Hk, int dtype,
+              const float* table, int table_rows, int rot, int layout,
+              const int64_t* positions, int64_t pos_sb, int64_t pos_st, int64_t start,
+              int B, int T, int d, int inverse, void* q_out, void* k_out, void* stream);
 
 /* Quantising append: k_new, v_new [B,G,T,128] (strides for B, G, T; dtype) become codes at their positions. A block's
  *   exponent is the smallest with amax <= 448 * 2^e over its finite values (in [-100, 120]); a block that keeps earlier
@@ -229,9 +230,11 @@ int al_rotary(const void* q, const int64_t* q_strides, int Hq, const void* k, co
  *   NaN code. With a table, k_new is rotated first (in fp32), and q [B,G,h,T,128] (strides for B, G, h, T), when given, is
  *   rotated to the contiguous q_out. */
 int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const int* lengths, int length,
-                 const void* k_new, const int64_t* k_strides, const void* v_new, const int64_t* v_strides, int dtype,
-                 const float* table, int table_rows, int rot, int layout, const void* q, const int64_t* q_strides, int h,
-                 void* q_out, int B, int G, int T, int C, int d, void* stream);
+                 const void* k_new, int64_t k_sb, int64_t k_sg, int64_t k_st,
+                 const void* v_new, int64_t v_sb, int64_t v_sg, int64_t v_st, int dtype,
+                 const float* table, int table_rows, int rot, int layout,
+                 const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t q_st, int h, void* q_out,
+                 int B, int G, int T, int C, int d, void* stream);
 
 /* Read-back: positions [lo, hi) as values in out_dtype, k_out and v_out [B,G,hi-lo,128] contiguous. */
 int al_read_q8(const void* k_codes, const void* v_codes, const void* k_exp, const void* v_exp, int B, int G, int C, int d,
@@ -240,12 +243,14 @@ int al_read_q8(const void* k_codes, const void* v_codes, const void* k_exp, cons
 /* Attention of q [B,G,h,T,128] (strides for B, G, h, T) over the cache: the query at position p sees tokens j <= p with
  *   window = 0, or j > p - window, or j < sinks. out [B,G,h,T,128] (dtype, contiguous); a row that sees nothing is zero.
  *   max_length (0 = C) is what the caller knows of the largest length; it only chooses how the work is split. The
- *   workspace (al_attend_q8_workspace bytes, 16-byte aligned; NULL when that is 0) holds partial results of the call. */
+ *   workspace (al_attend_q8_workspace bytes, 16-byte aligned; NULL when that is 0) holds partial results of the call;
+ *   with h*T <= AL_Q8_TOKEN_COLS query rows per group it is always 0. */
+#define AL_Q8_TOKEN_COLS 16
 int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int sinks, int max_length, size_t* bytes);
-int al_attend_q8(const void* q, const int64_t* q_strides, int dtype, const void* k_codes, const void* v_codes,
-                 const void* k_exp, const void* v_exp, const int* lengths, int length, int B, int G, int h, int T, int C,
-                 int d, int window, int sinks, float scale, int max_length, void* out, void* workspace,
-                 size_t workspace_bytes, void* stream);
+int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t q_st, int dtype,
+                 const void* k_codes, const void* v_codes, const void* k_exp, const void* v_exp,
+                 const int* lengths, int length, int B, int G, int h, int T, int C, int d, int window, int sinks,
+                 float scale, int max_length, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
