@@ -39,15 +39,30 @@ constexpr int kQpRegsSoftmax = 184, kQpRegsConvert = 104, kQpRegsMma = 40;
 constexpr uint32_t kQpIdescQK = (1u << 4) | ((uint32_t)(kQpKeys >> 3) << 17) | ((uint32_t)(kQpRows >> 4) << 24);
 constexpr uint32_t kQpIdescPV = kQpIdescQK | (1u << 16);
 
-__device__ __forceinline__ void qp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-               ::"r"(d), "l"(a), "l"(b), "r"(kQpIdescQK), "r"(accumulate) : "memory");
+// The MMA warp runs its loop with all lanes (waits, addresses and descriptors stay warp-uniform, so they live in uniform
+// registers); `lead`, set in one lane, predicates the instructions one thread issues. With the loop inside a lane-0
+// branch every MMA took two to four register moves and each wait about 300 cycles.
+__device__ __forceinline__ void qp_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(kQpIdescQK), "r"(accumulate), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void qp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-               ::"r"(d), "r"(a), "l"(b), "r"(kQpIdescPV), "r"(accumulate) : "memory");
+__device__ __forceinline__ void qp_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(b), "r"(kQpIdescPV), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void qp_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+               " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n"
+               ::"r"(smem_addr(bar)), "r"(lead) : "memory");
+}
+// pf_wait with the common case (the phase is complete) tested before anything else.
+__device__ __forceinline__ void qp_wait(uint64_t* bar, unsigned parity, volatile int* abort_flag, unsigned* err) {
+  uint32_t done;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+  if (!done) pf_wait(bar, parity, abort_flag, err);
 }
 __device__ __forceinline__ void qp_tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -73,7 +88,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
   constexpr int QP = SPLIT ? 2 : 1;                    // f16 terms per query row
   extern __shared__ __align__(1024) unsigned char qp_raw[];
-  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2], s_pfull[2], s_ofull[2];
+  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2], s_pfull[2][2], s_ofull[2];
   __shared__ uint32_t s_taddr;
   __shared__ int s_nan_count, s_nan[kQpNanList];
   __shared__ volatile int s_abort;
@@ -105,7 +120,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_qfull[i], kQpRows);
       mbar_init(&s_sfull[i], 1);
-      mbar_init(&s_pfull[i], kQpRows);
+      mbar_init(&s_pfull[i][0], kQpRows);
+      mbar_init(&s_pfull[i][1], kQpRows);
       mbar_init(&s_ofull[i], 1);
     }
     for (int i = 0; i < NS; ++i) {
@@ -134,29 +150,39 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       float f_row;
       {
         const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t * p.q_st;
-        uint32_t amax = 0;
-#pragma unroll 4
-        for (int c = 0; c < 16; ++c) {
-          float y[8];
-          q8_load8(src + 8 * c, y);
+        // the whole row in flight at once: the prologue's latency is not hidden by another CTA
+        constexpr int V = kHeadDim * (int)sizeof(T) / 16;
+        uint4 x[V];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(y[i]) & 0x7fffffffu);
+        for (int i = 0; i < V; ++i) x[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float y[V16<T>::n];
+          unpack(x[i], y, src);
+#pragma unroll
+          for (int k = 0; k < V16<T>::n; ++k) amax = max(amax, __float_as_uint(y[k]) & 0x7fffffffu);
         }
         const int eq = q8_row_exponent(amax);
         const float inv = q8_exp2i(-eq) * p.qsign;
         f_row = p.scale * q8_exp2i(eq);
         const uint32_t qtile = s_q + (uint32_t)(qt * QP) * kQpTile;
-#pragma unroll 4
+#pragma unroll
         for (int c = 0; c < 16; ++c) {
           float y[8];
-          q8_load8(src + 8 * c, y);
+          if constexpr (SPLIT) {
+            unpack(x[2 * c], y, src);
+            unpack(x[2 * c + 1], y + 4, src);
+          } else {
+            unpack(x[c], y, src);
+          }
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float a = y[2 * i] * inv, d = y[2 * i + 1] * inv;
             hi[i] = q8_pack_half2(a, d);
-            const float2 x = q8_half2_floats(hi[i]);
-            lo[i] = q8_pack_half2(a - x.x, d - x.y);
+            const float2 z = q8_half2_floats(hi[i]);
+            lo[i] = q8_pack_half2(a - z.x, d - z.y);
           }
           qp_st_shared16(qp_chunk(qtile, row, c), hi[0], hi[1], hi[2], hi[3]);
           if (SPLIT) qp_st_shared16(qp_chunk(qtile + kQpTile, row, c), lo[0], lo[1], lo[2], lo[3]);
@@ -175,7 +201,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       for (int it = 0; it < nt; ++it) {
         const int j0 = tile_token(it0 + it), blk = j0 / kQ8Block, blk1 = min(blk + 1, p.NB - 1);
         const int ek0 = keb[blk], ek1 = keb[blk1], ev0 = veb[blk], ev1 = veb[blk1];
-        pf_wait(&s_sfull[qt], (uint32_t)it & 1u, &s_abort, p.err);
+        qp_wait(&s_sfull[qt], (uint32_t)it & 1u, &s_abort, p.err);
         tmem_fence_after_sync();
         uint32_t s[4][32];
 #pragma unroll
@@ -271,11 +297,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             for (int i = 0; i < 16; ++i) { w[i] = s[2 * hb][i]; w[16 + i] = s[2 * hb + 1][i]; }
             qp_tmem_st32(tS + 64u + 32u * (uint32_t)hb, w);
           }
+          // each half of P is handed over as it is ready: its P V runs under the other half's exponentials
+          tmem_wait_st();
+          tmem_fence_before_sync();
+          pf_arrive(&s_pfull[qt][hb]);
         }
         l += sum[0] + sum[1];
-        tmem_wait_st();
-        tmem_fence_before_sync();
-        pf_arrive(&s_pfull[qt]);
       }
       pf_wait(&s_ofull[qt], 0, &s_abort, p.err);
       tmem_fence_after_sync();
@@ -376,7 +403,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     for (int it = 0; it < nt; ++it) {
       const int st = it % NS;
       const uint32_t par = (uint32_t)(it / NS) & 1u;
-      pf_wait(&s_kempty[st], par ^ 1u, &s_abort, p.err);
+      qp_wait(&s_kempty[st], par ^ 1u, &s_abort, p.err);
       store(s_k + (uint32_t)st * kQpTile, kr);
       qp_fence_async();
       pf_arrive(&s_kfull[st]);
@@ -402,7 +429,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           }
         }
       }
-      pf_wait(&s_vempty[st], par ^ 1u, &s_abort, p.err);
+      qp_wait(&s_vempty[st], par ^ 1u, &s_abort, p.err);
       store(s_v + (uint32_t)st * kQpTile, vr);
       qp_fence_async();
       pf_arrive(&s_vfull[st]);
@@ -411,53 +438,61 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   } else {
     // ---------------------------------------------------------------------------------------------- MMAs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsMma));
-    if (warp == 12 && lane == 0 && nt > 0) {
+    if (warp == 12 && nt > 0) {
+      uint32_t lead;
+      asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
+      const uint64_t dq = pf_sdesc(s_q, 16, 1024, 2), dk = pf_sdesc(s_k, 16, 1024, 2), dv = pf_sdesc(s_v, kQpHalf, 1024, 2);
       auto scores = [&](int qt, int st) {               // S = Q K^T
 #pragma unroll
         for (int term = 0; term < QP; ++term)
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const uint32_t o = (uint32_t)(ks >> 2) * kQpHalf + (uint32_t)(ks & 3) * 32u;
-            qp_mma_ss(tm + (uint32_t)qt * 128u, pf_sdesc(s_q + (uint32_t)(qt * QP + term) * kQpTile + o, 16, 1024, 2),
-                      pf_sdesc(s_k + (uint32_t)st * kQpTile + o, 16, 1024, 2), (term | ks) > 0 ? 1u : 0u);
+            qp_mma_ss(lead, tm + (uint32_t)qt * 128u, dq + (((uint32_t)(qt * QP + term) * kQpTile + o) >> 4),
+                      dk + (((uint32_t)st * kQpTile + o) >> 4), (term | ks) > 0 ? 1u : 0u);
           }
       };
-      auto values = [&](int qt, int st, bool first) {   // O += P V
+      auto values = [&](int qt, int st, int hb, bool first) {   // O += P V over one block (64 tokens) of the tile
 #pragma unroll
         for (int term = 0; term < QP; ++term)
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            qp_mma_ts(tm + 256u + (uint32_t)qt * 128u, tm + (uint32_t)qt * 128u + (uint32_t)term * 64u + (uint32_t)ks * 8u,
-                      pf_sdesc(s_v + (uint32_t)st * kQpTile + (uint32_t)ks * 2048u, kQpHalf, 1024, 2),
-                      (first && term == 0 && ks == 0) ? 0u : 1u);
+          for (int k4 = 0; k4 < 4; ++k4) {
+            const uint32_t ks = (uint32_t)(4 * hb + k4);
+            qp_mma_ts(lead, tm + 256u + (uint32_t)qt * 128u, tm + (uint32_t)qt * 128u + (uint32_t)term * 64u + ks * 8u,
+                      dv + (((uint32_t)st * kQpTile + ks * 2048u) >> 4), (first && term == 0 && ks == 0) ? 0u : 1u);
+          }
       };
-      pf_wait(&s_kfull[0], 0, &s_abort, p.err);
+      qp_wait(&s_kfull[0], 0, &s_abort, p.err);
       for (int qt = 0; qt < ntile; ++qt) {
-        pf_wait(&s_qfull[qt], 0, &s_abort, p.err);
+        qp_wait(&s_qfull[qt], 0, &s_abort, p.err);
         tmem_fence_after_sync();
         scores(qt, 0);
-        pf_commit(&s_sfull[qt]);
+        qp_commit(lead, &s_sfull[qt]);
       }
-      pf_commit(&s_kempty[0]);
+      qp_commit(lead, &s_kempty[0]);
 #pragma unroll 1
       for (int it = 0; it < nt; ++it) {
         const int st = it % NS, st1 = (it + 1) % NS;
         const bool more = it + 1 < nt;
-        pf_wait(&s_vfull[st], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
+        qp_wait(&s_vfull[st], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
+#pragma unroll 1
         for (int qt = 0; qt < ntile; ++qt) {
-          pf_wait(&s_pfull[qt], (uint32_t)it & 1u, &s_abort, p.err);
+          qp_wait(&s_pfull[qt][0], (uint32_t)it & 1u, &s_abort, p.err);
           tmem_fence_after_sync();
-          values(qt, st, it == 0);
-          if (qt == ntile - 1) pf_commit(&s_vempty[st]);
+          values(qt, st, 0, it == 0);
+          qp_wait(&s_pfull[qt][1], (uint32_t)it & 1u, &s_abort, p.err);
+          tmem_fence_after_sync();
+          values(qt, st, 1, false);
+          if (qt == ntile - 1) qp_commit(lead, &s_vempty[st]);
           if (more) {
             // S's columns hold P until the P V above has read them: MMAs of one thread run in order
-            if (qt == 0) pf_wait(&s_kfull[st1], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
+            if (qt == 0) qp_wait(&s_kfull[st1], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
             tmem_fence_after_sync();
             scores(qt, st1);
-            pf_commit(&s_sfull[qt]);
-            if (qt == ntile - 1) pf_commit(&s_kempty[st1]);
+            qp_commit(lead, &s_sfull[qt]);
+            if (qt == ntile - 1) qp_commit(lead, &s_kempty[st1]);
           } else {
-            pf_commit(&s_ofull[qt]);
+            qp_commit(lead, &s_ofull[qt]);
           }
         }
       }
