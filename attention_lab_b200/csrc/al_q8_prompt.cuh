@@ -3,9 +3,10 @@
 //
 // The T x h query rows of a KV group are one list (row r = t * h + head), so all heads of a group share every key tile.
 // A CTA takes 256 of them as two tiles of 128 rows (TMEM lanes) and walks the key tiles (128 tokens) that any of its
-// rows can see. Per key tile and query tile: S = Q K^T (tcgen05.mma, f16 operands from shared memory, fp32 in TMEM),
-// the softmax weights P go back into S's columns as f16, and O += P V (P from TMEM, V from shared memory). The two
-// query tiles alternate, so the tensor cores multiply for one while the other's weights are computed.
+// rows can see, in steps of one block of the cache (64 tokens). Per step and query tile: S = Q K^T (tcgen05.mma, f16
+// operands from shared memory, fp32 in TMEM), the softmax weights P go back into S's columns as f16, and O += P V (P
+// from TMEM, V from shared memory). S has two buffers per query tile, so the next step's scores are there before this
+// step's weights are done: the softmax warps do not wait for the tensor cores.
 //   warps 0-3, 4-7  one thread per query row: scores -> running maximum, weights, denominator; O is rescaled only when
 //                   a row's maximum grew by more than 2^8 (weights up to 2^14 fit f16)
 //   warps 8-11      read the codes from global memory, convert them to f16 (exact) and store them in the 128-byte
@@ -31,13 +32,13 @@ constexpr size_t kQpSmem = 1024 + 6 * kQpTile;         // 2 Q + 2 K + 2 V tiles,
 constexpr int kQpNanList = 64;
 constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8)
 // Registers a thread after the split: 2 x 128 softmax threads, 128 converting threads, the MMA warp's group.
-// 184 + 184 + 104 + 40 = 512 = 4 x the 128 of the launch.
-constexpr int kQpRegsSoftmax = 184, kQpRegsConvert = 104, kQpRegsMma = 40;
+// 176 + 176 + 112 + 48 = 512 = 4 x the 128 of the launch.
+constexpr int kQpRegsSoftmax = 176, kQpRegsConvert = 112, kQpRegsMma = 48;
 
-// Instruction descriptors (kind::f16): fp32 accumulator, f16 operands, M = N = 128; Q K^T has both operands K-major,
-// P V has V N-major.
-constexpr uint32_t kQpIdescQK = (1u << 4) | ((uint32_t)(kQpKeys >> 3) << 17) | ((uint32_t)(kQpRows >> 4) << 24);
-constexpr uint32_t kQpIdescPV = kQpIdescQK | (1u << 16);
+// Instruction descriptors (kind::f16): fp32 accumulator, f16 operands, M = 128; Q K^T has N = 64 (a block) and both
+// operands K-major, P V has N = 128 (the head dimension) and V N-major.
+constexpr uint32_t kQpIdescQK = (1u << 4) | ((uint32_t)(kQ8Block >> 3) << 17) | ((uint32_t)(kQpRows >> 4) << 24);
+constexpr uint32_t kQpIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kHeadDim >> 3) << 17) | ((uint32_t)(kQpRows >> 4) << 24);
 
 // The MMA warp runs its loop with all lanes (waits, addresses and descriptors stay warp-uniform, so they live in uniform
 // registers); `lead`, set in one lane, predicates the instructions one thread issues. With the loop inside a lane-0
@@ -76,6 +77,14 @@ __device__ __forceinline__ void qp_tmem_st32(uint32_t taddr, const uint32_t (&v)
 __device__ __forceinline__ void qp_st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ void qp_st_shared8(uint32_t a, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ uint4 qp_ld_shared16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void qp_fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 // 16-byte chunk c (0..15, 8 f16 each) of row r in a 128-byte swizzled tile of two 64-wide halves.
 __device__ __forceinline__ uint32_t qp_chunk(uint32_t tile, int r, int c) {
@@ -88,8 +97,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
   constexpr int QP = SPLIT ? 2 : 1;                    // f16 terms per query row
   extern __shared__ __align__(1024) unsigned char qp_raw[];
-  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2], s_pfull[2][2], s_ofull[2];
+  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2][2], s_pfull[2][2], s_pv[2];
   __shared__ uint32_t s_taddr;
+  __shared__ float s_frow[2 * kQpRows];
   __shared__ int s_nan_count, s_nan[kQpNanList];
   __shared__ volatile int s_abort;
 
@@ -119,10 +129,11 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_qfull[i], kQpRows);
-      mbar_init(&s_sfull[i], 1);
-      mbar_init(&s_pfull[i][0], kQpRows);
-      mbar_init(&s_pfull[i][1], kQpRows);
-      mbar_init(&s_ofull[i], 1);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&s_sfull[i][k], 1);
+        mbar_init(&s_pfull[i][k], kQpRows);
+      }
+      mbar_init(&s_pv[i], 1);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&s_kfull[i], 128); mbar_init(&s_kempty[i], 1);
@@ -144,98 +155,108 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     const int qt = warp >> 2, row = tid & 127;
     if (qt < ntile && nt > 0) {
       const int r = min(r0 + qt * kQpRows + row, R - 1);
-      const int t = r / p.h, head = r - t * p.h, pos = pbase + t;
+      const int t = r / p.h, pos = pbase + t;
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t tS = tm + lanes + (uint32_t)qt * 128u, tO = tm + lanes + 256u + (uint32_t)qt * 128u;
-      float f_row;
+      const int wrow0 = (warp & 3) * 32;               // the warp's first row of the tile
+      const uint32_t qtile = s_q + (uint32_t)(qt * QP) * kQpTile;
+      // The warp's 32 query rows: L lanes read one row (full lines), all loads of a batch in flight, then scale by the
+      // row's power of two, split and store.
       {
-        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t * p.q_st;
-        // the whole row in flight at once: the prologue's latency is not hidden by another CTA
-        constexpr int V = kHeadDim * (int)sizeof(T) / 16;
-        uint4 x[V];
+        constexpr int L = kHeadDim * (int)sizeof(T) / 16, PER = 32 / L, BATCH = 16;
+        const int sub = lane / L, c = lane % L;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32 / PER; i0 += BATCH) {
+          uint4 x[BATCH];
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-        uint32_t amax = 0;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float y[V16<T>::n];
-          unpack(x[i], y, src);
-#pragma unroll
-          for (int k = 0; k < V16<T>::n; ++k) amax = max(amax, __float_as_uint(y[k]) & 0x7fffffffu);
-        }
-        const int eq = q8_row_exponent(amax);
-        const float inv = q8_exp2i(-eq) * p.qsign;
-        f_row = p.scale * q8_exp2i(eq);
-        const uint32_t qtile = s_q + (uint32_t)(qt * QP) * kQpTile;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          float y[8];
-          if constexpr (SPLIT) {
-            unpack(x[2 * c], y, src);
-            unpack(x[2 * c + 1], y + 4, src);
-          } else {
-            unpack(x[c], y, src);
+          for (int i = 0; i < BATCH; ++i) {
+            const int rq = min(r0 + qt * kQpRows + wrow0 + (i0 + i) * PER + sub, R - 1), tq = rq / p.h;
+            const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + (rq - tq * p.h) * p.q_sh + tq * p.q_st;
+            x[i] = __ldg(reinterpret_cast<const uint4*>(src) + c);
           }
-          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = y[2 * i] * inv, d = y[2 * i + 1] * inv;
-            hi[i] = q8_pack_half2(a, d);
-            const float2 z = q8_half2_floats(hi[i]);
-            lo[i] = q8_pack_half2(a - z.x, d - z.y);
+          for (int i = 0; i < BATCH; ++i) {
+            constexpr int E = V16<T>::n;
+            float y[E];
+            unpack(x[i], y, static_cast<const T*>(p.q));
+            uint32_t amax = 0;
+#pragma unroll
+            for (int k = 0; k < E; ++k) amax = max(amax, __float_as_uint(y[k]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = 1; o < L; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const int eq = q8_row_exponent(amax);
+            const float inv = q8_exp2i(-eq) * p.qsign;
+            uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+            for (int k = 0; k < E / 2; ++k) {
+              const float a = y[2 * k] * inv, d = y[2 * k + 1] * inv;
+              hi[k] = q8_pack_half2(a, d);
+              const float2 z = q8_half2_floats(hi[k]);
+              lo[k] = q8_pack_half2(a - z.x, d - z.y);
+            }
+            const int rr = wrow0 + (i0 + i) * PER + sub;
+            if constexpr (SPLIT) {                       // 4 elements: half a 16-byte chunk
+              const uint32_t at = qp_chunk(qtile, rr, c >> 1) + (uint32_t)(c & 1) * 8u;
+              qp_st_shared8(at, hi[0], hi[1]);
+              qp_st_shared8(at + kQpTile, lo[0], lo[1]);
+            } else {
+              qp_st_shared16(qp_chunk(qtile, rr, c), hi[0], hi[1], hi[2], hi[3]);
+            }
+            if (c == 0) s_frow[qt * kQpRows + rr] = p.scale * q8_exp2i(eq);
           }
-          qp_st_shared16(qp_chunk(qtile, row, c), hi[0], hi[1], hi[2], hi[3]);
-          if (SPLIT) qp_st_shared16(qp_chunk(qtile + kQpTile, row, c), lo[0], lo[1], lo[2], lo[3]);
         }
+        __syncwarp();
         qp_fence_async();
         pf_arrive(&s_qfull[qt]);
       }
-      // positions of the warp's rows, for the test that a tile needs no mask
-      const int rw0 = r0 + qt * kQpRows + (warp & 3) * 32;
+      const float f_row = s_frow[qt * kQpRows + row];
+      // positions of the warp's rows, for the test that a step needs no mask
+      const int rw0 = r0 + qt * kQpRows + wrow0;
       const int wlo = pbase + min(rw0, R - 1) / p.h, whi = pbase + min(rw0 + 31, R - 1) / p.h;
       const signed char* keb = p.ke + (long long)bg * p.NB;
       const signed char* veb = p.ve + (long long)bg * p.NB;
       float m = -INFINITY, l = 0.0f;
       int ev_top = -128;                               // largest V exponent met so far
+      const int nsteps = 2 * nt;
+      auto step_token = [&](int step) { return tile_token(it0 + (step >> 1)) + kQ8Block * (step & 1); };
+      int ek = keb[step_token(0) / kQ8Block], ev = veb[step_token(0) / kQ8Block];
 #pragma unroll 1
-      for (int it = 0; it < nt; ++it) {
-        const int j0 = tile_token(it0 + it), blk = j0 / kQ8Block, blk1 = min(blk + 1, p.NB - 1);
-        const int ek0 = keb[blk], ek1 = keb[blk1], ev0 = veb[blk], ev1 = veb[blk1];
-        qp_wait(&s_sfull[qt], (uint32_t)it & 1u, &s_abort, p.err);
+      for (int step = 0; step < nsteps; ++step) {
+        const int buf = step & 1, j0 = step_token(step);
+        const float f = q8_factor(f_row, ek), fev = (float)ev;
+        const int ev_now = ev;
+        if (step + 1 < nsteps) {
+          const int blk = min(step_token(step + 1) / kQ8Block, p.NB - 1);
+          ek = keb[blk];
+          ev = veb[blk];
+        }
+        qp_wait(&s_sfull[qt][buf], (uint32_t)(step >> 1) & 1u, &s_abort, p.err);
         tmem_fence_after_sync();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) pf_tmem_ld32(tS + 32u * (uint32_t)c, s[c]);
+        uint32_t s[2][32];
+        pf_tmem_ld32(tS + 64u * (uint32_t)buf, s[0]);
+        pf_tmem_ld32(tS + 64u * (uint32_t)buf + 32u, s[1]);
         pf_tmem_wait(s[0]);
 #pragma unroll
-        for (int c = 1; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(s[c][i]));
-        const bool whole = j0 + kQpKeys - 1 <= wlo &&
-                           (p.window == 0 || j0 > whi - p.window || j0 + kQpKeys <= p.sinks);
+        for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(s[1][i]));
+        const bool whole = j0 + kQ8Block - 1 <= wlo && (p.window == 0 || j0 > whi - p.window || j0 + kQ8Block <= p.sinks);
         if (!whole) {
           const int last = pos - j0, left = p.window > 0 ? last - p.window : -1, sink = p.window > 0 ? p.sinks - j0 : 0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int x = 32 * c + i;
               if (!(x <= last && (x > left || x < sink))) s[c][i] = 0xff800000u;
             }
         }
-        const float f0 = q8_factor(f_row, ek0), f1 = q8_factor(f_row, ek1);
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float a = __uint_as_float(s[c][0]), d = __uint_as_float(s[c][1]);
+          mx[c] = __uint_as_float(s[c >> 1][16 * (c & 1)]);
 #pragma unroll
-          for (int i = 2; i < 32; i += 2) {
-            a = fmaxf(a, __uint_as_float(s[c][i]));
-            d = fmaxf(d, __uint_as_float(s[c][i + 1]));
-          }
-          mx[c] = fmaxf(a, d);
+          for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][16 * (c & 1) + i]));
         }
-        const float cand = fmaxf(fmaxf(mx[0], mx[1]) * f0 + (float)ev0, fmaxf(mx[2], mx[3]) * f1 + (float)ev1);
+        const float cand = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f + fev;
         const bool grow = cand > m + kQpLazy;            // m = -inf: any visible score
         if (__any_sync(0xffffffffu, grow)) {
           const float alpha = grow ? q8_ex2(m - cand) : 1.0f;
@@ -243,7 +264,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             l = q8_rescale(l, m - cand);
             m = cand;
           }
-          if (it > 0) {
+          if (step > 0) {
+            qp_wait(&s_pv[qt], (uint32_t)(step - 1) & 1u, &s_abort, p.err);   // O holds the earlier steps
+            tmem_fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
               uint32_t o[16];
@@ -257,61 +280,56 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
 #pragma unroll
               for (int i = 0; i < 16; i += 2) tmem_st2(tO + 16u * (uint32_t)c + (uint32_t)i, o[i], o[i + 1]);
             }
-            tmem_wait_st();
           }
         }
-        const float mref = (m == -INFINITY ? 0.0f : m) - kQpBias;
-        ev_top = max(ev_top, max(ev0, ev1));
-        float sum[2];
-#pragma unroll
-        for (int hb = 0; hb < 2; ++hb) {                 // the tile's two blocks
-          const int ev = hb ? ev1 : ev0;
-          const float f = hb ? f1 : f0, add = (float)ev - mref;
-          float a0 = 0.0f, a1 = 0.0f, far = 0.0f;
-          if (ev_top - ev > kQ8FarExp) {                 // the denominator's terms on their own (see kQ8FarExp)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) far += q8_ex2(fmaf(__uint_as_float(s[2 * hb + c][i]), f, -mref));
-          }
-          uint32_t w[32];
+        const float mref = (m == -INFINITY ? 0.0f : m) - kQpBias, add = fev - mref;
+        float far = 0.0f;
+        ev_top = max(ev_top, ev_now);
+        if (ev_top - ev_now > kQ8FarExp) {               // the denominator's terms on their own (see kQ8FarExp)
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float x = q8_ex2(fmaf(__uint_as_float(s[2 * hb + c][i]), f, add));
-              const float y = q8_ex2(fmaf(__uint_as_float(s[2 * hb + c][i + 1]), f, add));
-              a0 += x;
-              a1 += y;
-              const uint32_t hw = q8_pack_half2(x, y);
-              w[16 * c + i / 2] = hw;
-              if (SPLIT) {
-                const float2 z = q8_half2_floats(hw);
-                s[2 * hb + c][i / 2] = q8_pack_half2(x - z.x, y - z.y);
-              }
-            }
-          sum[hb] = ev_top - ev > kQ8FarExp ? far : (a0 + a1) * q8_exp2i(-ev);
-          qp_tmem_st32(tS + 32u * (uint32_t)hb, w);
-          if (SPLIT) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) { w[i] = s[2 * hb][i]; w[16 + i] = s[2 * hb + 1][i]; }
-            qp_tmem_st32(tS + 64u + 32u * (uint32_t)hb, w);
-          }
-          // each half of P is handed over as it is ready: its P V runs under the other half's exponentials
-          tmem_wait_st();
-          tmem_fence_before_sync();
-          pf_arrive(&s_pfull[qt][hb]);
+            for (int i = 0; i < 32; ++i) far += q8_ex2(fmaf(__uint_as_float(s[c][i]), f, -mref));
         }
-        l += sum[0] + sum[1];
+        float a0 = 0.0f, a1 = 0.0f;
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float x = q8_ex2(fmaf(__uint_as_float(s[c][i]), f, add));
+            const float y = q8_ex2(fmaf(__uint_as_float(s[c][i + 1]), f, add));
+            a0 += x;
+            a1 += y;
+            const uint32_t hw = q8_pack_half2(x, y);
+            w[16 * c + i / 2] = hw;
+            if (SPLIT) {
+              const float2 z = q8_half2_floats(hw);
+              s[c][i / 2] = q8_pack_half2(x - z.x, y - z.y);
+            }
+          }
+        qp_tmem_st32(tS + 64u * (uint32_t)buf, w);
+        if (SPLIT) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) { w[i] = s[0][i]; w[16 + i] = s[1][i]; }
+          qp_tmem_st32(tS + 64u * (uint32_t)buf + 32u, w);
+        }
+        l += ev_top - ev_now > kQ8FarExp ? far : (a0 + a1) * q8_exp2i(-ev_now);
+        tmem_wait_st();
+        tmem_fence_before_sync();
+        pf_arrive(&s_pfull[qt][buf]);
       }
-      pf_wait(&s_ofull[qt], 0, &s_abort, p.err);
+      qp_wait(&s_pv[qt], (uint32_t)(nsteps - 2) & 1u, &s_abort, p.err);
+      qp_wait(&s_pv[qt], (uint32_t)(nsteps - 1) & 1u, &s_abort, p.err);
       tmem_fence_after_sync();
-      const int rr = r0 + qt * kQpRows + row;
+      // O through shared memory (the query tile's, now free) so that rows go out as full lines, 256 bytes of
+      // each of the warp's 32 rows at a time
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int bad = s_nan_count;
-      float* part = p.part ? p.part + (((long long)split * BG + bg) * R + rr) * kHeadDim : nullptr;
-      T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim;
       const uint8_t* vbase = p.vc + (long long)bg * p.C * kHeadDim;
+      const bool part = p.part != nullptr;
+      const bool wide = part || SPLIT;                   // 32-bit rows: 64 dimensions at a time
+      const int rr = r0 + qt * kQpRows + row;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -328,21 +346,44 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             for (int d = 0; d < 32; ++d)
               if ((v[d] & 0x7f) == 0x7f) o[d] = 0x7fffffffu;
           }
+          __syncwarp();
         }
-        if (rr < R && part) {
+        if (!part) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else if (rr < R) {
+          for (int i = 0; i < 32; ++i) o[i] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+        }
+        if (wide) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float y[8];
+          for (int i = 0; i < 8; ++i)
+            qp_st_shared16(qp_chunk(qtile, row, 8 * (c & 1) + i), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = l == 0.0f ? 0.0f : __uint_as_float(o[i + k]) * inv;
-            q8_store8(dst + 32 * c + i, y);
+          for (int i = 0; i < 4; ++i) {
+            uint32_t h4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              h4[k] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]), __uint_as_float(o[8 * i + 2 * k + 1]));
+            qp_st_shared16(qp_chunk(qtile, row, 4 * c + i), h4[0], h4[1], h4[2], h4[3]);
           }
         }
-        __syncwarp();
+        if (c == 3 || (wide && (c & 1))) {
+          // 16 lanes a row, 2 rows at a time
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const int lr = wrow0 + 2 * i + (lane >> 4), ro = r0 + qt * kQpRows + lr, ch = lane & 15;
+            if (ro < R) {
+              const uint4 x = qp_ld_shared16(qp_chunk(qtile, lr, ch));
+              const int to = ro / p.h, ho = ro - to * p.h;
+              char* dst;
+              if (part) dst = reinterpret_cast<char*>(p.part + (((long long)split * BG + bg) * R + ro) * kHeadDim + 32 * (c - 1));
+              else dst = reinterpret_cast<char*>(static_cast<T*>(p.out) + (((long long)bg * p.h + ho) * p.T + to) * kHeadDim +
+                                                 (wide ? 32 * (c - 1) : 0));
+              *reinterpret_cast<uint4*>(dst + 16 * ch) = x;
+            }
+          }
+          __syncwarp();
+        }
       }
       if (part && rr < R) {
         float* ml = p.part_ml + (((long long)split * BG + bg) * R + rr) * 2;
@@ -442,57 +483,57 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       uint32_t lead;
       asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
       const uint64_t dq = pf_sdesc(s_q, 16, 1024, 2), dk = pf_sdesc(s_k, 16, 1024, 2), dv = pf_sdesc(s_v, kQpHalf, 1024, 2);
-      auto scores = [&](int qt, int st) {               // S = Q K^T
+      const int nsteps = 2 * nt;
+      auto scores = [&](int qt, int step) {             // S = Q K^T for one block of the key tile
+        const uint32_t kb = (uint32_t)((step >> 1) % NS) * kQpTile + (uint32_t)(step & 1) * (kQ8Block * 128u);
 #pragma unroll
         for (int term = 0; term < QP; ++term)
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const uint32_t o = (uint32_t)(ks >> 2) * kQpHalf + (uint32_t)(ks & 3) * 32u;
-            qp_mma_ss(lead, tm + (uint32_t)qt * 128u, dq + (((uint32_t)(qt * QP + term) * kQpTile + o) >> 4),
-                      dk + (((uint32_t)st * kQpTile + o) >> 4), (term | ks) > 0 ? 1u : 0u);
+            qp_mma_ss(lead, tm + (uint32_t)qt * 128u + (uint32_t)(step & 1) * 64u,
+                      dq + (((uint32_t)(qt * QP + term) * kQpTile + o) >> 4), dk + ((kb + o) >> 4), (term | ks) > 0 ? 1u : 0u);
           }
+        qp_commit(lead, &s_sfull[qt][step & 1]);
       };
-      auto values = [&](int qt, int st, int hb, bool first) {   // O += P V over one block (64 tokens) of the tile
+      auto values = [&](int qt, int step) {             // O += P V over the same block
+        const uint32_t vb = (uint32_t)((step >> 1) % NS) * kQpTile + (uint32_t)(step & 1) * (kQ8Block * 128u);
 #pragma unroll
         for (int term = 0; term < QP; ++term)
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4) {
-            const uint32_t ks = (uint32_t)(4 * hb + k4);
-            qp_mma_ts(lead, tm + 256u + (uint32_t)qt * 128u, tm + (uint32_t)qt * 128u + (uint32_t)term * 64u + ks * 8u,
-                      dv + (((uint32_t)st * kQpTile + ks * 2048u) >> 4), (first && term == 0 && ks == 0) ? 0u : 1u);
-          }
+          for (uint32_t ks = 0; ks < 4; ++ks)
+            qp_mma_ts(lead, tm + 256u + (uint32_t)qt * 128u,
+                      tm + (uint32_t)qt * 128u + (uint32_t)(step & 1) * 64u + (uint32_t)term * 32u + ks * 8u,
+                      dv + ((vb + ks * 2048u) >> 4), (step | term | (int)ks) > 0 ? 1u : 0u);
+        qp_commit(lead, &s_pv[qt]);
       };
       qp_wait(&s_kfull[0], 0, &s_abort, p.err);
       for (int qt = 0; qt < ntile; ++qt) {
         qp_wait(&s_qfull[qt], 0, &s_abort, p.err);
         tmem_fence_after_sync();
         scores(qt, 0);
-        qp_commit(lead, &s_sfull[qt]);
+        scores(qt, 1);
       }
       qp_commit(lead, &s_kempty[0]);
 #pragma unroll 1
-      for (int it = 0; it < nt; ++it) {
-        const int st = it % NS, st1 = (it + 1) % NS;
-        const bool more = it + 1 < nt;
-        qp_wait(&s_vfull[st], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
+      for (int step = 0; step < nsteps; ++step) {
+        const int it = step >> 1;
+        const bool odd = step & 1, more = step + 2 < nsteps;
+        if (!odd) qp_wait(&s_vfull[it % NS], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
 #pragma unroll 1
         for (int qt = 0; qt < ntile; ++qt) {
-          qp_wait(&s_pfull[qt][0], (uint32_t)it & 1u, &s_abort, p.err);
+          qp_wait(&s_pfull[qt][odd], (uint32_t)it & 1u, &s_abort, p.err);
           tmem_fence_after_sync();
-          values(qt, st, 0, it == 0);
-          qp_wait(&s_pfull[qt][1], (uint32_t)it & 1u, &s_abort, p.err);
-          tmem_fence_after_sync();
-          values(qt, st, 1, false);
-          if (qt == ntile - 1) qp_commit(lead, &s_vempty[st]);
+          values(qt, step);
+          if (odd && qt == ntile - 1) qp_commit(lead, &s_vempty[it % NS]);
           if (more) {
-            // S's columns hold P until the P V above has read them: MMAs of one thread run in order
-            if (qt == 0) qp_wait(&s_kfull[st1], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
-            tmem_fence_after_sync();
-            scores(qt, st1);
-            qp_commit(lead, &s_sfull[qt]);
-            if (qt == ntile - 1) qp_commit(lead, &s_kempty[st1]);
-          } else {
-            qp_commit(lead, &s_ofull[qt]);
+            // the scores after next go where P was: MMAs of one thread run in order
+            if (!odd && qt == 0) {
+              qp_wait(&s_kfull[(it + 1) % NS], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
+              tmem_fence_after_sync();
+            }
+            scores(qt, step + 2);
+            if (odd && qt == ntile - 1) qp_commit(lead, &s_kempty[(it + 1) % NS]);
           }
         }
       }
