@@ -32,8 +32,8 @@ constexpr size_t kQpSmem = 1024 + 6 * kQpTile;         // 2 Q + 2 K + 2 V tiles,
 constexpr int kQpNanList = 64;
 constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8)
 // Registers a thread after the split: 2 x 128 softmax threads, 128 converting threads, the MMA warp's group.
-// 176 + 176 + 112 + 48 = 512 = 4 x the 128 of the launch.
-constexpr int kQpRegsSoftmax = 176, kQpRegsConvert = 112, kQpRegsMma = 48;
+// 184 + 184 + 104 + 40 = 512 = 4 x the 128 of the launch.
+constexpr int kQpRegsSoftmax = 184, kQpRegsConvert = 104, kQpRegsMma = 40;
 
 // Instruction descriptors (kind::f16): fp32 accumulator, f16 operands, M = 128; Q K^T has N = 64 (a block) and both
 // operands K-major, P V has N = 128 (the head dimension) and V N-major.
@@ -74,6 +74,33 @@ __device__ __forceinline__ void qp_tmem_st32(uint32_t taddr, const uint32_t (&v)
                  "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
                : "memory");
 }
+// 64 consecutive TMEM columns of the thread's lane, defined on return.
+__device__ __forceinline__ void qp_tmem_ld64(uint32_t taddr, uint32_t (&v)[64]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,"
+               "%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                 "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+                 "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
+                 "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
+                 "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]),
+                 "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
+                 "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+               : "r"(taddr) : "memory");
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));
+}
+// Named barriers of a pair of warps: one waits, the other only arrives.
+__device__ __forceinline__ void qp_bar_sync(int id) { asm volatile("bar.sync %0, 64;\n" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void qp_bar_arrive(int id) { asm volatile("bar.arrive %0, 64;\n" ::"r"(id) : "memory"); }
+// Largest of three; a NaN gives way to a number.
+__device__ __forceinline__ float qp_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ void qp_st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -97,7 +124,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
   constexpr int QP = SPLIT ? 2 : 1;                    // f16 terms per query row
   extern __shared__ __align__(1024) unsigned char qp_raw[];
-  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2][2], s_pfull[2][2], s_pv[2];
+  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2][2], s_pfull[2][2], s_pv[2][2];
   __shared__ uint32_t s_taddr;
   __shared__ float s_frow[2 * kQpRows];
   __shared__ int s_nan_count, s_nan[kQpNanList];
@@ -132,8 +159,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       for (int k = 0; k < 2; ++k) {
         mbar_init(&s_sfull[i][k], 1);
         mbar_init(&s_pfull[i][k], kQpRows);
+        mbar_init(&s_pv[i][k], 1);                       // P V of the even, the odd steps
       }
-      mbar_init(&s_pv[i], 1);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&s_kfull[i], 128); mbar_init(&s_kempty[i], 1);
@@ -219,44 +246,48 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       int ev_top = -128;                               // largest V exponent met so far
       const int nsteps = 2 * nt;
       auto step_token = [&](int step) { return tile_token(it0 + (step >> 1)) + kQ8Block * (step & 1); };
-      int ek = keb[step_token(0) / kQ8Block], ev = veb[step_token(0) / kQ8Block];
-#pragma unroll 1
-      for (int step = 0; step < nsteps; ++step) {
+      auto step_block = [&](int step) { return min(step_token(step) / kQ8Block, p.NB - 1); };
+
+      // Scores of a step into registers, hidden ones -inf.
+      auto fetch = [&](uint32_t (&s)[64], int step) {
         const int buf = step & 1, j0 = step_token(step);
-        const float f = q8_factor(f_row, ek), fev = (float)ev;
-        const int ev_now = ev;
-        if (step + 1 < nsteps) {
-          const int blk = min(step_token(step + 1) / kQ8Block, p.NB - 1);
-          ek = keb[blk];
-          ev = veb[blk];
-        }
         qp_wait(&s_sfull[qt][buf], (uint32_t)(step >> 1) & 1u, &s_abort, p.err);
         tmem_fence_after_sync();
-        uint32_t s[2][32];
-        pf_tmem_ld32(tS + 64u * (uint32_t)buf, s[0]);
-        pf_tmem_ld32(tS + 64u * (uint32_t)buf + 32u, s[1]);
-        pf_tmem_wait(s[0]);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(s[1][i]));
+        __syncwarp();
+        qp_tmem_ld64(tS + 64u * (uint32_t)buf, s);
         const bool whole = j0 + kQ8Block - 1 <= wlo && (p.window == 0 || j0 > whi - p.window || j0 + kQ8Block <= p.sinks);
         if (!whole) {
           const int last = pos - j0, left = p.window > 0 ? last - p.window : -1, sink = p.window > 0 ? p.sinks - j0 : 0;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int x = 32 * c + i;
-              if (!(x <= last && (x > left || x < sink))) s[c][i] = 0xff800000u;
-            }
+          for (int x = 0; x < 64; ++x)
+            if (!(x <= last && (x > left || x < sink))) s[x] = 0xff800000u;
         }
-        float mx[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mx[c] = __uint_as_float(s[c >> 1][16 * (c & 1)]);
-#pragma unroll
-          for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][16 * (c & 1) + i]));
+      };
+      // The warps of the two query tiles that share a scheduler (w and w + 4) take turns with their exponentials: side
+      // by side in the same phase both waited for the MUFU pipe and left it idle together.
+      const bool turns = ntile == 2;
+      const int mine = 1 + (warp & 3) + 4 * qt, other = 1 + (warp & 3) + 4 * (1 - qt);
+      if (turns && qt == 1) qp_bar_arrive(other);
+      int ek = keb[step_block(0)], ev = veb[step_block(0)];
+#pragma unroll 1
+      for (int step = 0; step < nsteps; ++step) {
+        const int buf = step & 1;
+        uint32_t s[64];
+        const float f = q8_factor(f_row, ek), fev = (float)ev;
+        const int ev_now = ev;
+        if (step + 1 < nsteps) {
+          const int blk = step_block(step + 1);
+          ek = keb[blk];
+          ev = veb[blk];
         }
-        const float cand = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f + fev;
+        fetch(s, step);
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+          mx[0] = qp_max3(mx[0], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          mx[1] = qp_max3(mx[1], __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+        }
+        const float cand = fmaf(fmaxf(mx[0], mx[1]), f, fev);
         const bool grow = cand > m + kQpLazy;            // m = -inf: any visible score
         if (__any_sync(0xffffffffu, grow)) {
           const float alpha = grow ? q8_ex2(m - cand) : 1.0f;
@@ -265,8 +296,11 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             m = cand;
           }
           if (step > 0) {
-            qp_wait(&s_pv[qt], (uint32_t)(step - 1) & 1u, &s_abort, p.err);   // O holds the earlier steps
+            // O holds every earlier step. (This step's scores came after the P V two steps back, so the barrier's
+            // phase is this one or the next.)
+            qp_wait(&s_pv[qt][1 - buf], (uint32_t)((step - 1) >> 1) & 1u, &s_abort, p.err);
             tmem_fence_after_sync();
+            __syncwarp();
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
               uint32_t o[16];
@@ -283,45 +317,40 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           }
         }
         const float mref = (m == -INFINITY ? 0.0f : m) - kQpBias, add = fev - mref;
-        float far = 0.0f;
         ev_top = max(ev_top, ev_now);
-        if (ev_top - ev_now > kQ8FarExp) {               // the denominator's terms on their own (see kQ8FarExp)
+        float far = 0.0f;
+        const bool is_far = ev_top - ev_now > kQ8FarExp;
+        if (is_far) {                                    // the denominator's terms on their own (see kQ8FarExp)
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) far += q8_ex2(fmaf(__uint_as_float(s[c][i]), f, -mref));
+          for (int i = 0; i < 64; ++i) far += q8_ex2(fmaf(__uint_as_float(s[i]), f, -mref));
         }
-        float a0 = 0.0f, a1 = 0.0f;
-        uint32_t w[32];
+        if (turns) qp_bar_sync(mine);
+        const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
+        float2 sum = make_float2(0.0f, 0.0f);
+        uint32_t w[32], lo[SPLIT ? 32 : 1];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float x = q8_ex2(fmaf(__uint_as_float(s[c][i]), f, add));
-            const float y = q8_ex2(fmaf(__uint_as_float(s[c][i + 1]), f, add));
-            a0 += x;
-            a1 += y;
-            const uint32_t hw = q8_pack_half2(x, y);
-            w[16 * c + i / 2] = hw;
-            if (SPLIT) {
-              const float2 z = q8_half2_floats(hw);
-              s[c][i / 2] = q8_pack_half2(x - z.x, y - z.y);
-            }
+        for (int i = 0; i < 64; i += 2) {
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, add2);
+          const float2 y = make_float2(q8_ex2(x.x), q8_ex2(x.y));
+          sum = __fadd2_rn(sum, y);
+          const uint32_t hw = q8_pack_half2(y.x, y.y);
+          w[i / 2] = hw;
+          if (SPLIT) {
+            const float2 z = q8_half2_floats(hw);
+            lo[SPLIT ? i / 2 : 0] = q8_pack_half2(y.x - z.x, y.y - z.y);
           }
-        qp_tmem_st32(tS + 64u * (uint32_t)buf, w);
-        if (SPLIT) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) { w[i] = s[0][i]; w[16 + i] = s[1][i]; }
-          qp_tmem_st32(tS + 64u * (uint32_t)buf + 32u, w);
         }
-        l += ev_top - ev_now > kQ8FarExp ? far : (a0 + a1) * q8_exp2i(-ev_now);
+        qp_tmem_st32(tS + 64u * (uint32_t)buf, w);
+        if (turns && (qt == 0 || step + 1 < nsteps)) qp_bar_arrive(other);
+        if constexpr (SPLIT) qp_tmem_st32(tS + 64u * (uint32_t)buf + 32u, lo);
+        l += is_far ? far : (sum.x + sum.y) * q8_exp2i(-ev_now);
         tmem_wait_st();
         tmem_fence_before_sync();
         pf_arrive(&s_pfull[qt][buf]);
       }
-      qp_wait(&s_pv[qt], (uint32_t)(nsteps - 2) & 1u, &s_abort, p.err);
-      qp_wait(&s_pv[qt], (uint32_t)(nsteps - 1) & 1u, &s_abort, p.err);
+      qp_wait(&s_pv[qt][1], (uint32_t)(nt - 1) & 1u, &s_abort, p.err);
       tmem_fence_after_sync();
+      __syncwarp();
       // O through shared memory (the query tile's, now free) so that rows go out as full lines, 256 bytes of
       // each of the warp's 32 rows at a time
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -409,23 +438,28 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   } else if (warp < 12) {
     // ---------------------------------------------------------------------------------------------- codes -> f16 tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsConvert));
+    // A tile is converted in two halves of 64 tokens, K's then V's; two halves are in flight in registers while a third
+    // is converted (32 registers: more would be taken from the softmax threads).
     const int rw = (warp - 8) * 4 + (lane >> 3), c8 = lane & 7;     // row within a group of 16, 16-code piece of the row
     const long long off = (long long)bg * p.C * kHeadDim + 16 * c8;
-    uint4 kr[8], vr[8];
-    auto load = [&](const uint8_t* codes, int it, uint4 (&x)[8]) {
-      const int j0 = tile_token(it0 + it);
+    const uint8_t* const codes[2] = {p.kc + off, p.vc + off};
+    // half u of the walk: tile u / 4, K for u % 4 < 2, V after
+    auto load = [&](int u, uint4 (&x)[4]) {
+      if (u >= 4 * nt) return;
+      const int j0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1) + rw;
+      const uint8_t* src = codes[(u >> 1) & 1];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = j0 + 16 * i + rw;
-        x[i] = j < n ? __ldg(reinterpret_cast<const uint4*>(codes + off + (long long)j * kHeadDim)) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 16 * i;
+        x[i] = j < n ? __ldg(reinterpret_cast<const uint4*>(src + (long long)j * kHeadDim)) : make_uint4(0, 0, 0, 0);
       }
     };
-    auto store = [&](uint32_t dst, const uint4 (&x)[8]) {
-      // pieces 4-7 of a row (the second half) write their two chunks in the other order: no two lanes of a quarter
-      // warp share a bank
+    auto store = [&](uint32_t dst, const uint4 (&x)[4]) {
+      // pieces 4-7 of a row (the second 64 dimensions) write their two chunks in the other order: no two lanes of a
+      // quarter warp share a bank
       const int first = c8 >> 2;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const int r = 16 * i + rw;
         const uint32_t lo[4] = {q8_decode_lo(x[i].x), q8_decode_hi(x[i].x), q8_decode_lo(x[i].y), q8_decode_hi(x[i].y)};
         const uint32_t hi[4] = {q8_decode_lo(x[i].z), q8_decode_hi(x[i].z), q8_decode_lo(x[i].w), q8_decode_hi(x[i].w)};
@@ -439,42 +473,45 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
         }
       }
     };
-    if (nt > 0) { load(p.kc, 0, kr); load(p.vc, 0, vr); }
+    auto drop_nan = [&](int u, uint4 (&x)[4]) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bad |= q8_nan_mask(x[i].x) | q8_nan_mask(x[i].y) | q8_nan_mask(x[i].z) | q8_nan_mask(x[i].w);
+      if (!bad) return;
+      const int j0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1) + rw;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (q8_nan_mask(x[i].x) | q8_nan_mask(x[i].y) | q8_nan_mask(x[i].z) | q8_nan_mask(x[i].w)) {
+          const int at = atomicAdd(&s_nan_count, 1);
+          if (at < kQpNanList) s_nan[at] = j0 + 16 * i;
+        }
+        x[i] = make_uint4(q8_drop_nan(x[i].x), q8_drop_nan(x[i].y), q8_drop_nan(x[i].z), q8_drop_nan(x[i].w));
+      }
+    };
+    uint4 xa[4], xb[4];
+    load(0, xa);
+    load(1, xb);
 #pragma unroll 1
     for (int it = 0; it < nt; ++it) {
       const int st = it % NS;
-      const uint32_t par = (uint32_t)(it / NS) & 1u;
-      qp_wait(&s_kempty[st], par ^ 1u, &s_abort, p.err);
-      store(s_k + (uint32_t)st * kQpTile, kr);
+      const uint32_t par = ((uint32_t)(it / NS) & 1u) ^ 1u;
+      const uint32_t tk = s_k + (uint32_t)st * kQpTile, tv = s_v + (uint32_t)st * kQpTile;
+      qp_wait(&s_kempty[st], par, &s_abort, p.err);
+      store(tk, xa);
+      load(4 * it + 2, xa);
+      store(tk + kQ8Block * 128u, xb);
+      load(4 * it + 3, xb);
       qp_fence_async();
       pf_arrive(&s_kfull[st]);
-      if (it + 1 < nt) load(p.kc, it + 1, kr);
-      uint32_t bad = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) bad |= q8_nan_mask(vr[i].x) | q8_nan_mask(vr[i].y) | q8_nan_mask(vr[i].z) | q8_nan_mask(vr[i].w);
-      if (bad) {
-        const int j0 = tile_token(it0 + it);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-          uint32_t any = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            any |= q8_nan_mask(w[k]);
-            w[k] = q8_drop_nan(w[k]);
-          }
-          vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
-          if (any) {
-            const int at = atomicAdd(&s_nan_count, 1);
-            if (at < kQpNanList) s_nan[at] = j0 + 16 * i + rw;
-          }
-        }
-      }
-      qp_wait(&s_vempty[st], par ^ 1u, &s_abort, p.err);
-      store(s_v + (uint32_t)st * kQpTile, vr);
+      drop_nan(4 * it + 2, xa);
+      qp_wait(&s_vempty[st], par, &s_abort, p.err);
+      store(tv, xa);
+      load(4 * it + 4, xa);
+      drop_nan(4 * it + 3, xb);
+      store(tv + kQ8Block * 128u, xb);
+      load(4 * it + 5, xb);
       qp_fence_async();
       pf_arrive(&s_vfull[st]);
-      if (it + 1 < nt) load(p.vc, it + 1, vr);
     }
   } else {
     // ---------------------------------------------------------------------------------------------- MMAs
@@ -505,7 +542,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             qp_mma_ts(lead, tm + 256u + (uint32_t)qt * 128u,
                       tm + (uint32_t)qt * 128u + (uint32_t)(step & 1) * 64u + (uint32_t)term * 32u + ks * 8u,
                       dv + ((vb + ks * 2048u) >> 4), (step | term | (int)ks) > 0 ? 1u : 0u);
-        qp_commit(lead, &s_pv[qt]);
+        qp_commit(lead, &s_pv[qt][step & 1]);
       };
       qp_wait(&s_kfull[0], 0, &s_abort, p.err);
       for (int qt = 0; qt < ntile; ++qt) {

@@ -449,6 +449,26 @@ def test_attend_repeats_bit_for_bit_and_flags_bad_lengths():
         check_attend(cache, q, [3000, 0], 0, 0, c)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_prompts_alone_and_back_to_back(dtype):
+    """Short ragged prompts split over the keys, two query tiles a CTA, launched many times alone and back to back: the
+    same bits every time and no wait that gives up (late warps must find every barrier's phase)."""
+    cache = random_cache(11, 5, 2, 700)
+    q = make_q(5, 5, 2, 3, 333, dtype)
+    lengths = [641, 201, 311, 531, 421]
+    on_gpu = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    want = al().attend_q8(q, cache, on_gpu)
+    assert status() == 0
+    check_attend(cache, q[:2], lengths, 0, 0, want[:2])
+    for alone in (True, False):
+        for _ in range(60):
+            got = al().attend_q8(q, cache, on_gpu)
+            if alone:
+                torch.cuda.synchronize()
+                assert status() == 0
+        assert torch.equal(got, want) and status() == 0
+
+
 def test_misaligned_queries_are_copied():
     cache = random_cache(5, 1, 2, 100)
     wide = torch.randn(1, 2, 3, 1, 131, device=DEV)
