@@ -11,7 +11,7 @@
 //                   a row's maximum grew by more than 2^8 (weights up to 2^14 fit f16)
 //   warps 8-11      read the codes from global memory, convert them to f16 (exact) and store them in the 128-byte
 //                   swizzled layout both contractions read; the next tile's codes are in registers meanwhile
-//   warp 12         issues the MMAs
+//   warps 12, 13    issue the MMAs, one per query tile
 // 16-bit queries are one f16 operand (scaled by a power of two per row, exact). 32-bit queries and their weights are
 // split into two f16 terms (SPLIT): twice the MMAs, about 21 bits, single-buffered key tiles.
 //
@@ -92,9 +92,6 @@ __device__ __forceinline__ void qp_tmem_ld64(uint32_t taddr, uint32_t (&v)[64]) 
 #pragma unroll
   for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));
 }
-// Named barriers of a pair of warps: one waits, the other only arrives.
-__device__ __forceinline__ void qp_bar_sync(int id) { asm volatile("bar.sync %0, 64;\n" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void qp_bar_arrive(int id) { asm volatile("bar.arrive %0, 64;\n" ::"r"(id) : "memory"); }
 // Largest of three; a NaN gives way to a number.
 __device__ __forceinline__ float qp_max3(float a, float b, float c) {
   float d;
@@ -130,7 +127,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   __shared__ int s_nan_count, s_nan[kQpNanList];
   __shared__ volatile int s_abort;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // What steers the MMA warps is broadcast from lane 0, so that the compiler knows it to be the same in a warp and keeps
+  // descriptors and branches in the uniform datapath (otherwise every MMA takes some 45 instructions).
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t base = (smem_addr(qp_raw) + 1023u) & ~1023u;
   const uint32_t s_q = base, s_k = base + 2 * QP * kQpTile, s_v = s_k + NS * kQpTile;
 
@@ -139,7 +138,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   const int split = blockIdx.y;
   const int tile = p.row_tiles - 1 - (int)(blockIdx.x / BG), bg = (int)(blockIdx.x % BG);
   const int b = bg / p.G, g = bg - b * p.G;
-  int n = q8_length(p.len, b);
+  int n = __shfl_sync(0xffffffffu, q8_length(p.len, b), 0);
   if (n < 0 || n > p.C) {
     if (tid == 0) atomicOr(p.err, kErrQ8Range);
     n = max(0, min(n, p.C));
@@ -163,8 +162,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       }
     }
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&s_kfull[i], 128); mbar_init(&s_kempty[i], 1);
-      mbar_init(&s_vfull[i], 128); mbar_init(&s_vempty[i], 1);
+      mbar_init(&s_kfull[i], 128); mbar_init(&s_kempty[i], ntile);
+      mbar_init(&s_vfull[i], 128); mbar_init(&s_vempty[i], ntile);
     }
     mbar_init_fence();
     s_nan_count = 0;
@@ -174,7 +173,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   tmem_fence_before_sync();
   __syncthreads();
   tmem_fence_after_sync();
-  const uint32_t tm = s_taddr;                          // S0 | S1 | O0 | O1, 128 columns each
+  const uint32_t tm = __shfl_sync(0xffffffffu, s_taddr, 0);                          // S0 | S1 | O0 | O1, 128 columns each
 
   if (warp < 8) {
     // ---------------------------------------------------------------------------------------------- query rows
@@ -263,11 +262,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             if (!(x <= last && (x > left || x < sink))) s[x] = 0xff800000u;
         }
       };
-      // The warps of the two query tiles that share a scheduler (w and w + 4) take turns with their exponentials: side
-      // by side in the same phase both waited for the MUFU pipe and left it idle together.
-      const bool turns = ntile == 2;
-      const int mine = 1 + (warp & 3) + 4 * qt, other = 1 + (warp & 3) + 4 * (1 - qt);
-      if (turns && qt == 1) qp_bar_arrive(other);
       int ek = keb[step_block(0)], ev = veb[step_block(0)];
 #pragma unroll 1
       for (int step = 0; step < nsteps; ++step) {
@@ -324,7 +318,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
 #pragma unroll
           for (int i = 0; i < 64; ++i) far += q8_ex2(fmaf(__uint_as_float(s[i]), f, -mref));
         }
-        if (turns) qp_bar_sync(mine);
         const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
         float2 sum = make_float2(0.0f, 0.0f);
         uint32_t w[32], lo[SPLIT ? 32 : 1];
@@ -341,7 +334,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           }
         }
         qp_tmem_st32(tS + 64u * (uint32_t)buf, w);
-        if (turns && (qt == 0 || step + 1 < nsteps)) qp_bar_arrive(other);
         if constexpr (SPLIT) qp_tmem_st32(tS + 64u * (uint32_t)buf + 32u, lo);
         l += is_far ? far : (sum.x + sum.y) * q8_exp2i(-ev_now);
         tmem_wait_st();
@@ -516,62 +508,62 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   } else {
     // ---------------------------------------------------------------------------------------------- MMAs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsMma));
-    if (warp == 12 && nt > 0) {
+    const int qt = warp - 12;
+    if (qt < ntile && nt > 0) {
       uint32_t lead;
       asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
-      const uint64_t dq = pf_sdesc(s_q, 16, 1024, 2), dk = pf_sdesc(s_k, 16, 1024, 2), dv = pf_sdesc(s_v, kQpHalf, 1024, 2);
-      const int nsteps = 2 * nt;
-      auto scores = [&](int qt, int step) {             // S = Q K^T for one block of the key tile
+      const uint64_t dq = pf_sdesc(s_q + (uint32_t)(qt * QP) * kQpTile, 16, 1024, 2), dk = pf_sdesc(s_k, 16, 1024, 2),
+                     dv = pf_sdesc(s_v, kQpHalf, 1024, 2);
+      const uint32_t tS = tm + (uint32_t)qt * 128u, tO = tm + 256u + (uint32_t)qt * 128u;
+      auto scores = [&](int step) {                     // S = Q K^T for one block of the key tile
         const uint32_t kb = (uint32_t)((step >> 1) % NS) * kQpTile + (uint32_t)(step & 1) * (kQ8Block * 128u);
 #pragma unroll
         for (int term = 0; term < QP; ++term)
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const uint32_t o = (uint32_t)(ks >> 2) * kQpHalf + (uint32_t)(ks & 3) * 32u;
-            qp_mma_ss(lead, tm + (uint32_t)qt * 128u + (uint32_t)(step & 1) * 64u,
-                      dq + (((uint32_t)(qt * QP + term) * kQpTile + o) >> 4), dk + ((kb + o) >> 4), (term | ks) > 0 ? 1u : 0u);
+            qp_mma_ss(lead, tS + (uint32_t)(step & 1) * 64u, dq + (((uint32_t)term * kQpTile + o) >> 4),
+                      dk + ((kb + o) >> 4), (term | ks) > 0 ? 1u : 0u);
           }
         qp_commit(lead, &s_sfull[qt][step & 1]);
       };
-      auto values = [&](int qt, int step) {             // O += P V over the same block
+      auto values = [&](int step) {                     // O += P V over the same block
         const uint32_t vb = (uint32_t)((step >> 1) % NS) * kQpTile + (uint32_t)(step & 1) * (kQ8Block * 128u);
 #pragma unroll
         for (int term = 0; term < QP; ++term)
 #pragma unroll
           for (uint32_t ks = 0; ks < 4; ++ks)
-            qp_mma_ts(lead, tm + 256u + (uint32_t)qt * 128u,
-                      tm + (uint32_t)qt * 128u + (uint32_t)(step & 1) * 64u + (uint32_t)term * 32u + ks * 8u,
+            qp_mma_ts(lead, tO, tS + (uint32_t)(step & 1) * 64u + (uint32_t)term * 32u + ks * 8u,
                       dv + ((vb + ks * 2048u) >> 4), (step | term | (int)ks) > 0 ? 1u : 0u);
         qp_commit(lead, &s_pv[qt][step & 1]);
       };
       qp_wait(&s_kfull[0], 0, &s_abort, p.err);
-      for (int qt = 0; qt < ntile; ++qt) {
-        qp_wait(&s_qfull[qt], 0, &s_abort, p.err);
-        tmem_fence_after_sync();
-        scores(qt, 0);
-        scores(qt, 1);
-      }
+      qp_wait(&s_qfull[qt], 0, &s_abort, p.err);
+      tmem_fence_after_sync();
+      scores(0);
+      scores(1);
       qp_commit(lead, &s_kempty[0]);
 #pragma unroll 1
-      for (int step = 0; step < nsteps; ++step) {
-        const int it = step >> 1;
-        const bool odd = step & 1, more = step + 2 < nsteps;
-        if (!odd) qp_wait(&s_vfull[it % NS], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
-#pragma unroll 1
-        for (int qt = 0; qt < ntile; ++qt) {
-          qp_wait(&s_pfull[qt][odd], (uint32_t)it & 1u, &s_abort, p.err);
+      for (int it = 0; it < nt; ++it) {
+        const bool more = it + 1 < nt;
+        const uint32_t par = (uint32_t)it & 1u;
+        qp_wait(&s_vfull[it % NS], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
+        qp_wait(&s_pfull[qt][0], par, &s_abort, p.err);
+        tmem_fence_after_sync();
+        values(2 * it);
+        if (more) {
+          // the scores of the next tile go where P was: MMAs of one thread run in order
+          qp_wait(&s_kfull[(it + 1) % NS], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
           tmem_fence_after_sync();
-          values(qt, step);
-          if (odd && qt == ntile - 1) qp_commit(lead, &s_vempty[it % NS]);
-          if (more) {
-            // the scores after next go where P was: MMAs of one thread run in order
-            if (!odd && qt == 0) {
-              qp_wait(&s_kfull[(it + 1) % NS], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
-              tmem_fence_after_sync();
-            }
-            scores(qt, step + 2);
-            if (odd && qt == ntile - 1) qp_commit(lead, &s_kempty[(it + 1) % NS]);
-          }
+          scores(2 * it + 2);
+        }
+        qp_wait(&s_pfull[qt][1], par, &s_abort, p.err);
+        tmem_fence_after_sync();
+        values(2 * it + 1);
+        qp_commit(lead, &s_vempty[it % NS]);
+        if (more) {
+          scores(2 * it + 3);
+          qp_commit(lead, &s_kempty[(it + 1) % NS]);
         }
       }
     }
