@@ -74,7 +74,8 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
 int q8_attend_check(int B, int G, int h, int T, int C, int window, int sinks) {
   if (h < 1 || T < 0) return fail(AL_EINVAL, "h must be positive and T not negative, got h=%d T=%d", h, T);
   if (window < 0 || sinks < 0) return fail(AL_EINVAL, "window and sinks must not be negative, got %d and %d", window, sinks);
-  if ((long long)h * T > (1 << 28)) return fail(AL_EUNSUPPORTED, "h*T = %lld exceeds 2^28 query rows per group", (long long)h * T);
+  if (h > 64) return fail(AL_EUNSUPPORTED, "heads per group must be in [1, 64], got %d", h);
+  if ((long long)h * T > (1 << 25)) return fail(AL_EUNSUPPORTED, "h*T = %lld exceeds 2^25 query rows per group", (long long)h * T);
   if (B * (long long)G * (((long long)h * T + 255) / 256) > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query tiles");
   (void)C;
   return AL_OK;
@@ -276,6 +277,7 @@ int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_
   p.scale = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
   p.qsign = scale < 0 ? -1.0f : 1.0f;
   p.out = out; p.nsplit = pl.nsplit; p.row_tiles = pl.row_tiles; p.err = di->err;
+  p.h_magic = h > 1 ? 0xffffffffu / (unsigned)h + 1u : 0u;   // exact for r < 2^25, h <= 64: r * (h_magic * h - 2^32) < 2^32
   if (pl.bytes > 0) {
     p.part = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.ml_off);

@@ -41,6 +41,7 @@ struct Q8AttendParams {
   void* out;                               // [B,G,h,T,128] contiguous
   // tensor-core kernel for prompts: split of the key tiles and its partial results
   int nsplit, row_tiles;
+  uint32_t h_magic;                        // r / h = (r * h_magic) >> 32 for the row numbers used (h > 1)
   float* part;                             // [nsplit][B*G][R][128] unnormalised O, R = T * h
   float* part_ml;                          // [nsplit][B*G][R][2]
   unsigned* err;

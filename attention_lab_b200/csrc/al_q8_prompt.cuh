@@ -43,27 +43,42 @@ constexpr uint32_t kQpIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kHeadDim >>
 // The MMA warp runs its loop with all lanes (waits, addresses and descriptors stay warp-uniform, so they live in uniform
 // registers); `lead`, set in one lane, predicates the instructions one thread issues. With the loop inside a lane-0
 // branch every MMA took two to four register moves and each wait about 300 cycles.
-__device__ __forceinline__ void qp_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-               ::"r"(d), "l"(a), "l"(b), "r"(kQpIdescQK), "r"(accumulate), "r"(lead) : "memory");
+// Descriptors are passed as their low word (address and leading offset); the high word is the same for all tiles here.
+constexpr uint32_t kQpDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);   // 8-row stride 1 KB, version 1, 128-byte swizzle
+__device__ __forceinline__ void qp_mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p, q;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+               " mov.b64 da, {%1, %6};\n mov.b64 db, {%2, %6};\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "r"(b), "r"(kQpIdescQK), "r"(accumulate), "r"(lead), "r"(kQpDescHigh) : "memory");
 }
-__device__ __forceinline__ void qp_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-               ::"r"(d), "r"(a), "l"(b), "r"(kQpIdescPV), "r"(accumulate), "r"(lead) : "memory");
+__device__ __forceinline__ void qp_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p, q;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+               " mov.b64 db, {%2, %6};\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "r"(b), "r"(kQpIdescPV), "r"(accumulate), "r"(lead), "r"(kQpDescHigh) : "memory");
 }
 __device__ __forceinline__ void qp_commit(uint32_t lead, uint64_t* bar) {
   asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
                " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n"
                ::"r"(smem_addr(bar)), "r"(lead) : "memory");
 }
-// pf_wait with the common case (the phase is complete) tested before anything else.
+// Bounded wait for the phase with parity `parity`, small enough to be inlined everywhere (pf_wait's loop took 2 KB of
+// code a place, and the warps of this kernel live off the instruction cache). Gives up like pf_wait.
 __device__ __forceinline__ void qp_wait(uint64_t* bar, unsigned parity, volatile int* abort_flag, unsigned* err) {
+  const uint32_t a = smem_addr(bar);
   uint32_t done;
   asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-               : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
-  if (!done) pf_wait(bar, parity, abort_flag, err);
+               : "=r"(done) : "r"(a), "r"(parity) : "memory");
+  if (done || *abort_flag) return;
+  asm volatile("{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+               "WAIT:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+               " add.u32 n, n, 1;\n setp.lt.and.u32 q, n, %3, !p;\n @q bra WAIT;\n"
+               " selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(done) : "r"(a), "r"(parity), "r"((uint32_t)kWaitPolls) : "memory");
+  if (!done) {
+    *abort_flag = 1;
+    atomicOr(err, kErrWaitLimit);
+  }
 }
 __device__ __forceinline__ void qp_tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -92,6 +107,11 @@ __device__ __forceinline__ void qp_tmem_ld64(uint32_t taddr, uint32_t (&v)[64]) 
 #pragma unroll
   for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));
 }
+// Named barriers of a pair of warps: one waits, the other only arrives.
+__device__ __forceinline__ void qp_bar_sync(int id) { asm volatile("bar.sync %0, 64;\n" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void qp_bar_arrive(int id) { asm volatile("bar.arrive %0, 64;\n" ::"r"(id) : "memory"); }
+// The n lowest bits (n is clamped to [0, 64]).
+__device__ __forceinline__ uint64_t qp_low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; }
 // Largest of three; a NaN gives way to a number.
 __device__ __forceinline__ float qp_max3(float a, float b, float c) {
   float d;
@@ -115,13 +135,18 @@ __device__ __forceinline__ uint32_t qp_chunk(uint32_t tile, int r, int c) {
   return tile + (uint32_t)(c >> 3) * kQpHalf + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4);
 }
 
+// r / h for a query row.
+__device__ __forceinline__ int qp_row_token(int r, const Q8AttendParams& p) {
+  return p.h == 1 ? r : (int)__umulhi((uint32_t)r, p.h_magic);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8AttendParams p) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
   constexpr int QP = SPLIT ? 2 : 1;                    // f16 terms per query row
   extern __shared__ __align__(1024) unsigned char qp_raw[];
-  __shared__ uint64_t s_qfull[2], s_kfull[NS], s_kempty[NS], s_vfull[NS], s_vempty[NS], s_sfull[2][2], s_pfull[2][2], s_pv[2][2];
+  __shared__ uint64_t s_qfull[2], s_full[2][NS], s_empty[2][NS], s_sfull[2][2], s_pfull[2][2], s_pv[2][2];
   __shared__ uint32_t s_taddr;
   __shared__ float s_frow[2 * kQpRows];
   __shared__ int s_nan_count, s_nan[kQpNanList];
@@ -146,7 +171,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   const int r0 = tile * 2 * kQpRows;
   const int ntile = r0 + kQpRows < R ? 2 : 1;
   const int pbase = n - p.T;
-  const int plo = pbase + r0 / p.h, phi = pbase + min(r0 + 2 * kQpRows - 1, R - 1) / p.h;
+  const int plo = pbase + qp_row_token(r0, p), phi = pbase + qp_row_token(min(r0 + 2 * kQpRows - 1, R - 1), p);
   const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQpKeys);
   const int it0 = (int)((long long)rg.total * split / p.nsplit), it1 = (int)((long long)rg.total * (split + 1) / p.nsplit);
   const int nt = it1 - it0;
@@ -162,8 +187,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       }
     }
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&s_kfull[i], 128); mbar_init(&s_kempty[i], ntile);
-      mbar_init(&s_vfull[i], 128); mbar_init(&s_vempty[i], ntile);
+      for (int kv = 0; kv < 2; ++kv) { mbar_init(&s_full[kv][i], 128); mbar_init(&s_empty[kv][i], ntile); }
     }
     mbar_init_fence();
     s_nan_count = 0;
@@ -181,33 +205,37 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     const int qt = warp >> 2, row = tid & 127;
     if (qt < ntile && nt > 0) {
       const int r = min(r0 + qt * kQpRows + row, R - 1);
-      const int t = r / p.h, pos = pbase + t;
+      const int pos = pbase + qp_row_token(r, p);
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t tS = tm + lanes + (uint32_t)qt * 128u, tO = tm + lanes + 256u + (uint32_t)qt * 128u;
       const int wrow0 = (warp & 3) * 32;               // the warp's first row of the tile
       const uint32_t qtile = s_q + (uint32_t)(qt * QP) * kQpTile;
-      // The warp's 32 query rows: L lanes read one row (full lines), all loads of a batch in flight, then scale by the
-      // row's power of two, split and store.
+      // The warp's 32 query rows: L lanes read one row (full lines), BATCH loads in flight while the batch before is
+      // scaled by its rows' powers of two, split and stored.
       {
-        constexpr int L = kHeadDim * (int)sizeof(T) / 16, PER = 32 / L, BATCH = 16;
+        constexpr int E = V16<T>::n, L = kHeadDim / E, PER = 32 / L, BATCH = 4;
         const int sub = lane / L, c = lane % L;
+        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + E * c;
+        uint4 x[BATCH];
+        auto ask = [&](int i0) {
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int rq = min(r0 + qt * kQpRows + wrow0 + (i0 + i) * PER + sub, R - 1), tq = qp_row_token(rq, p);
+            x[i] = __ldg(reinterpret_cast<const uint4*>(src + (rq - tq * p.h) * p.q_sh + tq * p.q_st));
+          }
+        };
+        ask(0);
 #pragma unroll 1
         for (int i0 = 0; i0 < 32 / PER; i0 += BATCH) {
-          uint4 x[BATCH];
+          float y[BATCH][E];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) unpack(x[i], y[i], static_cast<const T*>(p.q));
+          if (i0 + BATCH < 32 / PER) ask(i0 + BATCH);
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
-            const int rq = min(r0 + qt * kQpRows + wrow0 + (i0 + i) * PER + sub, R - 1), tq = rq / p.h;
-            const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + (rq - tq * p.h) * p.q_sh + tq * p.q_st;
-            x[i] = __ldg(reinterpret_cast<const uint4*>(src) + c);
-          }
-#pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            constexpr int E = V16<T>::n;
-            float y[E];
-            unpack(x[i], y, static_cast<const T*>(p.q));
             uint32_t amax = 0;
 #pragma unroll
-            for (int k = 0; k < E; ++k) amax = max(amax, __float_as_uint(y[k]) & 0x7fffffffu);
+            for (int k = 0; k < E; ++k) amax = max(amax, __float_as_uint(y[i][k]) & 0x7fffffffu);
 #pragma unroll
             for (int o = 1; o < L; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             const int eq = q8_row_exponent(amax);
@@ -215,7 +243,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             uint32_t hi[E / 2], lo[E / 2];
 #pragma unroll
             for (int k = 0; k < E / 2; ++k) {
-              const float a = y[2 * k] * inv, d = y[2 * k + 1] * inv;
+              const float a = y[i][2 * k] * inv, d = y[i][2 * k + 1] * inv;
               hi[k] = q8_pack_half2(a, d);
               const float2 z = q8_half2_floats(hi[k]);
               lo[k] = q8_pack_half2(a - z.x, d - z.y);
@@ -238,7 +266,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       const float f_row = s_frow[qt * kQpRows + row];
       // positions of the warp's rows, for the test that a step needs no mask
       const int rw0 = r0 + qt * kQpRows + wrow0;
-      const int wlo = pbase + min(rw0, R - 1) / p.h, whi = pbase + min(rw0 + 31, R - 1) / p.h;
+      const int wlo = pbase + qp_row_token(min(rw0, R - 1), p), whi = pbase + qp_row_token(min(rw0 + 31, R - 1), p);
       const signed char* keb = p.ke + (long long)bg * p.NB;
       const signed char* veb = p.ve + (long long)bg * p.NB;
       float m = -INFINITY, l = 0.0f;
@@ -248,20 +276,31 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       auto step_block = [&](int step) { return min(step_token(step) / kQ8Block, p.NB - 1); };
 
       // Scores of a step into registers, hidden ones -inf.
-      auto fetch = [&](uint32_t (&s)[64], int step) {
-        const int buf = step & 1, j0 = step_token(step);
+      auto fetch = [&](uint32_t (&s)[64], int step, int j0) {
+        const int buf = step & 1;
         qp_wait(&s_sfull[qt][buf], (uint32_t)(step >> 1) & 1u, &s_abort, p.err);
         tmem_fence_after_sync();
         __syncwarp();
         qp_tmem_ld64(tS + 64u * (uint32_t)buf, s);
         const bool whole = j0 + kQ8Block - 1 <= wlo && (p.window == 0 || j0 > whi - p.window || j0 + kQ8Block <= p.sinks);
         if (!whole) {
+          // the visible columns as bits: [0, last], less those at or below `left` that are no sinks
           const int last = pos - j0, left = p.window > 0 ? last - p.window : -1, sink = p.window > 0 ? p.sinks - j0 : 0;
+          const uint64_t seen = qp_low_bits(last + 1) & (~qp_low_bits(left + 1) | qp_low_bits(sink));
+          const uint32_t m0 = (uint32_t)seen, m1 = (uint32_t)(seen >> 32);
 #pragma unroll
-          for (int x = 0; x < 64; ++x)
-            if (!(x <= last && (x > left || x < sink))) s[x] = 0xff800000u;
+          for (int i = 0; i < 32; ++i) {
+            if (!(m0 & (1u << i))) s[i] = 0xff800000u;
+            if (!(m1 & (1u << i))) s[32 + i] = 0xff800000u;
+          }
         }
       };
+      // The warps of the two query tiles that share a scheduler (w and w + 4) take turns with their exponentials: side
+      // by side in the same phase both wait for the MUFU pipe and then leave it idle together (602 -> 587 us for 8192
+      // tokens of 32/8 heads).
+      const bool turns = ntile == 2;
+      const int mine = 1 + (warp & 3) + 4 * qt, other = 1 + (warp & 3) + 4 * (1 - qt);
+      if (turns && qt == 1) qp_bar_arrive(other);
       int ek = keb[step_block(0)], ev = veb[step_block(0)];
 #pragma unroll 1
       for (int step = 0; step < nsteps; ++step) {
@@ -274,7 +313,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           ek = keb[blk];
           ev = veb[blk];
         }
-        fetch(s, step);
+        const int j0 = step_token(step);
+        fetch(s, step, j0);
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 64; i += 4) {
@@ -314,10 +354,21 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
         ev_top = max(ev_top, ev_now);
         float far = 0.0f;
         const bool is_far = ev_top - ev_now > kQ8FarExp;
-        if (is_far) {                                    // the denominator's terms on their own (see kQ8FarExp)
+        if (is_far) {
+          // the denominator's terms on their own (see kQ8FarExp), from the scores still in TMEM: a rare path, kept small
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 8) {
+            uint32_t x[8];
+            tmem_ld8(tS + 64u * (uint32_t)buf + (uint32_t)c, x);
+            tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 64; ++i) far += q8_ex2(fmaf(__uint_as_float(s[i]), f, -mref));
+            for (int i = 0; i < 8; ++i) {
+              asm volatile("" : "+r"(x[i]));
+              if (q8_sees(pos, j0 + c + i, p.window, p.sinks)) far += q8_ex2(fmaf(__uint_as_float(x[i]), f, -mref));
+            }
+          }
         }
+        if (turns) qp_bar_sync(mine);
         const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
         float2 sum = make_float2(0.0f, 0.0f);
         uint32_t w[32], lo[SPLIT ? 32 : 1];
@@ -333,6 +384,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             lo[SPLIT ? i / 2 : 0] = q8_pack_half2(y.x - z.x, y.y - z.y);
           }
         }
+        if (turns && (qt == 0 || step + 1 < nsteps)) qp_bar_arrive(other);
         qp_tmem_st32(tS + 64u * (uint32_t)buf, w);
         if constexpr (SPLIT) qp_tmem_st32(tS + 64u * (uint32_t)buf + 32u, lo);
         l += is_far ? far : (sum.x + sum.y) * q8_exp2i(-ev_now);
@@ -362,10 +414,14 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           for (int i = 0; i < cnt; ++i) {
             const int j = bad <= kQpNanList ? s_nan[i] : tile_token(it0 + i / kQpKeys) + i % kQpKeys;
             if (j >= n || !q8_sees(pos, j, p.window, p.sinks)) continue;
-            const uint8_t* v = vbase + (long long)j * kHeadDim + 32 * c;
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(vbase + (long long)j * kHeadDim + 32 * c);
 #pragma unroll
-            for (int d = 0; d < 32; ++d)
-              if ((v[d] & 0x7f) == 0x7f) o[d] = 0x7fffffffu;
+            for (int d = 0; d < 8; ++d) {
+              const uint32_t bits = q8_nan_mask(v[d]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (bits & (0x80u << (8 * k))) o[4 * d + k] = 0x7fffffffu;
+            }
           }
           __syncwarp();
         }
@@ -395,7 +451,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             const int lr = wrow0 + 2 * i + (lane >> 4), ro = r0 + qt * kQpRows + lr, ch = lane & 15;
             if (ro < R) {
               const uint4 x = qp_ld_shared16(qp_chunk(qtile, lr, ch));
-              const int to = ro / p.h, ho = ro - to * p.h;
+              const int to = qp_row_token(ro, p), ho = ro - to * p.h;
               char* dst;
               if (part) dst = reinterpret_cast<char*>(p.part + (((long long)split * BG + bg) * R + ro) * kHeadDim + 32 * (c - 1));
               else dst = reinterpret_cast<char*>(static_cast<T*>(p.out) + (((long long)bg * p.h + ho) * p.T + to) * kHeadDim +
@@ -420,7 +476,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           ml[0] = -INFINITY;
           ml[1] = 0.0f;
         } else {
-          const int t = rr / p.h, head = rr - t * p.h;
+          const int t = qp_row_token(rr, p), head = rr - t * p.h;
           T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim;
           const float z[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
           for (int c = 0; c < 16; ++c) q8_store8(dst + 8 * c, z);
@@ -431,79 +487,68 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     // ---------------------------------------------------------------------------------------------- codes -> f16 tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsConvert));
     // A tile is converted in two halves of 64 tokens, K's then V's; two halves are in flight in registers while a third
-    // is converted (32 registers: more would be taken from the softmax threads).
-    const int rw = (warp - 8) * 4 + (lane >> 3), c8 = lane & 7;     // row within a group of 16, 16-code piece of the row
-    const long long off = (long long)bg * p.C * kHeadDim + 16 * c8;
-    const uint8_t* const codes[2] = {p.kc + off, p.vc + off};
+    // is converted. A thread takes 8 codes of each 64-wide half of a row: 8 lanes read 64 contiguous bytes, and store
+    // the 8 chunks of one row of a swizzled half, each in its own banks.
+    const int rw = (warp - 8) * 4 + (lane >> 3), c8 = lane & 7;     // row within a group of 16, 8-code piece
+    const long long off = (long long)bg * p.C * kHeadDim + 8 * c8;
+    const uint32_t at = qp_chunk(0, rw, c8);
+    struct Half { uint2 a[4], b[4]; };                              // rows rw + 16 i: dimensions 8 c8 ..., 64 + 8 c8 ...
     // half u of the walk: tile u / 4, K for u % 4 < 2, V after
-    auto load = [&](int u, uint4 (&x)[4]) {
+    auto load = [&](int u, Half& x) {
       if (u >= 4 * nt) return;
       const int j0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1) + rw;
-      const uint8_t* src = codes[(u >> 1) & 1];
+      const uint8_t* src = ((u & 2) ? p.vc : p.kc) + off + (long long)j0 * kHeadDim;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int j = j0 + 16 * i;
-        x[i] = j < n ? __ldg(reinterpret_cast<const uint4*>(src + (long long)j * kHeadDim)) : make_uint4(0, 0, 0, 0);
+        const bool in = j0 + 16 * i < n;
+        x.a[i] = in ? __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim)) : make_uint2(0, 0);
+        x.b[i] = in ? __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim + 64)) : make_uint2(0, 0);
       }
     };
-    auto store = [&](uint32_t dst, const uint4 (&x)[4]) {
-      // pieces 4-7 of a row (the second 64 dimensions) write their two chunks in the other order: no two lanes of a
-      // quarter warp share a bank
-      const int first = c8 >> 2;
+    // Stores a half. `nan` collects 0 * value of V (screening the codes took half again as many instructions): NaN when
+    // there is a NaN code, and then the half is read again, the codes replaced by zeros and their tokens listed.
+    auto store = [&](uint32_t dst, const Half& x, int u) {
+      __half2 nan = __floats2half2_rn(0.0f, 0.0f);
+      const __half2 zero = nan;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * i + rw;
-        const uint32_t lo[4] = {q8_decode_lo(x[i].x), q8_decode_hi(x[i].x), q8_decode_lo(x[i].y), q8_decode_hi(x[i].y)};
-        const uint32_t hi[4] = {q8_decode_lo(x[i].z), q8_decode_hi(x[i].z), q8_decode_lo(x[i].w), q8_decode_hi(x[i].w)};
-        const uint32_t a0 = qp_chunk(dst, r, 2 * c8), a1 = qp_chunk(dst, r, 2 * c8 + 1);
-        if (first) {
-          qp_st_shared16(a1, hi[0], hi[1], hi[2], hi[3]);
-          qp_st_shared16(a0, lo[0], lo[1], lo[2], lo[3]);
-        } else {
-          qp_st_shared16(a0, lo[0], lo[1], lo[2], lo[3]);
-          qp_st_shared16(a1, hi[0], hi[1], hi[2], hi[3]);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint2 w = k ? x.b[i] : x.a[i];
+          const uint32_t h[4] = {q8_decode_lo(w.x), q8_decode_hi(w.x), q8_decode_lo(w.y), q8_decode_hi(w.y)};
+          qp_st_shared16(dst + at + (uint32_t)k * kQpHalf + (uint32_t)i * 2048u, h[0], h[1], h[2], h[3]);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) nan = __hfma2(*reinterpret_cast<const __half2*>(&h[d]), zero, nan);
         }
+      const uint32_t bits = *reinterpret_cast<const uint32_t*>(&nan);
+      if (!(u & 2) || (bits & 0x7fff7fffu) == 0u) return;
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const int j = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1) + rw + 16 * (i >> 1);
+        if (j >= n) break;
+        uint2 w = *reinterpret_cast<const uint2*>(p.vc + off + (long long)j * kHeadDim + 64 * (i & 1));
+        if ((q8_nan_mask(w.x) | q8_nan_mask(w.y)) == 0u) continue;
+        const int k = atomicAdd(&s_nan_count, 1);
+        if (k < kQpNanList) s_nan[k] = j;
+        w = make_uint2(q8_drop_nan(w.x), q8_drop_nan(w.y));
+        qp_st_shared16(dst + at + (uint32_t)(i & 1) * kQpHalf + (uint32_t)(i >> 1) * 2048u, q8_decode_lo(w.x),
+                       q8_decode_hi(w.x), q8_decode_lo(w.y), q8_decode_hi(w.y));
       }
     };
-    auto drop_nan = [&](int u, uint4 (&x)[4]) {
-      uint32_t bad = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bad |= q8_nan_mask(x[i].x) | q8_nan_mask(x[i].y) | q8_nan_mask(x[i].z) | q8_nan_mask(x[i].w);
-      if (!bad) return;
-      const int j0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1) + rw;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (q8_nan_mask(x[i].x) | q8_nan_mask(x[i].y) | q8_nan_mask(x[i].z) | q8_nan_mask(x[i].w)) {
-          const int at = atomicAdd(&s_nan_count, 1);
-          if (at < kQpNanList) s_nan[at] = j0 + 16 * i;
-        }
-        x[i] = make_uint4(q8_drop_nan(x[i].x), q8_drop_nan(x[i].y), q8_drop_nan(x[i].z), q8_drop_nan(x[i].w));
-      }
-    };
-    uint4 xa[4], xb[4];
+    Half xa, xb;
     load(0, xa);
     load(1, xb);
 #pragma unroll 1
-    for (int it = 0; it < nt; ++it) {
-      const int st = it % NS;
-      const uint32_t par = ((uint32_t)(it / NS) & 1u) ^ 1u;
-      const uint32_t tk = s_k + (uint32_t)st * kQpTile, tv = s_v + (uint32_t)st * kQpTile;
-      qp_wait(&s_kempty[st], par, &s_abort, p.err);
-      store(tk, xa);
-      load(4 * it + 2, xa);
-      store(tk + kQ8Block * 128u, xb);
-      load(4 * it + 3, xb);
+    for (int u = 0; u < 4 * nt; u += 2) {
+      const int it = u >> 2, st = it % NS, kv = (u >> 1) & 1;
+      const uint32_t tile = (kv ? s_v : s_k) + (uint32_t)st * kQpTile;
+      qp_wait(&s_empty[kv][st], ((uint32_t)(it / NS) & 1u) ^ 1u, &s_abort, p.err);
+      store(tile, xa, u);
+      load(u + 2, xa);
+      store(tile + kQ8Block * 128u, xb, u + 1);
+      load(u + 3, xb);
       qp_fence_async();
-      pf_arrive(&s_kfull[st]);
-      drop_nan(4 * it + 2, xa);
-      qp_wait(&s_vempty[st], par, &s_abort, p.err);
-      store(tv, xa);
-      load(4 * it + 4, xa);
-      drop_nan(4 * it + 3, xb);
-      store(tv + kQ8Block * 128u, xb);
-      load(4 * it + 5, xb);
-      qp_fence_async();
-      pf_arrive(&s_vfull[st]);
+      pf_arrive(&s_full[kv][st]);
     }
   } else {
     // ---------------------------------------------------------------------------------------------- MMAs
@@ -512,8 +557,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     if (qt < ntile && nt > 0) {
       uint32_t lead;
       asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
-      const uint64_t dq = pf_sdesc(s_q + (uint32_t)(qt * QP) * kQpTile, 16, 1024, 2), dk = pf_sdesc(s_k, 16, 1024, 2),
-                     dv = pf_sdesc(s_v, kQpHalf, 1024, 2);
+      // low descriptor words: address / 16, leading offset / 16 (1 where the K-major layout does not use it)
+      const uint32_t dq = ((s_q + (uint32_t)(qt * QP) * kQpTile) >> 4) | (1u << 16), dk = (s_k >> 4) | (1u << 16),
+                     dv = (s_v >> 4) | ((kQpHalf >> 4) << 16);
       const uint32_t tS = tm + (uint32_t)qt * 128u, tO = tm + 256u + (uint32_t)qt * 128u;
       auto scores = [&](int step) {                     // S = Q K^T for one block of the key tile
         const uint32_t kb = (uint32_t)((step >> 1) % NS) * kQpTile + (uint32_t)(step & 1) * (kQ8Block * 128u);
@@ -537,33 +583,33 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
                       dv + ((vb + ks * 2048u) >> 4), (step | term | (int)ks) > 0 ? 1u : 0u);
         qp_commit(lead, &s_pv[qt][step & 1]);
       };
-      qp_wait(&s_kfull[0], 0, &s_abort, p.err);
+      qp_wait(&s_full[0][0], 0, &s_abort, p.err);
       qp_wait(&s_qfull[qt], 0, &s_abort, p.err);
       tmem_fence_after_sync();
       scores(0);
       scores(1);
-      qp_commit(lead, &s_kempty[0]);
+      qp_commit(lead, &s_empty[0][0]);
 #pragma unroll 1
       for (int it = 0; it < nt; ++it) {
         const bool more = it + 1 < nt;
         const uint32_t par = (uint32_t)it & 1u;
-        qp_wait(&s_vfull[it % NS], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
+        qp_wait(&s_full[1][it % NS], (uint32_t)(it / NS) & 1u, &s_abort, p.err);
         qp_wait(&s_pfull[qt][0], par, &s_abort, p.err);
         tmem_fence_after_sync();
         values(2 * it);
         if (more) {
           // the scores of the next tile go where P was: MMAs of one thread run in order
-          qp_wait(&s_kfull[(it + 1) % NS], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
+          qp_wait(&s_full[0][(it + 1) % NS], (uint32_t)((it + 1) / NS) & 1u, &s_abort, p.err);
           tmem_fence_after_sync();
           scores(2 * it + 2);
         }
         qp_wait(&s_pfull[qt][1], par, &s_abort, p.err);
         tmem_fence_after_sync();
         values(2 * it + 1);
-        qp_commit(lead, &s_vempty[it % NS]);
+        qp_commit(lead, &s_empty[1][it % NS]);
         if (more) {
           scores(2 * it + 3);
-          qp_commit(lead, &s_kempty[(it + 1) % NS]);
+          qp_commit(lead, &s_empty[0][(it + 1) % NS]);
         }
       }
     }
