@@ -36,6 +36,19 @@ int q8_shape(int B, int G, int C, int d, const void* kc, const void* vc, const v
 
 int q8_blocks(int C) { return (C + kQ8Block - 1) / kQ8Block; }
 
+template <typename T>
+void rotary_launch(int mode, dim3 grid, cudaStream_t st, const RotaryParams& p) {
+  if (mode == kRotPairs) rotary_kernel<T, kRotPairs><<<grid, 256, 0, st>>>(p);
+  else if (mode == kRotInner) rotary_kernel<T, kRotInner><<<grid, 256, 0, st>>>(p);
+  else rotary_kernel<T, kRotOdd><<<grid, 256, 0, st>>>(p);
+}
+template <typename T>
+void append_launch(int mode, unsigned grid, cudaStream_t st, const Q8AppendParams& p) {
+  if (mode == kRotPairs) q8_append_kernel<T, kRotPairs><<<grid, kQ8AppendThreads, 0, st>>>(p);
+  else if (mode == kRotInner) q8_append_kernel<T, kRotInner><<<grid, kQ8AppendThreads, 0, st>>>(p);
+  else q8_append_kernel<T, kRotOdd><<<grid, kQ8AppendThreads, 0, st>>>(p);
+}
+
 // The attend's kernel, and how it splits its work.
 struct Q8Plan {
   bool token;                       // the few-column kernel (mma.sync); else the prompt kernel (tcgen05)
@@ -143,16 +156,20 @@ int al_rotary(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, int Hq,
     p.pos_sb = pos_sb; p.pos_st = pos_st;
   }
   p.start = start; p.B = B; p.T = T; p.d = d; p.sgn = inverse ? -1.0f : 1.0f; p.err = di->err;
-  const long long threads = (long long)B * T * (d / 8), heads = Hq + Hk;
+  const int mode = rot_mode(rot, layout);
+  p.items = rot_items(d, rot, mode);
+  const long long threads = (long long)B * T * p.items, heads = Hq + Hk;
   const long long blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many tokens");
+  if (threads > 0x7fffff00LL) return fail(AL_EUNSUPPORTED, "too many tokens for one call");
   // heads per thread: one while the launch does not fill the GPU, then as many as keep it filled (up to 8)
   p.hpt = 1;
   while (p.hpt < 8 && blocks * ((heads + 2 * p.hpt - 1) / (2 * p.hpt)) >= 8LL * di->sms) p.hpt *= 2;
-  const dim3 grid((unsigned)blocks, (unsigned)((heads + p.hpt - 1) / p.hpt));
+  const long long gy = (heads + p.hpt - 1) / p.hpt;
+  if (gy > 65535) return fail(AL_EUNSUPPORTED, "too many heads for one call");
+  const dim3 grid((unsigned)blocks, (unsigned)gy);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == AL_F32) rotary_kernel<float><<<grid, 256, 0, st>>>(p);
-  else rotary_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  if (dtype == AL_F32) rotary_launch<float>(mode, grid, st, p);
+  else rotary_launch<__nv_bfloat16>(mode, grid, st, p);
   return plain_launch_check("rotary_kernel");
 }
 
@@ -196,17 +213,25 @@ int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const i
   p.err = di->err;
   const long long kv = 2LL * B * G * p.touched;
   long long qc = 0;
+  const int mode = p.rt.table ? rot_mode(rot, layout) : kRotPairs;
+  p.items = rot_items(d, rot, mode);
   if (q) {
-    p.q = q; p.q_sb = q_sb; p.q_sg = q_sg; p.q_sh = q_sh; p.q_st = q_st;
-    p.h = h; p.q_out = q_out;
-    qc = ((long long)B * G * h * T * 16 + kQ8AppendThreads - 1) / kQ8AppendThreads;
+    p.q.x = q; p.q.sb = q_sb; p.q_sg = q_sg; p.q.sh = q_sh; p.q.st = q_st; p.q.H = h; p.q.out = q_out;
+    p.h = h;
+    // heads of a group per thread: one while the launch does not fill the GPU, then up to 4 at once
+    const long long per = (long long)B * G * T * p.items;
+    p.hpt = 1;
+    while (p.hpt < 4 && p.hpt < h && per * ((h + 2 * p.hpt - 1) / (2 * p.hpt)) >= 2048LL * di->sms) p.hpt *= 2;
+    const long long threads = per * ((h + p.hpt - 1) / p.hpt);
+    if (threads > 0x7fffff00LL) return fail(AL_EUNSUPPORTED, "too many query rows for one call");
+    qc = (threads + kQ8AppendThreads - 1) / kQ8AppendThreads;
   }
   if (kv + qc > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many rows for one call");
   p.kv_ctas = (int)kv;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const unsigned grid = (unsigned)(kv + qc);
-  if (dtype == AL_F32) q8_append_kernel<float><<<grid, kQ8AppendThreads, 0, st>>>(p);
-  else q8_append_kernel<__nv_bfloat16><<<grid, kQ8AppendThreads, 0, st>>>(p);
+  if (dtype == AL_F32) append_launch<float>(mode, grid, st, p);
+  else append_launch<__nv_bfloat16>(mode, grid, st, p);
   return plain_launch_check("q8_append_kernel");
 }
 
@@ -223,10 +248,8 @@ int al_read_q8(const void* k_codes, const void* v_codes, const void* k_exp, cons
   p.codes[0] = static_cast<const uint8_t*>(k_codes); p.codes[1] = static_cast<const uint8_t*>(v_codes);
   p.exps[0] = static_cast<const signed char*>(k_exp); p.exps[1] = static_cast<const signed char*>(v_exp);
   p.out[0] = k_out; p.out[1] = v_out;
-  p.C = C; p.NB = q8_blocks(C); p.lo = lo; p.n = hi - lo; p.rows = (long long)B * G * p.n;
-  const long long blocks = (p.rows * (kHeadDim / (16 / esize(out_dtype))) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many rows for one call");
-  const dim3 grid((unsigned)blocks, 2);
+  p.C = C; p.NB = q8_blocks(C); p.lo = lo; p.hi = hi;
+  const dim3 grid((unsigned)((hi - 1) / kQ8Block - lo / kQ8Block + 1), (unsigned)(B * G), 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (out_dtype == AL_F32) q8_read_kernel<float><<<grid, 256, 0, st>>>(p);
   else q8_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);

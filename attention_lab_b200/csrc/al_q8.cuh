@@ -57,6 +57,20 @@ __device__ __forceinline__ float2 q8_half2_floats(uint32_t h) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// 8 values times `scale` to 8 codes, and back to floats.
+__device__ __forceinline__ uint2 q8_encode8(const float (&x)[8], float scale) {
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(x[j], scale);
+  return make_uint2(q8_encode2(y[0], y[1]) | (q8_encode2(y[2], y[3]) << 16),
+                    q8_encode2(y[4], y[5]) | (q8_encode2(y[6], y[7]) << 16));
+}
+__device__ __forceinline__ void q8_decode8(const uint2& w, float (&x)[8]) {
+  const float2 a = q8_half2_floats(q8_decode_lo(w.x)), b = q8_half2_floats(q8_decode_hi(w.x));
+  const float2 c = q8_half2_floats(q8_decode_lo(w.y)), d = q8_half2_floats(q8_decode_hi(w.y));
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
+}
+
 // 8 elements of T as floats.
 __device__ __forceinline__ void q8_load8(const __nv_bfloat16* p, float (&f)[8]) {
   unpack(*reinterpret_cast<const uint4*>(p), f, p);
@@ -92,48 +106,78 @@ __device__ __forceinline__ void rot_pair(float& a, float& b, float c, float s) {
   a = x;
 }
 
-// Rotate the 8 dimensions [8 ch, 8 ch + 8) of the row at `row` (held in x); partners outside the chunk are read from
-// the row (it was just read by a neighbouring lane, so these reads hit L1). tr: the position's table row.
-template <typename T>
-__device__ __forceinline__ void rot_chunk(float (&x)[8], const T* row, const float* tr, int ch, const RotTable& rt,
-                                          float sgn) {
-  const int half = rt.rot >> 1, d0 = 8 * ch;
-  if (d0 >= rt.rot) return;
-  if (rt.layout == kRotInterleaved) {
+// A thread's share of a row's rotation: one item of 8 dimensions (or a pair of items half the rotated width apart),
+// with its cosines and sines in registers while it walks over heads, which all share them. How a row splits into items:
+//   kRotPairs   half layout, rot a multiple of 16: items 0 .. rot/16 - 1 are the dimension pairs [8 i, 8 i + 8) and
+//               [rot/2 + 8 i, ...), each read once; the others are 8 dimensions past rot, copied
+//   kRotInner   interleaved: 8 dimensions hold their own 4 pairs
+//   kRotOdd     half layout, other rot: 8 dimensions, partners read one by one from the row (it is in L1 by then)
+constexpr int kRotPairs = 0, kRotInner = 1, kRotOdd = 2;
+__host__ __device__ __forceinline__ int rot_mode(int rot, int layout) {
+  return layout == kRotInterleaved ? kRotInner : (rot % 16 == 0 ? kRotPairs : kRotOdd);
+}
+__host__ __device__ __forceinline__ int rot_items(int d, int rot, int mode) {   // items of a row
+  return mode == kRotPairs ? (d - rot) / 8 + rot / 16 : d / 8;
+}
+
+template <int MODE>
+struct RotItem {
+  float c[8], s[8];           // kRotInner: 4 of each
+  int d0, d1;                 // first dimension; of the second chunk (kRotPairs), or -1
+  int live;                   // dimensions from d0 on that are rotated (0: copied)
+
+  __device__ __forceinline__ void init(const RotTable& rt, const float* tr, int item, float sgn) {
+    const int half = rt.rot >> 1;
+    d1 = -1;
+    if (MODE == kRotPairs) {
+      const int pairs = rt.rot >> 4;
+      d0 = item < pairs ? 8 * item : rt.rot + 8 * (item - pairs);
+      live = item < pairs ? 8 : 0;
+      if (live) {
+        d1 = d0 + half;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pi = (d0 >> 1) + i;
-      if (pi < half) rot_pair(x[2 * i], x[2 * i + 1], __ldg(tr + pi), sgn * __ldg(tr + half + pi));
+        for (int i = 0; i < 8; i += 4) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(tr + d0 + i));
+          const float4 y = __ldg(reinterpret_cast<const float4*>(tr + half + d0 + i));
+          c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
+          s[i] = sgn * y.x; s[i + 1] = sgn * y.y; s[i + 2] = sgn * y.z; s[i + 3] = sgn * y.w;
+        }
+      }
+      return;
     }
-  } else if ((half & 7) == 0) {
-    const bool low = d0 < half;
-    const int i0 = low ? d0 : d0 - half;
-    float y[8];
-    q8_load8(row + (low ? d0 + half : d0 - half), y);
-    const float4 c0 = __ldg(reinterpret_cast<const float4*>(tr + i0)), c1 = __ldg(reinterpret_cast<const float4*>(tr + i0) + 1);
-    const float4 s0 = __ldg(reinterpret_cast<const float4*>(tr + half + i0)),
-                 s1 = __ldg(reinterpret_cast<const float4*>(tr + half + i0) + 1);
-    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    d0 = 8 * item;
+    live = max(0, min(8, rt.rot - d0));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float si = sgn * s[i];
-      x[i] = low ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], si))
-                 : __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], si));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = d0 + i;
-      if (d >= rt.rot) continue;
-      const bool low = d < half;
-      const int pi = low ? d : d - half;
-      const float y = tof(row[low ? d + half : d - half]);
-      const float c = __ldg(tr + pi), si = sgn * __ldg(tr + half + pi);
-      x[i] = low ? __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(y, si)) : __fadd_rn(__fmul_rn(x[i], c), __fmul_rn(y, si));
+    for (int i = 0; i < (MODE == kRotInner ? 4 : 8); ++i) {
+      const int pi = MODE == kRotInner ? (d0 >> 1) + i : (d0 + i < half ? d0 + i : d0 + i - half);
+      const bool on = (MODE == kRotInner ? 2 * i : i) < live;
+      c[i] = on ? __ldg(tr + pi) : 1.0f;
+      s[i] = on ? sgn * __ldg(tr + half + pi) : 0.0f;
     }
   }
-}
+  // x: the chunk at d0; y: the chunk at d1 (kRotPairs). row: the row in memory (kRotOdd's partners).
+  template <typename T>
+  __device__ __forceinline__ void turn(float (&x)[8], float (&y)[8], const T* row, const RotTable& rt) const {
+    if (MODE == kRotPairs) {
+      if (!live) return;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rot_pair(x[i], y[i], c[i], s[i]);
+    } else if (MODE == kRotInner) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (2 * i < live) rot_pair(x[2 * i], x[2 * i + 1], c[i], s[i]);
+    } else {
+      const int half = rt.rot >> 1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= live) continue;
+        const bool low = d0 + i < half;
+        const float z = tof(row[low ? d0 + i + half : d0 + i - half]);
+        x[i] = low ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(z, s[i])) : __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(z, s[i]));
+      }
+    }
+  }
+};
 
 // Rows of one tensor [B, H, T, d] (element strides sb, sh, st; last dimension contiguous) to a contiguous output.
 struct RotTensor {
@@ -150,37 +194,58 @@ struct RotaryParams {
   long long pos_sb, pos_st;
   long long start;
   int B, T, d;
+  int items;                  // items of a row (rot_items)
   int hpt;                    // heads per thread
   float sgn;                  // -1: the inverse rotation (the gradient)
   unsigned* err;
 };
 
-// One thread: 8 dimensions of one token for hpt heads (of q, then k).
-template <typename T>
+// Heads [h0, h1) of one tensor at (b, t): U rows in flight. `in`: the position is in the table (else zeros).
+template <typename T, int MODE>
+__device__ __forceinline__ void rot_heads(const RotTensor& x, int h0, int h1, int b, int t, int Tn, int d,
+                                          const RotItem<MODE>& it, const RotTable& rt, bool in) {
+  constexpr int U = sizeof(T) == 2 ? 4 : 2;
+  const T* src = static_cast<const T*>(x.x) + b * x.sb + t * x.st;
+  T* dst = static_cast<T*>(x.out) + ((long long)b * x.H * Tn + t) * d;
+  for (int h = h0; h < h1; h += U) {
+    float v[U][8], w[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = w[u][i] = 0.0f;
+      if (in && h + u < h1) {
+        q8_load8(src + (h + u) * x.sh + it.d0, v[u]);
+        if (MODE == kRotPairs && it.d1 >= 0) q8_load8(src + (h + u) * x.sh + it.d1, w[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h + u >= h1) break;
+      if (in) it.turn(v[u], w[u], src + (h + u) * x.sh, rt);
+      T* o = dst + (long long)(h + u) * Tn * d;
+      q8_store8(o + it.d0, v[u]);
+      if (MODE == kRotPairs && it.d1 >= 0) q8_store8(o + it.d1, w[u]);
+    }
+  }
+}
+
+// One thread: one item of one token for hpt heads (of q, then k). Bound: HBM, every row read and written once; a token's
+// table row (4 rot bytes) is read by heads / hpt threads an item, from L2 after the first.
+template <typename T, int MODE>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
-  const int chunks = p.d >> 3;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long tok = i / chunks;
-  if (tok >= (long long)p.B * p.T) return;
-  const int ch = (int)(i - tok * chunks);
-  const int b = (int)(tok / p.T), t = (int)(tok - (long long)b * p.T);
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  const unsigned tok = i / (unsigned)p.items;
+  if (tok >= (unsigned)p.B * (unsigned)p.T) return;
+  const int item = (int)(i - tok * (unsigned)p.items);
+  const int b = (int)(tok / (unsigned)p.T), t = (int)(tok - (unsigned)b * (unsigned)p.T);
   const long long pos = p.pos ? p.pos[b * p.pos_sb + t * p.pos_st] : p.start + t;
   const bool in = pos >= 0 && pos < p.rt.rows;
-  if (!in && pos >= 0 && ch == 0 && blockIdx.y == 0) atomicOr(p.err, kErrQ8Range);
-  const float* tr = p.rt.table + (in ? pos * p.rt.rot : 0);
+  if (!in && pos >= 0 && item == 0 && blockIdx.y == 0) atomicOr(p.err, kErrQ8Range);
+  RotItem<MODE> it;
+  it.init(p.rt, p.rt.table + (in ? pos * p.rt.rot : 0), item, p.sgn);
   const int h0 = blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, p.q.H + p.k.H);
-  for (int hh = h0; hh < h1; ++hh) {
-    const bool second = hh >= p.q.H;
-    const RotTensor& x = second ? p.k : p.q;
-    const int head = second ? hh - p.q.H : hh;
-    const T* row = static_cast<const T*>(x.x) + b * x.sb + head * x.sh + t * x.st;
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (in) {
-      q8_load8(row + 8 * ch, v);
-      rot_chunk(v, row, tr, ch, p.rt, p.sgn);
-    }
-    q8_store8(static_cast<T*>(x.out) + (((long long)b * x.H + head) * p.T + t) * p.d + 8 * ch, v);
-  }
+  if (h0 < p.q.H) rot_heads<T, MODE>(p.q, h0, min(h1, p.q.H), b, t, p.T, p.d, it, p.rt, in);
+  if (h1 > p.q.H) rot_heads<T, MODE>(p.k, max(h0 - p.q.H, 0), h1 - p.q.H, b, t, p.T, p.d, it, p.rt, in);
 }
 
 // ------------------------------------------------------------------------------------------------ quantising write
@@ -193,23 +258,23 @@ struct Q8AppendParams {
   int B, G, T, C, NB;
   int touched;                // blocks a request's T rows can reach
   RotTable rt;                // rt.table null: no rotation
-  const void* q;              // queries to rotate [B,G,h,T,128] (strides) or null
-  long long q_sb, q_sg, q_sh, q_st;
+  RotTensor q;                // queries to rotate, [B, G*h, T, 128] with head (g, i) at g * q_sg + i * sh; x null: none
+  long long q_sg;
   int h;
-  void* q_out;                // contiguous [B,G,h,T,128]
+  int items, hpt;             // of q's rotation
   int kv_ctas;                // CTAs of the write; the rest rotate q
   unsigned* err;
 };
 
-constexpr int kQ8AppendThreads = 128;      // 16 lanes x 8 dimensions per row, 8 rows at a time, 8 times
+constexpr int kQ8AppendThreads = 256;      // 8 threads a row, two chunks of 8 dimensions each; 32 rows at a time, twice
 
 // One CTA writes one block (64 tokens) of one (batch, group) of K or V: the new rows are read once into registers,
 // rotated (K), their largest finite value reduced over the CTA, then rounded and stored. Rows the block already holds
-// are touched only when the exponent grows.
-template <typename T>
+// are touched only when the exponent grows. A thread's two chunks are a rotation pair (kRotPairs) or its own columns.
+template <typename T, int MODE>
 __device__ __forceinline__ void q8_append_block(const Q8AppendParams& p, int kv, int bg, int n_idx) {
   __shared__ uint32_t s_max[kQ8AppendThreads / 32];
-  const int tid = threadIdx.x, ch = tid & 15, r0 = tid >> 4;
+  const int tid = threadIdx.x, item = tid & 7, r0 = tid >> 3;
   const int b = bg / p.G, g = bg - b * p.G;
   const int len = q8_length(p.len, b), n = min(len, p.C);
   if ((len < 0 || len > p.C) && tid == 0) atomicOr(p.err, kErrQ8Range);
@@ -219,102 +284,114 @@ __device__ __forceinline__ void q8_append_block(const Q8AppendParams& p, int kv,
   if (p0 >= n) return;
   const T* src = static_cast<const T*>(p.x[kv]) + b * p.sb[kv] + g * p.sg[kv];
   const bool turn = kv == 0 && p.rt.table != nullptr;
-  float x[8][8];
-  uint32_t amax = 0;
+  // chunks of this thread: the pair of its item where items pair up (rot = 128), else columns 8 item and 64 + 8 item
+  const int d0 = 8 * item, d1 = 64 + 8 * item;
+  float x[2][8], y[2][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int pos = p0 + r0 + 8 * i;
-    const bool fresh = pos >= start && pos < n;
+  for (int i = 0; i < 2; ++i) {
+    const int pos = p0 + r0 + 32 * i;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-    if (fresh) q8_load8(src + (long long)(pos - start) * p.st[kv] + 8 * ch, x[i]);
-  }
-  if (turn) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int pos = p0 + r0 + 8 * i;
-      if (pos < start || pos >= n) continue;
-      if (pos < p.rt.rows) {
-        rot_chunk(x[i], src + (long long)(pos - start) * p.st[0], p.rt.table + (long long)pos * p.rt.rot, ch, p.rt, 1.0f);
-      } else {
-        if (ch == 0) atomicOr(p.err, kErrQ8Range);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-      }
+    for (int j = 0; j < 8; ++j) x[i][j] = y[i][j] = 0.0f;
+    if (pos >= start && pos < n) {
+      q8_load8(src + (long long)(pos - start) * p.st[kv] + d0, x[i]);
+      q8_load8(src + (long long)(pos - start) * p.st[kv] + d1, y[i]);
     }
   }
+  signed char* ep = p.exps[kv] + (long long)bg * p.NB + blk;
+  const int kept = min(max(start - p0, 0), kQ8Block);   // rows the block already holds
+  const int e_old = kept > 0 ? (int)*ep : kQ8EMin;
+  uint32_t amax = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 2; ++i) {
+    const int pos = p0 + r0 + 32 * i;
+    if (turn && pos >= start && pos < n) {
+      if (pos < p.rt.rows) {
+        const float* tr = p.rt.table + (long long)pos * p.rt.rot;
+        const T* row = src + (long long)(pos - start) * p.st[0];
+        if (MODE == kRotPairs && p.rt.rot == kHeadDim) {
+          RotItem<kRotPairs> it;
+          it.init(p.rt, tr, item, 1.0f);
+          it.turn(x[i], y[i], row, p.rt);
+        } else {
+          // chunk by chunk; partners outside it come from the row
+          constexpr int M = MODE == kRotInner ? kRotInner : kRotOdd;
+          RotItem<M> it;
+          it.init(p.rt, tr, item, 1.0f);
+          it.turn(x[i], y[i], row, p.rt);
+          it.init(p.rt, tr, 8 + item, 1.0f);
+          it.turn(y[i], x[i], row, p.rt);
+        }
+      } else {
+        if (item == 0) atomicOr(p.err, kErrQ8Range);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = y[i][j] = 0.0f;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (q8_finite(x[i][j])) amax = max(amax, __float_as_uint(x[i][j]) & 0x7fffffffu);
       else x[i][j] = __uint_as_float(0x7fffffffu);
+      if (q8_finite(y[i][j])) amax = max(amax, __float_as_uint(y[i][j]) & 0x7fffffffu);
+      else y[i][j] = __uint_as_float(0x7fffffffu);
     }
+  }
   amax = __reduce_max_sync(0xffffffffu, amax);
   if ((tid & 31) == 0) s_max[tid >> 5] = amax;
-  signed char* ep = p.exps[kv] + (long long)bg * p.NB + blk;
-  const int kept = min(max(start - p0, 0), kQ8Block);   // rows the block already holds
-  const int e_old = kept > 0 ? (int)*ep : kQ8EMin;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kQ8AppendThreads / 32; ++w) amax = max(amax, s_max[w]);
   const int e = max(e_old, q8_exponent(amax));
   const float inv = q8_exp2i(-e);
-  uint8_t* dst = p.codes[kv] + ((long long)bg * p.C + p0) * kHeadDim + 8 * ch;
-  const float shift = q8_exp2i(e_old - e);
+  uint8_t* dst = p.codes[kv] + ((long long)bg * p.C + p0) * kHeadDim;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + 8 * i, pos = p0 + r;
-    uint2* out = reinterpret_cast<uint2*>(dst + r * kHeadDim);
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + 32 * i, pos = p0 + r;
+    uint2* o0 = reinterpret_cast<uint2*>(dst + r * kHeadDim + d0);
+    uint2* o1 = reinterpret_cast<uint2*>(dst + r * kHeadDim + d1);
     if (pos >= start && pos < n) {
-      float y[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(x[i][j], inv);
-      *out = make_uint2(q8_encode2(y[0], y[1]) | (q8_encode2(y[2], y[3]) << 16),
-                        q8_encode2(y[4], y[5]) | (q8_encode2(y[6], y[7]) << 16));
+      *o0 = q8_encode8(x[i], inv);
+      *o1 = q8_encode8(y[i], inv);
     } else if (r < kept && e != e_old) {
-      uint2 w = *out;
-      const float2 a = q8_half2_floats(q8_decode_lo(w.x)), c = q8_half2_floats(q8_decode_hi(w.x));
-      const float2 f = q8_half2_floats(q8_decode_lo(w.y)), u = q8_half2_floats(q8_decode_hi(w.y));
-      w.x = q8_encode2(a.x * shift, a.y * shift) | (q8_encode2(c.x * shift, c.y * shift) << 16);
-      w.y = q8_encode2(f.x * shift, f.y * shift) | (q8_encode2(u.x * shift, u.y * shift) << 16);
-      *out = w;
+      const float shift = q8_exp2i(e_old - e);
+      q8_decode8(*o0, x[i]);
+      q8_decode8(*o1, y[i]);
+      *o0 = q8_encode8(x[i], shift);
+      *o1 = q8_encode8(y[i], shift);
     }
   }
   if (tid == 0) *ep = (signed char)e;
 }
 
-template <typename T>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kQ8AppendThreads) q8_append_kernel(const Q8AppendParams p) {
-  const long long blk = blockIdx.x;
-  if (blk < p.kv_ctas) {
+  const unsigned blk = blockIdx.x;
+  if (blk < (unsigned)p.kv_ctas) {
     // block index fastest, then K / V, then (batch, group)
-    const int n_idx = (int)(blk % p.touched);
-    const long long rest = blk / p.touched;
-    q8_append_block<T>(p, (int)(rest & 1), (int)(rest >> 1), n_idx);
+    const unsigned rest = blk / (unsigned)p.touched;
+    q8_append_block<T, MODE>(p, (int)(rest & 1), (int)(rest >> 1), (int)(blk - rest * (unsigned)p.touched));
     return;
   }
-  // q: one thread rotates 8 dimensions of one (b, g, head, t) row
-  const long long i = (blk - p.kv_ctas) * kQ8AppendThreads + threadIdx.x;
-  const long long row = i >> 4;
-  const int ch = (int)(i & 15);
-  const int per_b = p.G * p.h * p.T;
-  if (row >= (long long)p.B * per_b) return;
-  const int b = (int)(row / per_b);
-  int rem = (int)(row - (long long)b * per_b);
-  const int t = rem % p.T;
-  rem /= p.T;
-  const int head = rem % p.h, g = rem / p.h;
+  // q: one thread rotates one item of one token for hpt heads of one group
+  const unsigned i = (blk - (unsigned)p.kv_ctas) * kQ8AppendThreads + threadIdx.x;
+  const unsigned tok = i / (unsigned)p.items;
+  const int item = (int)(i - tok * (unsigned)p.items);
+  const unsigned split = (unsigned)((p.h + p.hpt - 1) / p.hpt);      // threads over a group's heads
+  const unsigned bgs = tok / (unsigned)p.T;
+  const int t = (int)(tok - bgs * (unsigned)p.T);
+  const unsigned bg = bgs / split;
+  if (bg >= (unsigned)(p.B * p.G)) return;
+  const int b = (int)(bg / (unsigned)p.G), g = (int)(bg - (unsigned)b * (unsigned)p.G);
+  const int h0 = (int)(bgs - bg * split) * p.hpt;
   const long long pos = (long long)q8_length(p.len, b) - p.T + t;
   const bool in = pos >= 0 && pos < p.rt.rows;
-  if (!in && pos >= 0 && ch == 0) atomicOr(p.err, kErrQ8Range);
-  const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t * p.q_st;
-  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  if (in) {
-    q8_load8(src + 8 * ch, v);
-    rot_chunk(v, src, p.rt.table + pos * p.rt.rot, ch, p.rt, 1.0f);
-  }
-  q8_store8(static_cast<T*>(p.q_out) + row * kHeadDim + 8 * ch, v);
+  if (!in && pos >= 0 && item == 0) atomicOr(p.err, kErrQ8Range);
+  RotItem<MODE> it;
+  it.init(p.rt, p.rt.table + (in ? pos * p.rt.rot : 0), item, 1.0f);
+  RotTensor x = p.q;                       // this group's heads as a tensor of its own
+  x.x = static_cast<const T*>(p.q.x) + b * p.q.sb + g * p.q_sg;
+  x.out = static_cast<T*>(p.q.out) + (long long)bg * p.h * p.T * kHeadDim;
+  x.sb = 0;
+  rot_heads<T, MODE>(x, h0, min(h0 + p.hpt, p.h), 0, t, p.T, kHeadDim, it, p.rt, in);
 }
 
 // ------------------------------------------------------------------------------------------------ read-back
@@ -322,44 +399,54 @@ struct Q8ReadParams {
   const uint8_t* codes[2];
   const signed char* exps[2];
   void* out[2];               // [B,G,hi-lo,128] contiguous
-  int C, NB, lo, n;           // n = hi - lo
-  long long rows;             // B*G*n
+  int C, NB, lo, hi;
 };
 
-// One thread: 16 bytes of output (8 bf16 or 4 fp32), so that a warp's stores are contiguous.
+// One CTA reads one block's rows of one (batch, group) of K or V (grid: blocks, B*G, 2), so a CTA has one exponent and
+// no divisions. A thread writes 16 bytes at a time (8 bf16 or 4 fp32), so a warp's stores are contiguous; all of its
+// loads are in flight together. Bound: HBM, 1 byte in and 2 or 4 out per element.
 template <typename T>
 __global__ void __launch_bounds__(256) q8_read_kernel(const Q8ReadParams p) {
-  constexpr int E = 16 / (int)sizeof(T);             // elements per thread
-  constexpr int L = kHeadDim / E;                    // threads per row
-  const int kv = blockIdx.y;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = i / L;
-  if (row >= p.rows) return;
-  const int c = (int)(i % L) * E;
-  const long long bg = row / p.n;
-  const int pos = p.lo + (int)(row - bg * p.n);
-  const float scale = q8_exp2i(p.exps[kv][bg * p.NB + pos / kQ8Block]);
-  const uint8_t* src = p.codes[kv] + (bg * p.C + pos) * kHeadDim + c;
-  T* dst = static_cast<T*>(p.out[kv]) + row * kHeadDim + c;
-  uint32_t w[E / 4];
-  if (E == 8) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
-    w[0] = v.x;
-    w[E / 4 - 1] = v.y;
-  } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
-  }
-  float f[E];
+  constexpr int E = 16 / (int)sizeof(T);             // elements per thread and row
+  constexpr int L = kHeadDim / E, RPT = 256 / L;     // threads per row, rows at a time
+  constexpr int N = kQ8Block / RPT;                  // rows per thread
+  const int kv = blockIdx.z, blk = p.lo / kQ8Block + (int)blockIdx.x;
+  const long long bg = blockIdx.y;
+  const int r0 = threadIdx.x / L, c = (threadIdx.x % L) * E;
+  const int p0 = blk * kQ8Block + r0;
+  const float scale = q8_exp2i((kv ? p.exps[1] : p.exps[0])[bg * p.NB + blk]);
+  const uint8_t* src = (kv ? p.codes[1] : p.codes[0]) + (bg * p.C + p0) * kHeadDim + c;
+  T* dst = static_cast<T*>(kv ? p.out[1] : p.out[0]) + (bg * (p.hi - p.lo) + (p0 - p.lo)) * kHeadDim + c;
+  uint32_t w[N][E / 4];
 #pragma unroll
-  for (int j = 0; j < E / 4; ++j) {
-    const float2 a = q8_half2_floats(q8_decode_lo(w[j])), b = q8_half2_floats(q8_decode_hi(w[j]));
-    f[4 * j] = a.x * scale; f[4 * j + 1] = a.y * scale; f[4 * j + 2] = b.x * scale; f[4 * j + 3] = b.y * scale;
+  for (int i = 0; i < N; ++i) {
+    const int pos = p0 + i * RPT;
+    if (pos >= p.lo && pos < p.hi) {
+      if constexpr (E == 8) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(src + i * RPT * kHeadDim));
+        w[i][0] = v.x;
+        w[i][1] = v.y;
+      } else {
+        w[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src + i * RPT * kHeadDim));
+      }
+    }
   }
-  if (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
-  } else {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                                pack_bf16x2(f[E - 4], f[E - 3]), pack_bf16x2(f[E - 2], f[E - 1]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int pos = p0 + i * RPT;
+    if (pos < p.lo || pos >= p.hi) continue;
+    float f[E];
+#pragma unroll
+    for (int j = 0; j < E / 4; ++j) {
+      const float2 a = q8_half2_floats(q8_decode_lo(w[i][j])), b = q8_half2_floats(q8_decode_hi(w[i][j]));
+      f[4 * j] = a.x * scale; f[4 * j + 1] = a.y * scale; f[4 * j + 2] = b.x * scale; f[4 * j + 3] = b.y * scale;
+    }
+    uint4 o;
+    if constexpr (E == 8)
+      o = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    else
+      o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    *reinterpret_cast<uint4*>(dst + i * RPT * kHeadDim) = o;
   }
 }
 
