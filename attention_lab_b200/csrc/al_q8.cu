@@ -53,32 +53,45 @@ void append_launch(int mode, unsigned grid, cudaStream_t st, const Q8AppendParam
 struct Q8Plan {
   bool token;                       // the few-column kernel (mma.sync); else the prompt kernel (tcgen05)
   int cs;                           // token: CTAs per cluster
-  int row_tiles, nsplit;            // prompt: tiles of 256 rows, key splits
-  size_t ml_off, bytes;             // prompt with nsplit > 1: workspace layout
+  int row_tiles;                    // prompt: tiles of 256 rows
+  int nsplit;                       // key splits merged through the workspace
+  size_t ml_off, bytes;             // nsplit > 1: workspace layout
 };
 
-int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_length, int sms, Q8Plan* out) {
+int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_length, bool ragged, int sms, Q8Plan* out) {
   Q8Plan pl = {};
+  pl.nsplit = 1;
   const long long R = (long long)h * T, segs = (long long)B * G;
   int len = max_length > 0 ? std::min(max_length, C) : C;
   // tokens a query tile can see, as far as the host knows
   const long long span = window > 0 ? std::min<long long>(len, (long long)window + sinks) : len;
-  if (R <= AL_Q8_TOKEN_COLS) {
+  if (R <= kQ8TokenCols) {
     pl.token = true;
     const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
+    // One wave: clusters grow while the CTAs (two an SM) still fit at once and every warp keeps two steps. 6 x 8 segments
+    // of 4100 tokens: 4 CTAs a segment 19.4 us, 8 (more than a wave) 27.9; 8 segments of 2048: 8 CTAs 9.5 us, 16 10.5.
+    // Requests of their own lengths are split further, down to 8192 tokens a CTA, to even out the last wave: 256 segments
+    // of 16K to 32K tokens take 312 us unsplit, 281 us with 4 CTAs each (of one length 336 and 360: those stay unsplit).
     pl.cs = 1;
-    while (pl.cs < kMaxCluster && units * pl.cs < 2LL * sms && span > (long long)pl.cs * 2 * kQdWarps * kQdStep) pl.cs <<= 1;
+    while (pl.cs < kMaxCluster && units * pl.cs * 2 <= 2LL * sms && span >= pl.cs * 4LL * kQdWarps * kQdStep) pl.cs <<= 1;
+    if (ragged)
+      while (pl.cs < 4 && span > pl.cs * 8192LL) pl.cs <<= 1;
+    // Fewer segments than clusters of 16 can spread over the SMs: as many CTAs as fill them, merged by a second kernel.
+    const long long fill = std::min<long long>(2LL * sms / units, span / (2 * kQdWarps * kQdStep));
+    if (fill > kMaxCluster) {
+      pl.cs = 1;
+      pl.nsplit = (int)std::min<long long>(fill, 32 * kQmWarps);
+    }
   } else {
     pl.row_tiles = (int)((R + 2 * kQpRows - 1) / (2 * kQpRows));
     const long long ctas = segs * pl.row_tiles;
     const long long tiles = (span + T + kQpKeys - 1) / kQpKeys + 1;
-    pl.nsplit = 1;
     if (ctas < sms) pl.nsplit = (int)std::max<long long>(1, std::min<long long>(sms / ctas, tiles / 4));
-    if (pl.nsplit > 1) {
-      const size_t rows = (size_t)segs * (size_t)R;
-      pl.ml_off = (size_t)pl.nsplit * rows * kHeadDim * sizeof(float);
-      pl.bytes = pl.ml_off + (size_t)pl.nsplit * rows * 2 * sizeof(float);
-    }
+  }
+  if (pl.nsplit > 1) {
+    const size_t rows = (size_t)segs * (size_t)R;
+    pl.ml_off = (size_t)pl.nsplit * rows * kHeadDim * sizeof(float);
+    pl.bytes = pl.ml_off + (size_t)pl.nsplit * rows * 2 * sizeof(float);
   }
   *out = pl;
   return AL_OK;
@@ -90,6 +103,7 @@ int q8_attend_check(int B, int G, int h, int T, int C, int window, int sinks) {
   if (h > 64) return fail(AL_EUNSUPPORTED, "heads per group must be in [1, 64], got %d", h);
   if ((long long)h * T > (1 << 25)) return fail(AL_EUNSUPPORTED, "h*T = %lld exceeds 2^25 query rows per group", (long long)h * T);
   if (B * (long long)G * (((long long)h * T + 255) / 256) > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query tiles");
+  if (B * (long long)G * h * T > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query rows");
   (void)C;
   return AL_OK;
 }
@@ -100,9 +114,11 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
   const long long R = (long long)p.h * p.T;
   int rc;
   if (pl.token) {
+    if ((rc = prepare_kernel(q8_decode_kernel<T>, kQdSmem))) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)pl.cs, (unsigned)(p.B * p.G), (unsigned)((R + kQdCols - 1) / kQdCols));
+    cfg.gridDim = dim3((unsigned)(pl.nsplit > 1 ? pl.nsplit : pl.cs), (unsigned)(p.B * p.G), (unsigned)((R + kQdCols - 1) / kQdCols));
     cfg.blockDim = dim3(kQdThreads, 1, 1);
+    cfg.dynamicSmemBytes = kQdSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -110,19 +126,27 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (pl.cs > 8 && (rc = prepare_kernel(q8_decode_kernel<T>, 0))) return rc;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, q8_decode_kernel<T>, p);
-    return e == cudaSuccess ? AL_OK : cuda_fail(e, "q8_decode_kernel");
+    cfg.numAttrs = pl.cs > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, q8_decode_kernel<T>, p);
+    if (e != cudaSuccess) return cuda_fail(e, "q8_decode_kernel");
+  } else {
+    if ((rc = prepare_kernel(q8_prompt_kernel<T>, kQpSmem))) return rc;
+    const dim3 grid((unsigned)(p.B * p.G * pl.row_tiles), (unsigned)pl.nsplit);
+    q8_prompt_kernel<T><<<grid, kQpThreads, kQpSmem, st>>>(p);
+    if ((rc = plain_launch_check("q8_prompt_kernel"))) return rc;
   }
-  if ((rc = prepare_kernel(q8_prompt_kernel<T>, kQpSmem))) return rc;
-  const dim3 grid((unsigned)(p.B * p.G * pl.row_tiles), (unsigned)pl.nsplit);
-  q8_prompt_kernel<T><<<grid, kQpThreads, kQpSmem, st>>>(p);
-  if ((rc = plain_launch_check("q8_prompt_kernel"))) return rc;
   if (pl.nsplit > 1) {
-    const long long rows = (long long)p.B * p.G * R;
-    q8_merge_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
-    return plain_launch_check("q8_merge_kernel");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)p.B * p.G * R), 1, 1);
+    cfg.blockDim = dim3(32 * kQmWarps, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, q8_merge_kernel<T>, p);
+    if (e != cudaSuccess) return cuda_fail(e, "q8_merge_kernel");
   }
   return AL_OK;
 }
@@ -266,7 +290,7 @@ int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int si
   DeviceInfo* di = nullptr;
   if ((rc = device_info(&di))) return rc;
   Q8Plan pl;
-  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, di->sms, &pl))) return rc;
+  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, true, di->sms, &pl))) return rc;
   *bytes = pl.bytes;
   return AL_OK;
 }
@@ -287,7 +311,7 @@ int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_
   DeviceInfo* di = nullptr;
   if ((rc = device_info(&di))) return rc;
   Q8Plan pl;
-  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, di->sms, &pl))) return rc;
+  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, lengths != nullptr, di->sms, &pl))) return rc;
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)))
     return fail(AL_EINVAL, "this call needs a 16-byte aligned workspace of %zu bytes, got %zu", pl.bytes, workspace_bytes);
   Q8AttendParams p = {};

@@ -3,27 +3,34 @@
 //
 // A query at position p sees the tokens j <= p with window = 0, or j > p - window, or j < sinks. A CTA holds 8 columns
 // (query, head) of one (batch, group); its warps walk steps of 32 tokens and every warp keeps its own online softmax,
-// so no warp waits for another until the end. Per step a warp reads the 32 rows of K and V straight from global memory
-// into the registers of the tensor-core fragments (each row is 128 bytes, read as full lines): both contractions may
-// permute their summed index freely, so a thread's 16 contiguous bytes serve as the operand without a pass through
-// shared memory. K and V codes become f16 exactly; q and the softmax weights are split into two f16 terms that occupy
-// the two halves of the MMA's 16 rows (rows 0-7 high, 8-15 low), so 8 columns with about 21 bits each cost the same
-// MMAs as 16 columns with 11. The block's exponents enter as 2^(ek) on the scores and as an addend ev inside the
-// weights' exponent: weights are w = 2^(s + ev - m) with the running maximum m over s + ev, the output sums w * code,
-// and the denominator sums w * 2^-ev.
+// so no warp waits for another until the end. A warp streams its steps' K and V rows (8 KB a step) through a ring of its
+// own in shared memory with cp.async (16-byte chunks XOR-swizzled by row, rows past the end zero-filled) and reads them
+// as 16 bytes a lane straight into the tensor-core fragments: both contractions may permute their summed index, their
+// tokens and their dimensions freely, and the order is chosen so that no two lanes of a quarter warp share a bank. K and
+// V codes become f16 exactly; q and the softmax weights are split into two f16 terms that occupy the two halves of the
+// MMA's 16 rows (rows 0-7 high, 8-15 low), so 8 columns with about 21 bits each cost the same MMAs as 16 columns with
+// 11. The block's exponents enter as 2^(ek) on the scores and as an addend ev inside the weights' exponent: weights are
+// w = 2^(s + ev - m) with the running maximum m over s + ev, the output sums w * code, and the denominator sums
+// w * 2^-ev.
 //
 // Bound: HBM reads of 256 bytes per visible token and group. The work of a segment is split over a cluster of CTAs
-// whose partial (m, l, O) are merged through distributed shared memory, so one launch does the whole step.
+// whose partial (m, l, O) are merged through distributed shared memory, so one launch does the whole step; with so few
+// segments that clusters of 16 leave SMs idle, over as many CTAs as fill them, whose partials go through global memory to
+// q8_merge_kernel.
 #pragma once
 #include <cuda_fp16.h>
 #include "al_q8.cuh"
 
 namespace al {
 
+constexpr int kQ8TokenCols = 16;          // up to this many columns per group take this kernel, more the prompt kernel
 constexpr int kQdWarps = 4;
 constexpr int kQdThreads = 32 * kQdWarps;
 constexpr int kQdCols = 8;                 // columns (query, head) per CTA
 constexpr int kQdStep = 32;                // tokens per warp step (half a block: one exponent each for K and V)
+constexpr int kQdStages = 2;               // ring stages per warp
+constexpr uint32_t kQdStageBytes = 2 * kQdStep * kHeadDim;           // 8 KB: K rows, then V rows
+constexpr size_t kQdSmem = kQdWarps * kQdStages * kQdStageBytes;     // 64 KB
 constexpr float kQdBias = 10.0f;           // weights run up to 2^10, so f16's normal range starts 2^-24 below the largest
 
 struct Q8AttendParams {
@@ -39,7 +46,7 @@ struct Q8AttendParams {
   float scale;                             // |softmax scale| * log2 e; its sign is folded into q
   float qsign;
   void* out;                               // [B,G,h,T,128] contiguous
-  // tensor-core kernel for prompts: split of the key tiles and its partial results
+  // split of the key range over CTAs that write partial results (part null: none), and the prompt kernel's row tiles
   int nsplit, row_tiles;
   uint32_t h_magic;                        // r / h = (r * h_magic) >> 32 for the row numbers used (h > 1)
   float* part;                             // [nsplit][B*G][R][128] unnormalised O, R = T * h
@@ -120,9 +127,22 @@ __device__ __forceinline__ float q8_factor(float f_row, int ek) {
   return fminf(fmaxf(f_row * q8_exp2i(ek), 1.17549435e-38f), 3.0e38f);
 }
 
+// 16 bytes global -> shared, zeros when !in (nothing is read then).
+__device__ __forceinline__ void qd_copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 qd_lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// Two CTAs of four warps an SM: 297 us for 32 x 8 segments of 16K to 32K tokens; three CTAs (168 registers, spills) 366,
+// one of eight warps 302 to 321.
 template <typename T>
 __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8AttendParams p) {
-  __shared__ __align__(16) float s_o[kQdWarps][kQdCols][kHeadDim];
+  extern __shared__ __align__(1024) unsigned char qd_raw[];
+  float (*s_o)[kQdCols][kHeadDim] = reinterpret_cast<float (*)[kQdCols][kHeadDim]>(qd_raw);   // after the loop
   __shared__ float s_m[kQdWarps][kQdCols], s_l[kQdWarps][kQdCols];
   __shared__ float s_cm[kQdCols], s_cl[kQdCols];
 
@@ -141,6 +161,40 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   const int myp = n - p.T + mycol / p.h;                 // this thread's column: position
   const int plo = n - p.T + col0 / p.h, phi = n - p.T + col_last / p.h;
   const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQdStep);
+
+  const uint8_t* kbase = p.kc + (long long)bg * p.C * kHeadDim;
+  const uint8_t* vbase = p.vc + (long long)bg * p.C * kHeadDim;
+  const signed char* keb = p.ke + (long long)bg * p.NB;
+  const signed char* veb = p.ve + (long long)bg * p.NB;
+  const int W = cs * kQdWarps;
+  const uint32_t ring = smem_addr(qd_raw) + (uint32_t)warp * (kQdStages * kQdStageBytes);
+  auto step_token = [&](int s) { return (s < rg.ns ? s : rg.first + (s - rg.ns)) * kQdStep; };
+  // Copy a step: 8 lanes a row, 4 rows at a time; chunk c of row r goes to place c ^ (r & 7).
+  const int crow = lane >> 3, cch = lane & 7;
+  auto copy = [&](int s, int stage) {
+    if (s < rg.total) {
+      const int j0 = step_token(s) + crow;
+      const uint32_t dst = ring + (uint32_t)stage * kQdStageBytes + (uint32_t)crow * kHeadDim;
+      const long long at = (long long)j0 * kHeadDim + 16 * cch;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t d = dst + (uint32_t)i * 512u + (uint32_t)((cch ^ ((crow + 4 * i) & 7)) << 4);
+        const bool in = j0 + 4 * i < n;
+        qd_copy16(d, kbase + (in ? at + i * 512 : 0), in);
+        qd_copy16(d + kQdStep * kHeadDim, vbase + (in ? at + i * 512 : 0), in);
+      }
+    }
+    cp_async_commit();
+  };
+  int step = rank * kQdWarps + warp;
+#pragma unroll
+  for (int i = 0; i < kQdStages; ++i) copy(step + i * W, i);
+  int ek = 0, ev = 0;
+  if (step < rg.total) {
+    const int blk = step_token(step) / kQ8Block;
+    ek = keb[blk];
+    ev = veb[blk];
+  }
 
   // q fragments: k-slots (2t, 2t+1 | 2t+8, 2t+9) of MMA ks hold dimensions 4 ks .. 4 ks + 3 of the thread's 16-byte
   // pieces [16 t, 16 t + 16) (ks < 4) and [64 + 16 t, ...) (ks >= 4)
@@ -186,68 +240,37 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   float m = -INFINITY, l = 0.0f;
   int ev_top = -128;                                     // largest V exponent met so far
 
-  const uint8_t* kbase = p.kc + (long long)bg * p.C * kHeadDim;
-  const uint8_t* vbase = p.vc + (long long)bg * p.C * kHeadDim;
-  const signed char* keb = p.ke + (long long)bg * p.NB;
-  const signed char* veb = p.ve + (long long)bg * p.NB;
-
-  const int W = cs * kQdWarps;
-  int step = rank * kQdWarps + warp;
-  uint4 kr[8], vr[8];
-  int ek = 0, ev = 0;
-  auto step_token = [&](int s) { return (s < rg.ns ? s : rg.first + (s - rg.ns)) * kQdStep; };
-  auto load_k = [&](int j0) {
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-      const int j = j0 + 8 * nt + g8;
-      const uint8_t* r = kbase + (long long)j * kHeadDim + 16 * t4;
-      if (j < n) {
-        kr[2 * nt] = ldg_stream16(r);
-        kr[2 * nt + 1] = ldg_stream16(r + 64);
-      } else {
-        kr[2 * nt] = kr[2 * nt + 1] = make_uint4(0, 0, 0, 0);
-      }
-    }
-  };
-  auto load_v = [&](int j0) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int j = j0 + 16 * (i >> 2) + 8 * ((i >> 1) & 1) + 2 * t4 + (i & 1);
-      vr[i] = j < n ? ldg_stream16(vbase + (long long)j * kHeadDim + 16 * g8) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  int j0 = 0;
-  if (step < rg.total) {
-    j0 = step_token(step);
-    load_k(j0);
-    load_v(j0);
-    ek = keb[j0 / kQ8Block];
-    ev = veb[j0 / kQ8Block];
-  }
+  // Fragment addresses: K row of n index g8 is (g8 >> 1) + 4 (g8 & 1), its chunks t4 and t4 + 4; V row of k-slot 2t + u
+  // is t4 + 4u, its chunk (the n index g8) (g8 >> 1) + 4 (g8 & 1).
+  const int rho = (g8 >> 1) | ((g8 & 1) << 2);
+  const uint32_t ka0 = (uint32_t)rho * 128u + (uint32_t)((t4 ^ rho) << 4), ka1 = ka0 ^ 64u;
+  const uint32_t va0 = (uint32_t)t4 * 128u + (uint32_t)((rho ^ t4) << 4), va1 = (uint32_t)(t4 + 4) * 128u + (uint32_t)((rho ^ (t4 + 4)) << 4);
+  int stage = 0;
 #pragma unroll 1
   for (; step < rg.total; step += W) {
-    const int nxt = step + W;
-    const bool more = nxt < rg.total;
-    const int j1 = more ? step_token(nxt) : 0;
+    const int j0 = step_token(step);
+    cp_async_wait<kQdStages - 1>();
+    __syncwarp();
+    const uint32_t kst = ring + (uint32_t)stage * kQdStageBytes, vst = kst + kQdStep * kHeadDim;
     // scores: 4 n-tiles of 8 tokens
     float s[8];
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
-      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const uint32_t w[8] = {kr[2 * nt].x, kr[2 * nt].y, kr[2 * nt].z, kr[2 * nt].w,
-                             kr[2 * nt + 1].x, kr[2 * nt + 1].y, kr[2 * nt + 1].z, kr[2 * nt + 1].w};
+      const uint4 k0 = qd_lds16(kst + ka0 + (uint32_t)nt * 1024u), k1 = qd_lds16(kst + ka1 + (uint32_t)nt * 1024u);
+      float acc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};   // two chains of four MMAs
+      const uint32_t w[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks)
-        mma_f16_16816(acc, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], q8_decode_lo(w[ks]), q8_decode_hi(w[ks]));
-      s[2 * nt] = acc[0] + acc[2];
-      s[2 * nt + 1] = acc[1] + acc[3];
+        mma_f16_16816(acc[ks >> 2], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], q8_decode_lo(w[ks]), q8_decode_hi(w[ks]));
+      s[2 * nt] = (acc[0][0] + acc[1][0]) + (acc[0][2] + acc[1][2]);
+      s[2 * nt + 1] = (acc[0][1] + acc[1][1]) + (acc[0][3] + acc[1][3]);
     }
     const float f = q8_factor(f_row, ek), fev = (float)ev, inv_ev = q8_exp2i(-ev);
     const int ev_now = ev;
-    if (more) {
-      load_k(j1);
-      ek = keb[j1 / kQ8Block];
-      ev = veb[j1 / kQ8Block];
+    if (step + W < rg.total) {
+      const int blk = step_token(step + W) / kQ8Block;
+      ek = keb[blk];
+      ev = veb[blk];
     }
     // a step is whole when every column sees all of it
     const bool whole = j0 + kQdStep - 1 <= plo && (p.window == 0 || j0 > phi - p.window || j0 + kQdStep <= p.sinks);
@@ -256,7 +279,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int j = j0 + 8 * (i >> 1) + 2 * t4 + (i & 1);
+        const int j = j0 + 8 * (i >> 1) + 4 * (i & 1) + t4;
         if (!q8_sees(myp, j, p.window, p.sinks)) s[i] = -INFINITY;
       }
     }
@@ -295,13 +318,19 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
     } else {
       l += sum * inv_ev;
     }
+    uint4 vr[8];                                            // row 16 (i >> 2) + 8 (i >> 1 & 1) + 4 (i & 1) + t4
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vr[i] = qd_lds16(vst + ((i & 1) ? va1 : va0) + (uint32_t)(i >> 1) * 1024u);
+    __syncwarp();
+    copy(step + kQdStages * W, stage);
+    if (++stage == kQdStages) stage = 0;
     // O += P V. Rows that no column sees become zero codes. A NaN code in a row that only some columns see must not
     // reach the others (0 * NaN): such codes become zero too, and the columns that see them get their NaN here.
     if (!whole) {
       uint32_t bad = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int j = j0 + 16 * (i >> 2) + 8 * ((i >> 1) & 1) + 2 * t4 + (i & 1);
+        const int j = j0 + 8 * (i >> 1) + 4 * (i & 1) + t4;
         const bool none = j > phi || (p.window > 0 && j <= plo - p.window && j >= p.sinks);
         if (none) vr[i] = make_uint4(0, 0, 0, 0);
         bad |= q8_nan_mask(vr[i].x) | q8_nan_mask(vr[i].y) | q8_nan_mask(vr[i].z) | q8_nan_mask(vr[i].w);
@@ -315,11 +344,11 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
 #pragma unroll 1
         for (int j = j0; j < min(j0 + kQdStep, n); ++j) {
           if (!q8_sees(myp, j, p.window, p.sinks)) continue;
-          const uint8_t* v = vbase + (long long)j * kHeadDim + 32 * t4;
+          const uint8_t* v = vbase + (long long)j * kHeadDim + 16 * t4;
 #pragma unroll
           for (int d = 0; d < 16; ++d) {
             if ((v[d] & 0x7f) == 0x7f) o[d][0] = __uint_as_float(0x7fffffffu);
-            if ((v[16 + d] & 0x7f) == 0x7f) o[d][1] = __uint_as_float(0x7fffffffu);
+            if ((v[64 + d] & 0x7f) == 0x7f) o[d][1] = __uint_as_float(0x7fffffffu);
           }
         }
         __syncwarp();
@@ -340,27 +369,30 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
         mma_f16_16816(o[4 * w + 3], pa[ks][0], pa[ks][1], pa[ks][2], pa[ks][3], q8_decode_hi(xh), q8_decode_hi(yh));
       }
     }
-    if (more) load_v(j1);
-    j0 = j1;
   }
+  cp_async_wait<0>();
+  __syncthreads();                                          // the rings give way to the partial results
 
-  // the CTA's partial: thread holds column g8, dimensions 32 t + j (o[j][0] + o[j][2]) and 32 t + 16 + j
+  // the CTA's partial: thread holds column g8, dimensions 16 t + j (o[j][0] + o[j][2]) and 64 + 16 t + j
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
-    *reinterpret_cast<float4*>(&s_o[warp][g8][32 * t4 + j]) =
+    *reinterpret_cast<float4*>(&s_o[warp][g8][16 * t4 + j]) =
         make_float4(o[j][0] + o[j][2], o[j + 1][0] + o[j + 1][2], o[j + 2][0] + o[j + 2][2], o[j + 3][0] + o[j + 3][2]);
-    *reinterpret_cast<float4*>(&s_o[warp][g8][32 * t4 + 16 + j]) =
+    *reinterpret_cast<float4*>(&s_o[warp][g8][64 + 16 * t4 + j]) =
         make_float4(o[j][1] + o[j][3], o[j + 1][1] + o[j + 1][3], o[j + 2][1] + o[j + 2][3], o[j + 3][1] + o[j + 3][3]);
   }
   if (t4 == 0) { s_m[warp][g8] = m; s_l[warp][g8] = l; }
   __syncthreads();
-  // merge the warps into s_o[0]: thread d (0..127) takes dimension d of every column
+  // merge the warps into s_o[0]: a thread takes one dimension of every NT-th column
   {
-    float acc[kQdCols];
+    constexpr int NT = kQdThreads / kHeadDim, NC = kQdCols / NT;
+    const int d = tid % kHeadDim, c0 = tid / kHeadDim;
+    float acc[NC];
 #pragma unroll
-    for (int c = 0; c < kQdCols; ++c) {
+    for (int i = 0; i < NC; ++i) {
+      const int c = c0 + i * NT;
       float M = s_m[0][c];
 #pragma unroll
       for (int w = 1; w < kQdWarps; ++w) M = fmaxf(M, s_m[w][c]);
@@ -368,18 +400,29 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
 #pragma unroll
       for (int w = 0; w < kQdWarps; ++w) {
         const float e = q8_merge_weight(s_l[w][c], s_m[w][c], M);
-        a += e != 0.0f ? e * s_o[w][c][tid] : 0.0f;
+        a += e != 0.0f ? e * s_o[w][c][d] : 0.0f;
         L += q8_merge_l(s_l[w][c], s_m[w][c], M);
       }
-      acc[c] = a;
-      if (tid == c) { s_cm[c] = M; s_cl[c] = L; }
+      acc[i] = a;
+      if (d == 0) { s_cm[c] = M; s_cl[c] = L; }
     }
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < kQdCols; ++c) s_o[0][c][tid] = acc[c];
+    for (int i = 0; i < NC; ++i) s_o[0][c0 + i * NT][d] = acc[i];
   }
   const int ncol = col_last - col0 + 1;
-  if (cs > 1) {
+  if (p.part) {
+    __syncthreads();
+    const long long row0 = ((long long)rank * gridDim.y + bg) * R + col0;
+    for (int i = tid; i < ncol * (kHeadDim / 4); i += kQdThreads) {
+      const int c = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4));
+      *reinterpret_cast<float4*>(p.part + (row0 + c) * kHeadDim + d) = *reinterpret_cast<const float4*>(&s_o[0][c][d]);
+    }
+    if (tid < ncol) {
+      p.part_ml[(row0 + tid) * 2] = s_cm[tid];
+      p.part_ml[(row0 + tid) * 2 + 1] = s_cl[tid];
+    }
+  } else if (cs > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     // rank r merges every cs-th (column, 4 dimensions) piece over the CTAs

@@ -21,6 +21,7 @@ nothing synchronises, ValueError for shapes, dtypes and ranges.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -31,7 +32,6 @@ from . import _lib
 BLOCK = 64                     # tokens that share one exponent
 HEAD_DIM = 128
 LAYOUTS = {"half": 0, "interleaved": 1}
-TOKEN_ROWS = 16                # up to this many query rows per group attention needs no workspace (AL_Q8_TOKEN_COLS)
 _CODES = torch.float8_e4m3fn
 _DTYPES = {torch.float32: _lib.AL_F32, torch.bfloat16: _lib.AL_BF16}
 
@@ -284,6 +284,14 @@ def read_q8(cache, lo: int, hi: int, *, dtype=torch.bfloat16):
     return k_out, v_out
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(dev: int, B: int, G: int, h: int, T: int, C: int, window: int, sinks: int, most: int) -> int:
+    """What al_attend_q8 needs for a call of these sizes (the answer depends on nothing else)."""
+    need = ctypes.c_size_t(0)
+    _call_on(dev, _lib.load().al_attend_q8_workspace, B, G, h, T, C, window, sinks, most, ctypes.byref(need))
+    return need.value
+
+
 def attend_q8(q: torch.Tensor, cache, lengths, *, window: int = 0, sinks: int = 0, scale=None, max_length=None):
     """Attention of q [B,G,h,T,d] over the cache, causal: the query at position p sees the tokens j <= p, with a
     `window` > 0 only those with j > p - window or j < sinks. A row that sees nothing is zero. `max_length` (default: the
@@ -305,14 +313,9 @@ def attend_q8(q: torch.Tensor, cache, lengths, *, window: int = 0, sinks: int = 
     q, qp, qs = _rows(q)
     out = q.new_empty(shape)
     lib = _lib.load()
-    work, wp, wn = None, None, 0
-    if h * T > TOKEN_ROWS:
-        need = ctypes.c_size_t(0)
-        _call_on(dev, lib.al_attend_q8_workspace, B, G, h, T, C, window, sinks, most, ctypes.byref(need))
-        wn = need.value
-        if wn:
-            work = torch.empty(wn, dtype=torch.uint8, device=q.device)
-            wp = work.data_ptr()
+    wn = _workspace_bytes(dev, B, G, h, T, C, window, sinks, most)
+    work = torch.empty(wn, dtype=torch.uint8, device=q.device) if wn else None
+    wp = work.data_ptr() if wn else None
     _call(dev, lib.al_attend_q8, qp, qs[0], qs[1], qs[2], qs[3], code, k.data_ptr(), v.data_ptr(), ke.data_ptr(),
           ve.data_ptr(), lp, length, B, G, h, T, C, d, window, sinks, 1.0 / math.sqrt(d) if scale is None else float(scale),
           most, out.data_ptr(), wp, wn)
