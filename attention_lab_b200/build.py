@@ -1,4 +1,5 @@
-"""Build the sm_100a C-ABI library in-tree: attention_lab_b200/libattention_lab_b200.so.
+"""Build the sm_100a C-ABI library in-tree, attention_lab_b200/libattention_lab_b200.so, and the Python binding of its
+8-bit cache operators, attention_lab_b200/_q8_bind.so (C++ against the installed torch, linked to the library).
 
     python -m attention_lab_b200.build [--verbose]
 
@@ -9,16 +10,19 @@ again when its source, a header or this file is newer. `--verbose` adds `-Xptxas
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 SRC = PKG / "csrc"
 LIB = PKG / "libattention_lab_b200.so"
+BIND = PKG / "_q8_bind.so"
 OBJ = PKG / "_build"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -31,11 +35,11 @@ def nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(SRC.glob("*.cu")) + sorted(SRC.glob("*.cuh")) + sorted(SRC.glob("*.h")) + [PKG.parent / "include" / "attention_lab_b200.h"]
+    return sorted(SRC.glob("*.cu")) + sorted(SRC.glob("*.cpp")) + sorted(SRC.glob("*.cuh")) + sorted(SRC.glob("*.h")) + [PKG.parent / "include" / "attention_lab_b200.h"]
 
 
 def up_to_date() -> bool:
-    return LIB.exists() and all(LIB.stat().st_mtime >= s.stat().st_mtime for s in sources())
+    return all(out.exists() and all(out.stat().st_mtime >= s.stat().st_mtime for s in sources()) for out in (LIB, BIND))
 
 
 def included(src: Path) -> set[Path]:
@@ -53,6 +57,21 @@ def included(src: Path) -> set[Path]:
     return seen
 
 
+def bind_command(obj: Path) -> list[str]:
+    """The compiler line of the binding's object (no torch import: its headers are found by location)."""
+    torch_dir = Path(importlib.util.find_spec("torch").origin).parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", str(torch_dir / "include"),
+            "-I", sysconfig.get_paths()["include"], "-I", str(cuda / "include"), "-c", str(SRC / "bind_q8.cpp"),
+            "-o", str(obj) + ".tmp"]
+
+
+def link_bind(obj: Path) -> list[str]:
+    torch_lib = Path(importlib.util.find_spec("torch").origin).parent / "lib"
+    return ["g++", "-shared", str(obj), "-L", str(PKG), "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN", "-L", str(torch_lib),
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-o", str(BIND) + ".tmp"]
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
     if up_to_date() and not force:
         return LIB
@@ -61,15 +80,17 @@ def build(verbose: bool = False, force: bool = False) -> Path:
              "-I", str(PKG.parent / "include")]
     if verbose:
         flags.insert(1, "-Xptxas=-v")
+    commands = {src: lambda obj, src=src: [*flags, "-c", str(src), "-o", str(obj) + ".tmp"] for src in sorted(SRC.glob("*.cu"))}
+    commands[SRC / "bind_q8.cpp"] = bind_command
     jobs, objects = [], []
-    for src in sorted(SRC.glob("*.cu")):
+    for src, command in commands.items():
         obj = OBJ / (src.stem + ".o")
-        objects.append(str(obj))
+        if src.suffix == ".cu":
+            objects.append(str(obj))
         if not force and obj.exists() and all(obj.stat().st_mtime >= f.stat().st_mtime
                                               for f in included(src) | {Path(__file__).resolve()}):
             continue
-        jobs.append((obj, subprocess.Popen([*flags, "-c", str(src), "-o", str(obj) + ".tmp"], stdout=subprocess.PIPE,
-                                           stderr=subprocess.STDOUT, text=True)))
+        jobs.append((obj, subprocess.Popen(command(obj), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = False
     for obj, job in jobs:
         out = job.communicate()[0]
@@ -80,13 +101,14 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         else:
             os.replace(str(obj) + ".tmp", obj)
     if failed:
-        raise RuntimeError("nvcc failed")
-    res = subprocess.run([nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", *objects,
-                          "-o", str(LIB) + ".tmp"], capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError(f"linking failed with exit code {res.returncode}")
-    os.replace(str(LIB) + ".tmp", LIB)
+        raise RuntimeError("compilation failed")
+    for out, command in ((LIB, [nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", *objects,
+                                "-o", str(LIB) + ".tmp"]), (BIND, link_bind(OBJ / "bind_q8.o"))):
+        res = subprocess.run(command, capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError(f"linking {out.name} failed with exit code {res.returncode}")
+        os.replace(str(out) + ".tmp", out)
     return LIB
 
 
