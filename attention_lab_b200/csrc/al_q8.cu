@@ -137,7 +137,9 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
   }
   if (pl.nsplit > 1) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)p.B * p.G * R), 1, 1);
+    const long long rows = (long long)p.B * p.G * R;
+    const bool wide = pl.nsplit > 8;                       // warps per row: 8, or 1
+    cfg.gridDim = dim3((unsigned)(wide ? rows : (rows + kQmWarps - 1) / kQmWarps), 1, 1);
     cfg.blockDim = dim3(32 * kQmWarps, 1, 1);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -145,7 +147,8 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, q8_merge_kernel<T>, p);
+    const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, q8_merge_kernel<T, kQmWarps>, p)
+                               : cudaLaunchKernelEx(&cfg, q8_merge_kernel<T, 1>, p);
     if (e != cudaSuccess) return cuda_fail(e, "q8_merge_kernel");
   }
   return AL_OK;

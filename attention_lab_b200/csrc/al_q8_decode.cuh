@@ -425,20 +425,45 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   } else if (cs > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    // rank r merges every cs-th (column, 4 dimensions) piece over the CTAs
+    // Every CTA's (m, l), one remote load a thread, into a table of weights; then rank r sums every cs-th (column,
+    // 4 dimensions) piece over the CTAs with its remote loads in flight together. (Read one after the other in two
+    // loops these loads took about 3 us.)
+    __shared__ float s_gm[kMaxCluster][kQdCols], s_gl[kMaxCluster][kQdCols];
+    const int gr = tid >> 3, gc = tid & 7;                 // kMaxCluster * kQdCols = kQdThreads
+    static_assert(kMaxCluster * kQdCols == kQdThreads && kQdCols == 8, "one thread per (CTA, column)");
+    float mr = -INFINITY, lr = 0.0f;
+    if (gr < cs) {
+      mr = *cluster.map_shared_rank(&s_cm[gc], gr);
+      lr = *cluster.map_shared_rank(&s_cl[gc], gr);
+    }
+    s_gm[gr][gc] = mr;
+    __syncthreads();
+    float M = s_gm[0][gc];
+#pragma unroll
+    for (int r = 1; r < kMaxCluster; ++r) M = fmaxf(M, s_gm[r][gc]);
+    s_gl[gr][gc] = q8_merge_l(lr, mr, M);
+    __syncthreads();
+    s_gm[gr][gc] = q8_merge_weight(lr, mr, M);             // the weight takes the maximum's place
+    __syncthreads();
     for (int i = rank * kQdThreads + tid; i < ncol * (kHeadDim / 4); i += cs * kQdThreads) {
       const int c = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4));
-      float M = -INFINITY;
-      for (int r = 0; r < cs; ++r) M = fmaxf(M, *cluster.map_shared_rank(&s_cm[c], r));
       float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       float L = 0.0f;
-      for (int r = 0; r < cs; ++r) {
-        const float mr = *cluster.map_shared_rank(&s_cm[c], r), lr = *cluster.map_shared_rank(&s_cl[c], r);
-        const float e = q8_merge_weight(lr, mr, M);
-        L += q8_merge_l(lr, mr, M);
-        if (e == 0.0f) continue;
-        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s_o[0][c][d], r));
-        a.x += e * v.x; a.y += e * v.y; a.z += e * v.z; a.w += e * v.w;
+#pragma unroll
+      for (int r0 = 0; r0 < kMaxCluster; r0 += 8) {
+        if (r0 >= cs) break;
+        float4 v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r0 + r < cs) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s_o[0][c][d], r0 + r));
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          if (r0 + r >= cs) break;
+          const float e = s_gm[r0 + r][c];
+          L += s_gl[r0 + r][c];
+          if (e == 0.0f) continue;
+          a.x += e * v[r].x; a.y += e * v[r].y; a.z += e * v[r].z; a.w += e * v[r].w;
+        }
       }
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;
       const int cc = col0 + c, hd = cc % p.h, t = cc / p.h;

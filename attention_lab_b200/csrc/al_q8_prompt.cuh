@@ -621,53 +621,58 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   if (warp == 12) tmem_dealloc(tm, 512);
 }
 
-// Merge of the key splits: one CTA per row, the splits over its warps, a lane per 4 dimensions, then over the warps
-// through shared memory. Launched so that it may start while the splits still run; it waits for them first.
+// Merge of the key splits: WPR warps per row share the splits, a lane per 4 dimensions, then meet in shared memory (8
+// for many splits of few rows, a token's; 1 for few splits of many rows, a prompt's). Launched so that it may start while
+// the splits still run; it waits for them first.
 constexpr int kQmWarps = 8;
-template <typename T>
+template <typename T, int WPR>
 __global__ void __launch_bounds__(32 * kQmWarps) q8_merge_kernel(const Q8AttendParams p) {
   __shared__ float s_m[kQmWarps], s_l[kQmWarps];
   __shared__ __align__(16) float s_o[kQmWarps][kHeadDim];
   const int BG = p.B * p.G, R = p.h * p.T, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
-  const long long row = blockIdx.x, rows = (long long)BG * R;
+  const int first = warp - warp % WPR, part = warp % WPR;  // the row's first warp; this warp takes splits part + WPR i
+  const long long rows = (long long)BG * R, row = min((long long)blockIdx.x * (kQmWarps / WPR) + warp / WPR, rows - 1);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  // the common maximum: a lane per split (nsplit <= 32 * kQmWarps)
-  const int mine = warp + kQmWarps * lane;
+  // the common maximum: a lane per split (nsplit <= 32 * WPR)
+  const int mine = part + WPR * lane;
   float2 ml = make_float2(-INFINITY, 0.0f);
   if (mine < p.nsplit) ml = *reinterpret_cast<const float2*>(p.part_ml + ((long long)mine * rows + row) * 2);
   float M = ml.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (lane == 0) s_m[warp] = M;
-  __syncthreads();
+  if (WPR > 1) {
+    if (lane == 0) s_m[warp] = M;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kQmWarps; ++w) M = fmaxf(M, s_m[w]);
+    for (int w = 0; w < WPR; ++w) M = fmaxf(M, s_m[first + w]);
+  }
   const float wgt = q8_merge_weight(ml.y, ml.x, M);
   float L = q8_merge_l(ml.y, ml.x, M);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-  for (int i = 0; warp + kQmWarps * i < p.nsplit; ++i) {
+  for (int i = 0; part + WPR * i < p.nsplit; ++i) {
     const float e = __shfl_sync(0xffffffffu, wgt, i);
     if (e == 0.0f) continue;                             // also an empty split, whose O was not written
-    const float4 v = *reinterpret_cast<const float4*>(p.part + ((long long)(warp + kQmWarps * i) * rows + row) * kHeadDim + d);
+    const float4 v = *reinterpret_cast<const float4*>(p.part + ((long long)(part + WPR * i) * rows + row) * kHeadDim + d);
     a.x += e * v.x; a.y += e * v.y; a.z += e * v.z; a.w += e * v.w;
   }
-  *reinterpret_cast<float4*>(&s_o[warp][d]) = a;
-  if (lane == 0) s_l[warp] = L;
-  __syncthreads();
-  if (threadIdx.x >= kHeadDim) return;
-  float o = 0.0f;
-  L = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kQmWarps; ++w) {
-    o += s_o[w][threadIdx.x];
-    L += s_l[w];
+  if (WPR > 1) {
+    *reinterpret_cast<float4*>(&s_o[warp][d]) = a;
+    if (lane == 0) s_l[warp] = L;
+    __syncthreads();
+    if (part > 0) return;
+    for (int w = 1; w < WPR; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(&s_o[first + w][d]);
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+      L += s_l[first + w];
+    }
   }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   const int bg = (int)(row / R), r = (int)(row - (long long)bg * R), t = r / p.h, head = r - t * p.h;
-  static_cast<T*>(p.out)[(((long long)bg * p.h + head) * p.T + t) * kHeadDim + threadIdx.x] =
-      fromf<T>(L == 0.0f ? 0.0f : o / L);
+  T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim + d;
+  dst[0] = fromf<T>(a.x * inv); dst[1] = fromf<T>(a.y * inv); dst[2] = fromf<T>(a.z * inv); dst[3] = fromf<T>(a.w * inv);
 }
 
 }  // namespace al
