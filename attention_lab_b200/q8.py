@@ -69,8 +69,8 @@ def _layout(layout: str) -> int:
         raise ValueError(f"unknown layout {layout!r}; choose from {tuple(LAYOUTS)}") from None
 
 
-def rotary_table(length: int, rotary_dim: int = HEAD_DIM, *, base: float = 10000.0, scaling=None,
-                 device="cuda") -> torch.Tensor:
+def rotary_table(length: int, rotary_dim: int = HEAD_DIM, *, base: float = 10000.0, scaling=None, frequencies=None,
+                 amplitude: float = 1.0, device="cuda") -> torch.Tensor:
     """The rotary table [length, rotary_dim] (float32: cosines, then sines) of positions 0 .. length - 1 at frequencies
     base^(-2i/rotary_dim), computed in float64. `scaling` stretches the context by `factor`:
 
@@ -83,13 +83,18 @@ def rotary_table(length: int, rotary_dim: int = HEAD_DIM, *, base: float = 10000
     length, rot = int(length), int(rotary_dim)
     if length < 1 or rot < 2 or rot % 2:
         raise ValueError("need length >= 1 and an even rotary_dim >= 2")
+    if frequencies is not None:
+        if scaling is not None or frequencies.shape != (rot // 2,):
+            raise ValueError("frequencies must be [rotary_dim / 2], without scaling")
+        ang = torch.arange(length, dtype=torch.float64, device=device)[:, None] * frequencies.to(device).double()
+        return (torch.cat([ang.cos(), ang.sin()], dim=1) * amplitude).float().contiguous()
     scaling = dict(scaling or {"type": "none"})
     kind, s = scaling.pop("type", None), float(scaling.pop("factor", 1.0))
     if not s > 0:
         raise ValueError("the scaling factor must be positive")
     i = torch.arange(rot // 2, dtype=torch.float64, device=device)
     pos = torch.arange(length, dtype=torch.float64, device=device)
-    amp = 1.0
+    amp = float(amplitude)
     if kind == "ntk":
         if rot < 4:
             raise ValueError("ntk scaling needs rotary_dim >= 4")
@@ -106,7 +111,7 @@ def rotary_table(length: int, rotary_dim: int = HEAD_DIM, *, base: float = 10000
         turns = freq * float(scaling.pop("original")) / (2 * math.pi)
         keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
         freq = freq * keep + freq / s * (1.0 - keep)
-        amp = float(scaling.pop("amplitude", 0.1 * math.log(s) + 1.0))
+        amp *= float(scaling.pop("amplitude", 0.1 * math.log(s) + 1.0))
     elif kind not in ("none", "ntk"):
         raise ValueError(f"unknown scaling type {kind!r}")
     if scaling:

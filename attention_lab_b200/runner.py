@@ -15,6 +15,9 @@ What runs where:
                         gather-free attention, one launch per layer
     selectors B / C     their row lists (selection rules of decode.py:94-127), then al_gathered_attend
     full decode (A)     al_dense_decode over [0, legal length) (or torch SDPA, decode_backend="sdpa_fold")
+    8-bit cache         make_state(..., cache_format="q8"): per layer one append_q8 (q and k rotated, K/V quantised as they
+                        are written) and one attend_q8 (prompt chunks and single tokens alike; optional sliding window
+                        with first tokens that stay visible). Full mode only; half the cache bytes of bfloat16
     prefill read        torch scaled_dot_product_attention over [0, L0 + T) with the legality mask (a dense,
                         compute-bound read outside the decode hot path; full.py:17-45 sdpa_fold semantics)
 
@@ -32,7 +35,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import ops
+from . import ops, q8
 from .selection import FIXED_PREFIX, FIXED_RECENT, fixed_budget, row_offsets, selection_layout
 
 try:  # transformers is needed by the wrapper only; the operators import without it
@@ -144,6 +147,56 @@ class LabCache:
         return {"kv_bytes": kv, "index_bytes": z, "total_bytes": kv + z}
 
 
+class Q8LabCache(LabCache):
+    """The 8-bit form of the static cache: per layer a q8.Q8Cache (e4m3 codes, one exponent per 64 tokens and head) in
+    place of K/V, and the rotary table that K and q are rotated with as they are written. One legal length for all
+    layers, as in LabCache. A rollback keeps the exponents of the block it ends in: rows appended there again share a
+    block exponent at least as large as before."""
+
+    def __init__(self, *, layers: int, batch: int, groups: int, capacity: int, head_dim: int, table: torch.Tensor, device):
+        if int(capacity) <= 0 or int(layers) <= 0:
+            raise ValueError("capacity and layers must be positive")
+        if table.shape[0] < int(capacity):
+            raise ValueError(f"the rotary table's {table.shape[0]} rows do not cover the capacity {capacity}")
+        self.layers, self.batch, self.groups = int(layers), int(batch), int(groups)
+        self.capacity, self.head_dim = int(capacity), int(head_dim)
+        self.index_dim, self.z = None, None
+        self.device = torch.device(device)
+        self.table = table
+        self.kv = [q8.Q8Cache.empty(self.batch, self.groups, self.capacity, self.device, self.head_dim)
+                   for _ in range(self.layers)]
+        self.valid_length = 0
+        self.writes = [0] * self.layers
+        self.last_write = [None] * self.layers
+        self._pending = None
+
+    def append(self, layer: int, k_pre: torch.Tensor, v: torch.Tensor, q_pre: torch.Tensor) -> torch.Tensor:
+        """Rotate k_pre [B,G,T,d] and q_pre [B,G,h,T,d] to [valid_length, valid_length + T), write K and V there and
+        return the rotated q. Exactly once per layer per forward."""
+        start, T = self.valid_length, int(k_pre.shape[2])
+        if start + T > self.capacity:
+            raise RuntimeError(f"cache capacity {self.capacity} exceeded: valid {start} + new {T}")
+        if self._pending is None:
+            self._pending = T
+        elif self._pending != T:
+            raise RuntimeError("layers appended different lengths within one forward")
+        q_main = q8.append_q8(self.kv[layer], start + T, k_pre, v, q=q_pre, table=self.table)
+        self.writes[layer] += 1
+        self.last_write[layer] = (start, T)
+        return q_main
+
+    def clone(self) -> "Q8LabCache":
+        new = Q8LabCache.__new__(Q8LabCache)
+        new.__dict__.update({k: v for k, v in self.__dict__.items() if k not in ("kv", "writes", "last_write")})
+        new.kv = [q8.Q8Cache(*(t.clone() for t in layer)) for layer in self.kv]
+        new.writes, new.last_write = list(self.writes), list(self.last_write)
+        return new
+
+    def bytes(self) -> dict:
+        kv = sum(t.numel() * t.element_size() for layer in self.kv for t in layer)
+        return {"kv_bytes": kv, "index_bytes": 0, "total_bytes": kv}
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # per-step plan
 # ---------------------------------------------------------------------------------------------------------------------
@@ -241,7 +294,15 @@ class LabState:
 
     def __init__(self, cache: LabCache, indexers=None, *, mode: str = "full", selector: str = "index",
                  uniform_seed: int = 0, sparse_layers=None, cache_guard=None, canonical_order=False,
-                 decode_backend: str = "kernel"):
+                 decode_backend: str = "kernel", window: int = 0, sinks: int = 0):
+        self.eight_bit = isinstance(cache, Q8LabCache)
+        if self.eight_bit and (mode != "full" or decode_backend != "kernel"):
+            raise ValueError("an 8-bit cache is read in full mode by its own kernels")
+        if not self.eight_bit and (window or sinks):
+            raise ValueError("window and sinks need an 8-bit cache (cache_format='q8')")
+        if int(window) < 0 or int(sinks) < 0:
+            raise ValueError("window and sinks must not be negative")
+        self.window, self.sinks = int(window), int(sinks)
         if mode not in ("full", "sparse"):
             raise ValueError("mode must be 'full' or 'sparse'")
         if decode_backend not in DECODE_BACKENDS:
@@ -336,6 +397,8 @@ class LabAttention(nn.Module):
         q_pre = inner.q_norm(inner.q_proj(hidden_states).view(shape)).transpose(1, 2)   # [B,H,T,d], before RoPE
         k_pre = inner.k_norm(inner.k_proj(hidden_states).view(shape)).transpose(1, 2)   # [B,G,T,d], before RoPE
         v = inner.v_proj(hidden_states).view(shape).transpose(1, 2)
+        if st.eight_bit:
+            return inner.o_proj(self._read_q8(st, q_pre, k_pre, v)), None
         cos, sin = position_embeddings
         q_main, k_main = apply_rotary_pos_emb(q_pre, k_pre, cos, sin)
         cache, l = st.cache, self.layer_idx
@@ -387,6 +450,21 @@ class LabAttention(nn.Module):
         return inner.o_proj(attn), None
 
 
+    def _read_q8(self, st, q_pre, k_pre, v):
+        """The 8-bit cache's read: one quantising append (which rotates q and k) and one attention launch, for prompt
+        chunks and single tokens alike. Returns [B,T,H*d]."""
+        cache, l = st.cache, self.layer_idx
+        B, _, T, d = q_pre.shape
+        if st.phase not in ("prefill", "decode"):
+            raise RuntimeError("LabState.phase must be 'prefill' or 'decode' (set by LabRunner.prefill / "
+                               "LabRunner.step); the phase is never inferred from the input length")
+        if st.phase == "decode" and T != 1:
+            raise RuntimeError("a decode step takes exactly one new token")
+        q = cache.append(l, k_pre, v, q_pre.view(B, self.num_groups, self.heads_per_group, T, d))
+        out = q8.attend_q8(q, cache.kv[l], cache.valid_length + T, window=st.window, sinks=st.sinks, scale=self.scaling)
+        return out.reshape(B, self.num_heads, T, d).transpose(1, 2).reshape(B, T, self.num_heads * d)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # geometry, construction, wrap / unwrap
 # ---------------------------------------------------------------------------------------------------------------------
@@ -434,6 +512,22 @@ def make_cache(model, capacity: int, *, with_index: bool, index_dim: int = 32, b
                     dtype=p.dtype if dtype is None else dtype, index_dtype=index_dtype)
 
 
+def model_rotary_table(model, length: int, device=None) -> torch.Tensor:
+    """The model's own rotary frequencies and scaling as a q8 rotary table [length, head_dim] (half layout)."""
+    rot = model.model.rotary_emb
+    device = rot.inv_freq.device if device is None else device
+    return q8.rotary_table(length, 2 * rot.inv_freq.numel(), frequencies=rot.inv_freq,
+                           amplitude=float(getattr(rot, "attention_scaling", 1.0)), device=device)
+
+
+def make_q8_cache(model, capacity: int, *, batch: int = 1, device=None) -> Q8LabCache:
+    geo = geometry_of(model)
+    p = next(model.parameters())
+    device = p.device if device is None else device
+    return Q8LabCache(layers=geo.layers, batch=batch, groups=geo.groups, capacity=capacity, head_dim=geo.head_dim,
+                      table=model_rotary_table(model, capacity, device), device=device)
+
+
 def make_indexers(model, *, r: int = 32, seed: int = 0, dtype=None, device=None) -> list[Indexer]:
     """One untrained grouped indexer per layer, seeded seed * 1000 + layer (qwen_wrap.py:376-381)."""
     geo = geometry_of(model)
@@ -443,9 +537,16 @@ def make_indexers(model, *, r: int = 32, seed: int = 0, dtype=None, device=None)
 
 
 def make_state(model, capacity: int, mode: str, *, selector: str = "index", r: int = 32, seed: int = 0,
-               batch: int = 1, index_dtype=None, **kw) -> LabState:
+               batch: int = 1, index_dtype=None, cache_format: str = "plain", **kw) -> LabState:
     """A: mode "full". D0: mode "sparse" (index table + indexers). B / C: mode "sparse" with selector "recent" /
-    "uniform" (no index table)."""
+    "uniform" (no index table). cache_format "q8": mode "full" over an 8-bit cache, with `window` and `sinks` for a
+    sliding window whose first tokens stay visible."""
+    if cache_format not in ("plain", "q8"):
+        raise ValueError("cache_format must be 'plain' or 'q8'")
+    if cache_format == "q8":
+        if mode != "full":
+            raise ValueError("an 8-bit cache is read in full mode by its own kernels")
+        return LabState(make_q8_cache(model, capacity, batch=batch), None, mode=mode, selector=selector, **kw)
     with_index = mode == "sparse" and selector == "index"
     cache = make_cache(model, capacity, with_index=with_index, index_dim=r, batch=batch, index_dtype=index_dtype)
     idx = make_indexers(model, r=r, seed=seed, dtype=cache.index_dtype) if with_index else None
