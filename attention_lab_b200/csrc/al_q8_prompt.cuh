@@ -121,9 +121,6 @@ __device__ __forceinline__ float qp_max3(float a, float b, float c) {
 __device__ __forceinline__ void qp_st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-__device__ __forceinline__ void qp_st_shared8(uint32_t a, uint32_t x, uint32_t y) {
-  asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(a), "r"(x), "r"(y) : "memory");
-}
 __device__ __forceinline__ uint4 qp_ld_shared16(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -161,8 +158,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   // the longest row tiles first; all (batch, group) pairs of a row tile together
   const int BG = p.B * p.G, R = p.h * p.T;
   const int split = blockIdx.y;
-  const int tile = p.row_tiles - 1 - (int)(blockIdx.x / BG), bg = (int)(blockIdx.x % BG);
-  const int b = bg / p.G, g = bg - b * p.G;
+  const int tile = p.row_tiles - 1 - (int)(blockIdx.x / (unsigned)BG), bg = (int)(blockIdx.x % (unsigned)BG);
+  const int b = (int)((unsigned)bg / (unsigned)p.G), g = bg - b * p.G;
   int n = __shfl_sync(0xffffffffu, q8_length(p.len, b), 0);
   if (n < 0 || n > p.C) {
     if (tid == 0) atomicOr(p.err, kErrQ8Range);
@@ -173,7 +170,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   const int pbase = n - p.T;
   const int plo = pbase + qp_row_token(r0, p), phi = pbase + qp_row_token(min(r0 + 2 * kQpRows - 1, R - 1), p);
   const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQpKeys);
-  const int it0 = (int)((long long)rg.total * split / p.nsplit), it1 = (int)((long long)rg.total * (split + 1) / p.nsplit);
+  // (total < 2^24 and nsplit <= 148: the products fit 32 bits)
+  const int it0 = (int)((unsigned)rg.total * (unsigned)split / (unsigned)p.nsplit);
+  const int it1 = (int)((unsigned)rg.total * (unsigned)(split + 1) / (unsigned)p.nsplit);
   const int nt = it1 - it0;
   auto tile_token = [&](int it) { return (it < rg.ns ? it : rg.first + (it - rg.ns)) * kQpKeys; };
 
@@ -210,56 +209,66 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       const uint32_t tS = tm + lanes + (uint32_t)qt * 128u, tO = tm + lanes + 256u + (uint32_t)qt * 128u;
       const int wrow0 = (warp & 3) * 32;               // the warp's first row of the tile
       const uint32_t qtile = s_q + (uint32_t)(qt * QP) * kQpTile;
-      // The warp's 32 query rows: L lanes read one row (full lines), BATCH loads in flight while the batch before is
-      // scaled by its rows' powers of two, split and stored.
+      // The warp's 32 query rows come straight into their places in the query tile (full lines, all copies in flight;
+      // 32-bit rows fill the places of both terms), then every thread scales its row by a power of two and splits it.
       {
-        constexpr int E = V16<T>::n, L = kHeadDim / E, PER = 32 / L, BATCH = 4;
-        const int sub = lane / L, c = lane % L;
-        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + E * c;
-        uint4 x[BATCH];
-        auto ask = [&](int i0) {
+        constexpr int CH = kHeadDim * (int)sizeof(T) / 16, PER = 32 / CH;   // 16-byte chunks a row, rows at a time
+        const int c = lane % CH;
+        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + V16<T>::n * c;
+        const uint32_t chunk_tile = qtile + (uint32_t)(c >> 4) * kQpTile;
+#pragma unroll 4
+        for (int i = 0; i < 32 / PER; ++i) {
+          const int lr = wrow0 + i * PER + lane / CH, rq = min(r0 + qt * kQpRows + lr, R - 1), tq = qp_row_token(rq, p);
+          qd_copy16(qp_chunk(chunk_tile, lr, c & 15), src + (rq - tq * p.h) * p.q_sh + tq * p.q_st, true);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncwarp();
+        uint32_t amax = 0;
+#pragma unroll 4
+        for (int i = 0; i < CH; ++i) {
+          const uint4 x = qp_ld_shared16(qp_chunk(qtile + (uint32_t)(i >> 4) * kQpTile, row, i & 15));
+          float y[V16<T>::n];
+          unpack(x, y, static_cast<const T*>(p.q));
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            const int rq = min(r0 + qt * kQpRows + wrow0 + (i0 + i) * PER + sub, R - 1), tq = qp_row_token(rq, p);
-            x[i] = __ldg(reinterpret_cast<const uint4*>(src + (rq - tq * p.h) * p.q_sh + tq * p.q_st));
-          }
-        };
-        ask(0);
-#pragma unroll 1
-        for (int i0 = 0; i0 < 32 / PER; i0 += BATCH) {
-          float y[BATCH][E];
+          for (int k = 0; k < V16<T>::n; ++k) amax = max(amax, __float_as_uint(y[k]) & 0x7fffffffu);
+        }
+        const int eq = q8_row_exponent(amax);
+        const float inv = q8_exp2i(-eq) * p.qsign;
+        s_frow[qt * kQpRows + row] = p.scale * q8_exp2i(eq);
+        if constexpr (SPLIT) {
+          // 8 dimensions: two raw chunks in, one chunk of each term out. Raw chunks 2i, 2i + 1 of the first half lie where
+          // the high term's chunks 2i, 2i + 1 go, of the second half where the low term's do: read 64 dimensions of raw
+          // data ahead of the writes that take their places.
+          uint4 raw[32];
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) unpack(x[i], y[i], static_cast<const T*>(p.q));
-          if (i0 + BATCH < 32 / PER) ask(i0 + BATCH);
+          for (int i = 0; i < 32; ++i) raw[i] = qp_ld_shared16(qp_chunk(qtile + (uint32_t)(i >> 4) * kQpTile, row, i & 15));
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            uint32_t amax = 0;
+          for (int i = 0; i < 16; ++i) {
+            float y[8];
+            unpack(raw[2 * i], y, static_cast<const float*>(nullptr));
+            unpack(raw[2 * i + 1], y + 4, static_cast<const float*>(nullptr));
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int k = 0; k < E; ++k) amax = max(amax, __float_as_uint(y[i][k]) & 0x7fffffffu);
-#pragma unroll
-            for (int o = 1; o < L; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            const int eq = q8_row_exponent(amax);
-            const float inv = q8_exp2i(-eq) * p.qsign;
-            uint32_t hi[E / 2], lo[E / 2];
-#pragma unroll
-            for (int k = 0; k < E / 2; ++k) {
-              const float a = y[i][2 * k] * inv, d = y[i][2 * k + 1] * inv;
-              hi[k] = q8_pack_half2(a, d);
+            for (int k = 0; k < 4; ++k) {
+              const float u = y[2 * k] * inv, w = y[2 * k + 1] * inv;
+              hi[k] = q8_pack_half2(u, w);
               const float2 z = q8_half2_floats(hi[k]);
-              lo[k] = q8_pack_half2(a - z.x, d - z.y);
+              lo[k] = q8_pack_half2(u - z.x, w - z.y);
             }
-            const int rr = wrow0 + (i0 + i) * PER + sub;
-            if constexpr (SPLIT) {                       // 4 elements: half a 16-byte chunk
-              const uint32_t at = qp_chunk(qtile, rr, c >> 1) + (uint32_t)(c & 1) * 8u;
-              qp_st_shared8(at, hi[0], hi[1]);
-              qp_st_shared8(at + kQpTile, lo[0], lo[1]);
-            } else {
-              qp_st_shared16(qp_chunk(qtile, rr, c), hi[0], hi[1], hi[2], hi[3]);
-            }
-            if (c == 0) s_frow[qt * kQpRows + rr] = p.scale * q8_exp2i(eq);
+            qp_st_shared16(qp_chunk(qtile, row, i), hi[0], hi[1], hi[2], hi[3]);
+            qp_st_shared16(qp_chunk(qtile + kQpTile, row, i), lo[0], lo[1], lo[2], lo[3]);
+          }
+        } else {
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t at = qp_chunk(qtile, row, i);
+            float y[8];
+            unpack(qp_ld_shared16(at), y, static_cast<const __nv_bfloat16*>(nullptr));
+            qp_st_shared16(at, q8_pack_half2(y[0] * inv, y[1] * inv), q8_pack_half2(y[2] * inv, y[3] * inv),
+                           q8_pack_half2(y[4] * inv, y[5] * inv), q8_pack_half2(y[6] * inv, y[7] * inv));
           }
         }
-        __syncwarp();
         qp_fence_async();
         pf_arrive(&s_qfull[qt]);
       }
