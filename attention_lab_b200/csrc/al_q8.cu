@@ -52,7 +52,7 @@ void append_launch(int mode, unsigned grid, cudaStream_t st, const Q8AppendParam
 // The attend's kernel, and how it splits its work.
 struct Q8Plan {
   bool token;                       // the few-column kernel (mma.sync); else the prompt kernel (tcgen05)
-  int cs;                           // token: CTAs per cluster
+  int cs, chunk;                    // token: CTAs per cluster; steps per CTA of a split
   int row_tiles;                    // prompt: tiles of 256 rows
   int nsplit;                       // key splits merged through the workspace
   size_t ml_off, bytes;             // nsplit > 1: workspace layout
@@ -68,19 +68,22 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
   if (R <= kQ8TokenCols) {
     pl.token = true;
     const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
-    // One wave: clusters grow while the CTAs (two an SM) still fit at once and every warp keeps two steps. 6 x 8 segments
-    // of 4100 tokens: 4 CTAs a segment 19.4 us, 8 (more than a wave) 27.9; 8 segments of 2048: 8 CTAs 9.5 us, 16 10.5.
-    // Requests of their own lengths are split further, down to 8192 tokens a CTA, to even out the last wave: 256 segments
-    // of 16K to 32K tokens take 312 us unsplit, 281 us with 4 CTAs each (of one length 336 and 360: those stay unsplit).
+    // One wave: clusters grow while the CTAs (two an SM) still fit at once and every warp keeps two steps. 8 segments of
+    // 2048 tokens: 8 CTAs 8.6 us, 16 10.5; 6 x 8 segments of 4100 tokens: 4 CTAs 19.4 us, 6 21.6, 8 27.9.
     pl.cs = 1;
     while (pl.cs < kMaxCluster && units * pl.cs * 2 <= 2LL * sms && span >= pl.cs * 4LL * kQdWarps * kQdStep) pl.cs <<= 1;
-    if (ragged)
-      while (pl.cs < 4 && span > pl.cs * 8192LL) pl.cs <<= 1;
-    // Fewer segments than clusters of 16 can spread over the SMs: as many CTAs as fill them, merged by a second kernel.
-    const long long fill = std::min<long long>(2LL * sms / units, span / (2 * kQdWarps * kQdStep));
-    if (fill > kMaxCluster) {
+    // Splits merged by a second kernel: more CTAs a segment than clusters spread over the SMs (one request of 128K: 50 us
+    // against 92), and for requests of their own lengths runs of 4096 tokens, so that the load evens out whatever the
+    // lengths are: 256 segments of 16K to 32K tokens 272 us against 282 with clusters of 4 (runs of 2048: 290), 64 of 100
+    // to 32K 54 against 76; 64 segments that all have 32K lose, 102 against 92.
+    long long fill = std::min<long long>(2LL * sms / units, span / (2 * kQdWarps * kQdStep));
+    if (ragged) fill = std::max<long long>(fill, span / kQdChunk);
+    fill = std::min<long long>(fill, 32 * kQmWarps);
+    if (fill >= 3 && fill > pl.cs) {
+      const long long steps = span / kQdStep + 2;           // a window may straddle one step more at either end
       pl.cs = 1;
-      pl.nsplit = (int)std::min<long long>(fill, 32 * kQmWarps);
+      pl.chunk = (int)((steps + fill - 1) / fill);
+      pl.nsplit = (int)((steps + pl.chunk - 1) / pl.chunk);
     }
   } else {
     pl.row_tiles = (int)((R + 2 * kQpRows - 1) / (2 * kQpRows));
@@ -326,7 +329,7 @@ int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_
   p.window = window; p.sinks = window > 0 ? sinks : 0;
   p.scale = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
   p.qsign = scale < 0 ? -1.0f : 1.0f;
-  p.out = out; p.nsplit = pl.nsplit; p.row_tiles = pl.row_tiles; p.err = di->err;
+  p.out = out; p.nsplit = pl.nsplit; p.row_tiles = pl.row_tiles; p.chunk = pl.chunk; p.err = di->err;
   p.h_magic = h > 1 ? 0xffffffffu / (unsigned)h + 1u : 0u;   // exact for r < 2^25, h <= 64: r * (h_magic * h - 2^32) < 2^32
   if (pl.bytes > 0) {
     p.part = static_cast<float*>(workspace);

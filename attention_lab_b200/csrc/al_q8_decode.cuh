@@ -28,6 +28,7 @@ constexpr int kQdWarps = 4;
 constexpr int kQdThreads = 32 * kQdWarps;
 constexpr int kQdCols = 8;                 // columns (query, head) per CTA
 constexpr int kQdStep = 32;                // tokens per warp step (half a block: one exponent each for K and V)
+constexpr int kQdChunk = 4096;             // tokens per CTA where requests have their own lengths
 constexpr int kQdStages = 2;               // ring stages per warp
 constexpr uint32_t kQdStageBytes = 2 * kQdStep * kHeadDim;           // 8 KB: K rows, then V rows
 constexpr size_t kQdSmem = kQdWarps * kQdStages * kQdStageBytes;     // 64 KB
@@ -48,6 +49,7 @@ struct Q8AttendParams {
   void* out;                               // [B,G,h,T,128] contiguous
   // split of the key range over CTAs that write partial results (part null: none), and the prompt kernel's row tiles
   int nsplit, row_tiles;
+  int chunk;                               // token kernel with nsplit > 1: steps per CTA
   uint32_t h_magic;                        // r / h = (r * h_magic) >> 32 for the row numbers used (h > 1)
   float* part;                             // [nsplit][B*G][R][128] unnormalised O, R = T * h
   float* part_ml;                          // [nsplit][B*G][R][2]
@@ -86,7 +88,7 @@ __device__ __forceinline__ uint32_t q8_pack_half2(float lo, float hi) {
 // D += A (16x16 f16, row) * B (16x8 f16, col) with fp32 accumulate.
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                "{%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -166,13 +168,25 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   const uint8_t* vbase = p.vc + (long long)bg * p.C * kHeadDim;
   const signed char* keb = p.ke + (long long)bg * p.NB;
   const signed char* veb = p.ve + (long long)bg * p.NB;
-  const int W = cs * kQdWarps;
   const uint32_t ring = smem_addr(qd_raw) + (uint32_t)warp * (kQdStages * kQdStageBytes);
   auto step_token = [&](int s) { return (s < rg.ns ? s : rg.first + (s - rg.ns)) * kQdStep; };
   // Copy a step: 8 lanes a row, 4 rows at a time; chunk c of row r goes to place c ^ (r & 7).
   const int crow = lane >> 3, cch = lane & 7;
+  // steps of this warp: first, stride, end. A cluster's CTAs interleave; splits merged through global memory take a run of
+  // steps each, of one length whatever the request's, so that short requests leave their CTAs to others at once.
+  int step = p.part ? rank * p.chunk + warp : rank * kQdWarps + warp;
+  const int W = p.part ? kQdWarps : cs * kQdWarps;
+  const int end = p.part ? min(rg.total, (rank + 1) * p.chunk) : rg.total;
+  if (p.part && rank * p.chunk >= rg.total) {              // nothing for this split: an empty partial
+    if (tid <= col_last - col0) {
+      float* ml = p.part_ml + (((long long)rank * gridDim.y + bg) * R + col0 + tid) * 2;
+      ml[0] = -INFINITY;
+      ml[1] = 0.0f;
+    }
+    return;
+  }
   auto copy = [&](int s, int stage) {
-    if (s < rg.total) {
+    if (s < end) {
       const int j0 = step_token(s) + crow;
       const uint32_t dst = ring + (uint32_t)stage * kQdStageBytes + (uint32_t)crow * kHeadDim;
       const long long at = (long long)j0 * kHeadDim + 16 * cch;
@@ -186,11 +200,10 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
     }
     cp_async_commit();
   };
-  int step = rank * kQdWarps + warp;
 #pragma unroll
   for (int i = 0; i < kQdStages; ++i) copy(step + i * W, i);
   int ek = 0, ev = 0;
-  if (step < rg.total) {
+  if (step < end) {
     const int blk = step_token(step) / kQ8Block;
     ek = keb[blk];
     ev = veb[blk];
@@ -247,7 +260,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   const uint32_t va0 = (uint32_t)t4 * 128u + (uint32_t)((rho ^ t4) << 4), va1 = (uint32_t)(t4 + 4) * 128u + (uint32_t)((rho ^ (t4 + 4)) << 4);
   int stage = 0;
 #pragma unroll 1
-  for (; step < rg.total; step += W) {
+  for (; step < end; step += W) {
     const int j0 = step_token(step);
     cp_async_wait<kQdStages - 1>();
     __syncwarp();
@@ -267,7 +280,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
     }
     const float f = q8_factor(f_row, ek), fev = (float)ev, inv_ev = q8_exp2i(-ev);
     const int ev_now = ev;
-    if (step + W < rg.total) {
+    if (step + W < end) {
       const int blk = step_token(step + W) / kQ8Block;
       ek = keb[blk];
       ev = veb[blk];
