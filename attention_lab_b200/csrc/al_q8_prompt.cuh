@@ -132,6 +132,8 @@ __device__ __forceinline__ uint32_t qp_chunk(uint32_t tile, int r, int c) {
   return tile + (uint32_t)(c >> 3) * kQpHalf + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4);
 }
 
+template <bool B> struct QpFlag { static constexpr bool value = B; };
+
 // r / h for a query row.
 __device__ __forceinline__ int qp_row_token(int r, const Q8AttendParams& p) {
   return p.h == 1 ? r : (int)__umulhi((uint32_t)r, p.h_magic);
@@ -495,28 +497,38 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   } else if (warp < 12) {
     // ---------------------------------------------------------------------------------------------- codes -> f16 tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsConvert));
-    // A tile is converted in two halves of 64 tokens, K's then V's; two halves are in flight in registers while a third
-    // is converted. A thread takes 8 codes of each 64-wide half of a row: 8 lanes read 64 contiguous bytes, and store
+    // A tile is converted in two halves of 64 tokens, K's then V's; four halves are in flight in registers (with two the
+    // loads' latency showed: 545 us for 8192 tokens of 32/8 heads against 526). A thread takes 8 codes of each 64-wide half of a row: 8 lanes read 64 contiguous bytes, and store
     // the 8 chunks of one row of a swizzled half, each in its own banks.
     const int rw = (warp - 8) * 4 + (lane >> 3), c8 = lane & 7;     // row within a group of 16, 8-code piece
     const long long off = (long long)bg * p.C * kHeadDim + 8 * c8;
     const uint32_t at = qp_chunk(0, rw, c8);
     struct Half { uint2 a[4], b[4]; };                              // rows rw + 16 i: dimensions 8 c8 ..., 64 + 8 c8 ...
-    // half u of the walk: tile u / 4, K for u % 4 < 2, V after
+    // half u of the walk: tile u / 4, K for u % 4 < 2, V after. Rows past the length repeat the last one (their weights
+    // are zero; what matters is that they are finite, see `store`).
     auto load = [&](int u, Half& x) {
       if (u >= 4 * nt) return;
-      const int j0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1) + rw;
-      const uint8_t* src = ((u & 2) ? p.vc : p.kc) + off + (long long)j0 * kHeadDim;
+      const int t0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1), j0 = t0 + rw;
+      const uint8_t* src = ((u & 2) ? p.vc : p.kc) + off;
+      if (t0 + kQ8Block <= n) {
+        src += (long long)j0 * kHeadDim;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = j0 + 16 * i < n;
-        x.a[i] = in ? __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim)) : make_uint2(0, 0);
-        x.b[i] = in ? __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim + 64)) : make_uint2(0, 0);
+        for (int i = 0; i < 4; ++i) {
+          x.a[i] = __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim));
+          x.b[i] = __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim + 64));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* row = src + (long long)min(j0 + 16 * i, n - 1) * kHeadDim;
+          x.a[i] = __ldg(reinterpret_cast<const uint2*>(row));
+          x.b[i] = __ldg(reinterpret_cast<const uint2*>(row + 64));
+        }
       }
     };
-    // Stores a half. `nan` collects 0 * value of V (screening the codes took half again as many instructions): NaN when
-    // there is a NaN code, and then the half is read again, the codes replaced by zeros and their tokens listed.
-    auto store = [&](uint32_t dst, const Half& x, int u) {
+    // Stores a half. For V, `nan` collects 0 * value (screening the codes took half again as many instructions): NaN
+    // when there is a NaN code, and then the half is read again, the codes replaced by zeros and their tokens listed.
+    auto store = [&](uint32_t dst, const Half& x, int u, auto is_v) {
       __half2 nan = __floats2half2_rn(0.0f, 0.0f);
       const __half2 zero = nan;
 #pragma unroll
@@ -526,38 +538,49 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           const uint2 w = k ? x.b[i] : x.a[i];
           const uint32_t h[4] = {q8_decode_lo(w.x), q8_decode_hi(w.x), q8_decode_lo(w.y), q8_decode_hi(w.y)};
           qp_st_shared16(dst + at + (uint32_t)k * kQpHalf + (uint32_t)i * 2048u, h[0], h[1], h[2], h[3]);
+          if (decltype(is_v)::value) {
 #pragma unroll
-          for (int d = 0; d < 4; ++d) nan = __hfma2(*reinterpret_cast<const __half2*>(&h[d]), zero, nan);
+            for (int d = 0; d < 4; ++d) nan = __hfma2(*reinterpret_cast<const __half2*>(&h[d]), zero, nan);
+          }
         }
       const uint32_t bits = *reinterpret_cast<const uint32_t*>(&nan);
-      if (!(u & 2) || (bits & 0x7fff7fffu) == 0u) return;
+      if (!decltype(is_v)::value || (bits & 0x7fff7fffu) == 0u) return;
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
         const int j = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1) + rw + 16 * (i >> 1);
-        if (j >= n) break;
-        uint2 w = *reinterpret_cast<const uint2*>(p.vc + off + (long long)j * kHeadDim + 64 * (i & 1));
+        uint2 w = *reinterpret_cast<const uint2*>(p.vc + off + (long long)min(j, n - 1) * kHeadDim + 64 * (i & 1));
         if ((q8_nan_mask(w.x) | q8_nan_mask(w.y)) == 0u) continue;
-        const int k = atomicAdd(&s_nan_count, 1);
-        if (k < kQpNanList) s_nan[k] = j;
+        if (j < n) {
+          const int k = atomicAdd(&s_nan_count, 1);
+          if (k < kQpNanList) s_nan[k] = j;
+        }
         w = make_uint2(q8_drop_nan(w.x), q8_drop_nan(w.y));
         qp_st_shared16(dst + at + (uint32_t)(i & 1) * kQpHalf + (uint32_t)(i >> 1) * 2048u, q8_decode_lo(w.x),
                        q8_decode_hi(w.x), q8_decode_lo(w.y), q8_decode_hi(w.y));
       }
     };
-    Half xa, xb;
-    load(0, xa);
-    load(1, xb);
-#pragma unroll 1
-    for (int u = 0; u < 4 * nt; u += 2) {
-      const int it = u >> 2, st = it % NS, kv = (u >> 1) & 1;
+    Half x0, x1, x2, x3;
+    load(0, x0);
+    load(1, x1);
+    load(2, x2);
+    load(3, x3);
+    // two halves into one tile: wait for its place, convert, ask for what comes four halves later, hand over
+    auto fill = [&](Half& a, Half& c, int u, auto is_v) {
+      constexpr int kv = decltype(is_v)::value ? 1 : 0;
+      const int it = u >> 2, st = it % NS;
       const uint32_t tile = (kv ? s_v : s_k) + (uint32_t)st * kQpTile;
       qp_wait(&s_empty[kv][st], ((uint32_t)(it / NS) & 1u) ^ 1u, &s_abort, p.err);
-      store(tile, xa, u);
-      load(u + 2, xa);
-      store(tile + kQ8Block * 128u, xb, u + 1);
-      load(u + 3, xb);
+      store(tile, a, u, is_v);
+      load(u + 4, a);
+      store(tile + kQ8Block * 128u, c, u + 1, is_v);
+      load(u + 5, c);
       qp_fence_async();
       pf_arrive(&s_full[kv][st]);
+    };
+#pragma unroll 1
+    for (int u = 0; u < 4 * nt; u += 4) {
+      fill(x0, x1, u, QpFlag<false>());
+      fill(x2, x3, u + 2, QpFlag<true>());
     }
   } else {
     // ---------------------------------------------------------------------------------------------- MMAs
