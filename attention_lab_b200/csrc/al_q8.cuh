@@ -248,7 +248,10 @@ __device__ __forceinline__ void rot_heads(const RotTensor& x, int h0, int h1, in
 }
 
 // One thread: one item of one token for hpt heads (of q, then k). Bound: HBM, every row read and written once; a token's
-// table row (4 rot bytes) is read by heads / hpt threads an item, from L2 after the first.
+// table row (4 rot bytes) is read by heads / hpt threads an item, from L2 after the first. 2 x 8191 tokens of 32 + 8 fp32
+// heads, interleaved, 64 of 128 dimensions: 109 us, 6.2 TB/s (a thread a chunk and head, table read each time: 180 us);
+// 8192 tokens, bf16, half layout: 32 us, 5.4 TB/s. Half layouts whose rotated width is no multiple of 16 read partners one
+// by one: 62 us for the same tokens with 20 dimensions rotated.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   const unsigned i = blockIdx.x * 256u + threadIdx.x;
@@ -288,8 +291,10 @@ struct Q8AppendParams {
 constexpr int kQ8AppendThreads = 256;      // 8 threads a row, two chunks of 8 dimensions each; 32 rows at a time, twice
 
 // One CTA writes one block (64 tokens) of one (batch, group) of K or V: the new rows are read once into registers,
-// rotated (K), their largest finite value reduced over the CTA, then rounded and stored. Rows the block already holds
-// are touched only when the exponent grows. A thread's two chunks are a rotation pair (kRotPairs) or its own columns.
+// rotated (K), their largest finite value reduced over the CTA, then rounded and stored: the block's scale needs no pass
+// of its own, because the block is the CTA's tile. Rows the block already holds are touched only when the exponent grows.
+// A thread's two chunks are a rotation pair (kRotPairs) or its own columns. Bound: HBM (2 or 4 bytes in, 1 out per
+// element; q's rotation reads and writes as much again per head).
 template <typename T, int MODE>
 __device__ __forceinline__ void q8_append_block(const Q8AppendParams& p, int kv, int bg, int n_idx) {
   __shared__ uint32_t s_max[kQ8AppendThreads / 32];
@@ -425,7 +430,8 @@ struct Q8ReadParams {
 
 // One CTA reads one block's rows of one (batch, group) of K or V (grid: blocks, B*G, 2), so a CTA has one exponent and
 // no divisions. A thread writes 16 bytes at a time (8 bf16 or 4 fp32), so a warp's stores are contiguous; all of its
-// loads are in flight together. Bound: HBM, 1 byte in and 2 or 4 out per element.
+// loads are in flight together. Bound: HBM, 1 byte in and 2 or 4 out per element. 8 heads of 131072 tokens to bf16:
+// 122 us, 6.6 TB/s (one row a thread with 64-bit divisions: 363 us).
 template <typename T>
 __global__ void __launch_bounds__(256) q8_read_kernel(const Q8ReadParams p) {
   constexpr int E = 16 / (int)sizeof(T);             // elements per thread and row

@@ -15,8 +15,11 @@
 //
 // Bound: HBM reads of 256 bytes per visible token and group. The work of a segment is split over a cluster of CTAs
 // whose partial (m, l, O) are merged through distributed shared memory, so one launch does the whole step; with so few
-// segments that clusters of 16 leave SMs idle, over as many CTAs as fill them, whose partials go through global memory to
-// q8_merge_kernel.
+// segments that clusters of 16 leave SMs idle, or with requests of their own lengths, over runs of steps whose partials go
+// through global memory to q8_merge_kernel. 32 requests of 16K to 32K tokens, 32/8 heads: 272 us, 5.9 TB/s; 32 of 32K: 338
+// us, 6.4 TB/s; one of 128K: 50 us, 5.4 TB/s; one of 2048: 8.6 us, all latency (launch, length, rows, two steps, merge).
+// Registers fed from global memory without the ring ran the first at 417 us: two CTAs of four warps an SM held too few
+// bytes in flight.
 #pragma once
 #include <cuda_fp16.h>
 #include "al_q8.cuh"
@@ -139,8 +142,8 @@ __device__ __forceinline__ uint4 qd_lds16(uint32_t a) {
   return v;
 }
 
-// Two CTAs of four warps an SM: 297 us for 32 x 8 segments of 16K to 32K tokens; three CTAs (168 registers, spills) 366,
-// one of eight warps 302 to 321.
+// Two CTAs of four warps an SM (with clusters of two, 32 x 8 segments of 16K to 32K tokens: 296 us; three CTAs at 168
+// registers, with spills, 366; one of eight warps 302).
 template <typename T>
 __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8AttendParams p) {
   extern __shared__ __align__(1024) unsigned char qd_raw[];

@@ -15,6 +15,12 @@
 // 16-bit queries are one f16 operand (scaled by a power of two per row, exact). 32-bit queries and their weights are
 // split into two f16 terms (SPLIT): twice the MMAs, about 21 bits, single-buffered key tiles.
 //
+// Bound: shared memory and the MUFU together. A step's MMAs read their operands for 1280 cycles of an SM's shared-memory
+// bandwidth (Q again for every 64 keys), the converting warps store 32 KB (256 cycles), and its exponentials hold the MUFU
+// pipe for 1024; measured are about 1800 a step. 8192 tokens of 32/8 heads: 525 us, 1.05 PFLOP/s of causal pairs; 1024
+// tokens late in two 16K contexts with a window of 2048: 104 us (256 CTAs in two waves). Q K^T over 128 keys reads less
+// but leaves one score buffer: 614 us.
+//
 // V codes that are NaN would reach rows that do not see them (0 * NaN in the MMA): they are replaced by zero on the way
 // in, their tokens noted, and rows that do see one get their NaN in the epilogue.
 #pragma once
