@@ -34,7 +34,7 @@ int q8_shape(int B, int G, int C, int d, const void* kc, const void* vc, const v
   return AL_OK;
 }
 
-int q8_blocks(int C) { return (C + kQ8Block - 1) / kQ8Block; }
+int q8_blocks(int C) { return (C - 1) / kQ8Block + 1; }
 
 template <typename T>
 void rotary_launch(int mode, dim3 grid, cudaStream_t st, const RotaryParams& p) {
@@ -80,7 +80,7 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
     if (ragged) fill = std::max<long long>(fill, span / kQdChunk);
     fill = std::min<long long>(fill, 32 * kQmWarps);
     if (fill >= 3 && fill > pl.cs) {
-      const long long steps = span / kQdStep + 2;           // a window may straddle one step more at either end
+      const long long steps = span / kQdStep + 2;
       pl.cs = 1;
       pl.chunk = (int)((steps + fill - 1) / fill);
       pl.nsplit = (int)((steps + pl.chunk - 1) / pl.chunk);
@@ -239,7 +239,7 @@ int al_append_q8(void* k_codes, void* v_codes, void* k_exp, void* v_exp, const i
   p.sb[1] = v_sb; p.sg[1] = v_sg; p.st[1] = v_st;
   p.len.per_batch = lengths; p.len.all = length;
   p.B = B; p.G = G; p.T = T; p.C = C; p.NB = q8_blocks(C);
-  p.touched = std::min((T + kQ8Block - 2) / kQ8Block + 1, p.NB);
+  p.touched = (int)std::min<long long>(((long long)T + kQ8Block - 2) / kQ8Block + 1, p.NB);
   p.err = di->err;
   const long long kv = 2LL * B * G * p.touched;
   long long qc = 0;

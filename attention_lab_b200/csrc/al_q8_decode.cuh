@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   // steps each, of one length whatever the request's, so that short requests leave their CTAs to others at once.
   int step = p.part ? rank * p.chunk + warp : rank * kQdWarps + warp;
   const int W = p.part ? kQdWarps : cs * kQdWarps;
-  const int end = p.part ? min(rg.total, (rank + 1) * p.chunk) : rg.total;
+  // the last split takes whatever is left: the host's idea of the lengths sizes the runs, it does not bound them
+  const int end = p.part && rank + 1 < cs ? min(rg.total, (rank + 1) * p.chunk) : rg.total;
   if (p.part && rank * p.chunk >= rg.total) {              // nothing for this split: an empty partial
     if (tid <= col_last - col0) {
       float* ml = p.part_ml + (((long long)rank * gridDim.y + bg) * R + col0 + tid) * 2;

@@ -326,6 +326,22 @@ def test_attend_long_context_split(dtype, T):
         check_attend(cache, q, [L], 500, 4, al().attend_q8(q, cache, L, window=500, sinks=4))
 
 
+@pytest.mark.parametrize("h, T", [(2, 1), (1, 7), (2, 40)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (1000, 33), (1023, 1), (8000, 95)])
+def test_attend_split_covers_every_token(h, T, window, sinks):
+    """Splits by runs of tokens: windows and sinks that straddle a step more at either end, lengths far below and above
+    what the caller says (a hint that is too small must not lose tokens)."""
+    C = 20011
+    cache = random_cache(h, 2, 1, C, spread=1)
+    q = make_q(T, 2, 1, h, T, "f32")
+    for lengths in ([C, 513], [8191, 16385]):
+        on_gpu = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+        for hint in (None, C, 3000, 1):
+            out = al().attend_q8(q, cache, on_gpu, window=window, sinks=sinks, max_length=hint)
+            check_attend(cache, q, lengths, window, sinks, out)
+    assert status() == 0
+
+
 @pytest.mark.parametrize("h, T", [(4, 1), (3, 2), (4, 60)])
 def test_attend_scales(h, T):
     """Exponents far apart from block to block (a quiet block may carry all the weight), large and tiny q, negative
