@@ -65,9 +65,13 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
   int len = max_length > 0 ? std::min(max_length, C) : C;
   // tokens a query tile can see, as far as the host knows
   const long long span = window > 0 ? std::min<long long>(len, (long long)window + sinks) : len;
-  if (R <= kQ8TokenCols) {
+  // The few-column kernel reads the cache once per 8 query rows, the prompt kernel once per 256 but fills 128 x 128 tiles
+  // and takes 11 us for the least work. Up to 16 rows the first wins throughout (16 heads over 32 x 8192 tokens: 180 us
+  // against 212); up to 128 while everything it reads is small (one request, 8 groups: 64 rows over 512 tokens 9.0 us
+  // against 15.0, over 4096 tokens 18.1 against 18.8; 32 rows over 32 x 8192 tokens 326 against 216).
+  const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
+  if (R <= kQ8TokenCols || (R <= kQ8FewCols && units * span <= kQ8FewTokens)) {
     pl.token = true;
-    const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
     // One wave: clusters grow while the CTAs (two an SM) still fit at once and every warp keeps two steps. 8 segments of
     // 2048 tokens: 8 CTAs 8.6 us, 16 10.5; 6 x 8 segments of 4100 tokens: 4 CTAs 19.4 us, 6 21.6, 8 27.9.
     pl.cs = 1;

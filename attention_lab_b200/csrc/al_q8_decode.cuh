@@ -1,4 +1,4 @@
-// Attention of a few query columns (a decode step: T * h columns per KV group, T usually 1) over the 8-bit cache, with
+// Attention of a few query columns (a decode step, or a short chunk: T * h columns per KV group) over the 8-bit cache, with
 // an optional sliding window and first tokens (sinks) that stay visible.
 //
 // A query at position p sees the tokens j <= p with window = 0, or j > p - window, or j < sinks. A CTA holds 8 columns
@@ -26,7 +26,9 @@
 
 namespace al {
 
-constexpr int kQ8TokenCols = 16;          // up to this many columns per group take this kernel, more the prompt kernel
+constexpr int kQ8TokenCols = 16;           // up to this many query rows per group always take this kernel
+constexpr int kQ8FewCols = 128;            // up to this many do while (segments x groups of 8 rows x tokens) is at most
+constexpr long long kQ8FewTokens = 1 << 17;   // this; the rest take the prompt kernel
 constexpr int kQdWarps = 4;
 constexpr int kQdThreads = 32 * kQdWarps;
 constexpr int kQdCols = 8;                 // columns (query, head) per CTA

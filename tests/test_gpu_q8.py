@@ -284,7 +284,7 @@ def make_q(seed, B, G, h, T, dtype):
 
 
 SHAPES = [(1, 1), (4, 1), (8, 1), (3, 2), (9, 1), (16, 1), (5, 3),       # few columns
-          (17, 1), (1, 40), (4, 70), (3, 130)]                             # prompts
+          (17, 1), (1, 40), (4, 70), (3, 130), (1, 150), (17, 9), (64, 3)]  # short chunks, prompts
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -312,7 +312,7 @@ def test_attend_window_and_sinks(dtype, h, T, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("T", [1, 30])
+@pytest.mark.parametrize("T", [1, 30, 90])
 def test_attend_long_context_split(dtype, T):
     """One request: the key range is split over CTAs and merged."""
     n = 9000
@@ -406,7 +406,7 @@ def test_attend_many_nan_rows():
     assert torch.equal(got[..., keep], base[..., keep])
 
 
-@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("T", [1, 20, 80])
 def test_attend_past_32_bit_offsets(T):
     """A cache of more than 2^32 bytes: the last tokens of the last head."""
     C = (1 << 25) // 2 + 333
