@@ -17,8 +17,8 @@
 //
 // Bound: shared memory and the MUFU together. A step's MMAs read their operands for 1280 cycles of an SM's shared-memory
 // bandwidth (Q again for every 64 keys), the converting warps store 32 KB (256 cycles), and its exponentials hold the MUFU
-// pipe for 1024; measured are about 1800 a step. 8192 tokens of 32/8 heads: 525 us, 1.05 PFLOP/s of causal pairs; 1024
-// tokens late in two 16K contexts with a window of 2048: 104 us (256 CTAs in two waves). Q K^T over 128 keys reads less
+// pipe for 1024; measured are about 1800 a step. 8192 tokens of 32/8 heads: 522 us, 1.05 PFLOP/s of causal pairs; 1024
+// tokens late in two 16K contexts with a window of 2048: 103 us (256 CTAs in two waves). Q K^T over 128 keys reads less
 // but leaves one score buffer: 614 us.
 //
 // V codes that are NaN would reach rows that do not see them (0 * NaN in the MMA): they are replaced by zero on the way
@@ -222,25 +222,36 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       {
         constexpr int CH = kHeadDim * (int)sizeof(T) / 16, PER = 32 / CH;   // 16-byte chunks a row, rows at a time
         const int c = lane % CH;
-        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + V16<T>::n * c;
         const uint32_t chunk_tile = qtile + (uint32_t)(c >> 4) * kQpTile;
+        // rows PER apart: PER / h tokens and PER % h heads further, one token more where the head wraps
+        const int lr0 = wrow0 + lane / CH, left = R - (r0 + qt * kQpRows + lr0);   // rows from this one on
+        const int t0 = qp_row_token(r0 + qt * kQpRows + lr0, p), dt = PER / p.h, dh = PER - dt * p.h;
+        int head = r0 + qt * kQpRows + lr0 - t0 * p.h;
+        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t0 * p.q_st + V16<T>::n * c;
+        const long long hop = dt * p.q_st + dh * p.q_sh, wrap = p.q_st - p.h * p.q_sh;
 #pragma unroll 4
         for (int i = 0; i < 32 / PER; ++i) {
-          const int lr = wrow0 + i * PER + lane / CH, rq = min(r0 + qt * kQpRows + lr, R - 1), tq = qp_row_token(rq, p);
-          qd_copy16(qp_chunk(chunk_tile, lr, c & 15), src + (rq - tq * p.h) * p.q_sh + tq * p.q_st, true);
+          const bool in = i * PER < left;                // rows past the last are zeros and are not stored
+          qd_copy16(qp_chunk(chunk_tile, lr0 + i * PER, c & 15), in ? src : static_cast<const T*>(p.q), in);
+          src += hop;
+          head += dh;
+          if (head >= p.h) { head -= p.h; src += wrap; }
         }
         cp_async_commit();
         cp_async_wait<0>();
         __syncwarp();
-        uint32_t amax = 0;
+        uint32_t amax = 0;                               // of the bits without the sign: fp32's, or two bf16's
 #pragma unroll 4
         for (int i = 0; i < CH; ++i) {
           const uint4 x = qp_ld_shared16(qp_chunk(qtile + (uint32_t)(i >> 4) * kQpTile, row, i & 15));
-          float y[V16<T>::n];
-          unpack(x, y, static_cast<const T*>(p.q));
-#pragma unroll
-          for (int k = 0; k < V16<T>::n; ++k) amax = max(amax, __float_as_uint(y[k]) & 0x7fffffffu);
+          if constexpr (SPLIT) {
+            amax = max(amax, max(max(x.x & 0x7fffffffu, x.y & 0x7fffffffu), max(x.z & 0x7fffffffu, x.w & 0x7fffffffu)));
+          } else {
+            amax = __vmaxu2(amax, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                           __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+          }
         }
+        if constexpr (!SPLIT) amax = max(amax << 16, amax & 0xffff0000u);
         const int eq = q8_row_exponent(amax);
         const float inv = q8_exp2i(-eq) * p.qsign;
         s_frow[qt * kQpRows + row] = p.scale * q8_exp2i(eq);
@@ -461,20 +472,23 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           }
         }
         if (c == 3 || (wide && (c & 1))) {
-          // 16 lanes a row, 2 rows at a time
+          // 16 lanes a row, 2 rows at a time; row r of a group is token r / h, head r % h (partial results keep r)
           __syncwarp();
+          const int lr0 = wrow0 + (lane >> 4), ro0 = r0 + qt * kQpRows + lr0, to = qp_row_token(ro0, p);
+          int ho = ro0 - to * p.h;
+          const int dt = 2 / p.h, dh = 2 - dt * p.h;
+          const long long row_bytes = kHeadDim * (part ? 4 : (int)sizeof(T));
+          char* dst = part ? reinterpret_cast<char*>(p.part + (((long long)split * BG + bg) * R + ro0) * kHeadDim)
+                           : reinterpret_cast<char*>(static_cast<T*>(p.out) + (((long long)bg * p.h + ho) * p.T + to) * kHeadDim);
+          dst += (wide ? 128 * (c - 1) : 0) + 16 * (lane & 15);
+          const long long hop = part ? 2 * row_bytes : (dh * (long long)p.T + dt) * row_bytes;
+          const long long wrap = part ? 0 : (1 - p.h * (long long)p.T) * row_bytes;
 #pragma unroll 4
           for (int i = 0; i < 16; ++i) {
-            const int lr = wrow0 + 2 * i + (lane >> 4), ro = r0 + qt * kQpRows + lr, ch = lane & 15;
-            if (ro < R) {
-              const uint4 x = qp_ld_shared16(qp_chunk(qtile, lr, ch));
-              const int to = qp_row_token(ro, p), ho = ro - to * p.h;
-              char* dst;
-              if (part) dst = reinterpret_cast<char*>(p.part + (((long long)split * BG + bg) * R + ro) * kHeadDim + 32 * (c - 1));
-              else dst = reinterpret_cast<char*>(static_cast<T*>(p.out) + (((long long)bg * p.h + ho) * p.T + to) * kHeadDim +
-                                                 (wide ? 32 * (c - 1) : 0));
-              *reinterpret_cast<uint4*>(dst + 16 * ch) = x;
-            }
+            if (ro0 + 2 * i < R) *reinterpret_cast<uint4*>(dst) = qp_ld_shared16(qp_chunk(qtile, lr0 + 2 * i, lane & 15));
+            dst += hop;
+            ho += dh;
+            if (ho >= p.h) { ho -= p.h; dst += wrap; }
           }
           __syncwarp();
         }
