@@ -17,8 +17,8 @@
 //
 // Bound: shared memory and the MUFU together. A step's MMAs read their operands for 1280 cycles of an SM's shared-memory
 // bandwidth (Q again for every 64 keys), the converting warps store 32 KB (256 cycles), and its exponentials hold the MUFU
-// pipe for 1024; measured are about 1800 a step. 8192 tokens of 32/8 heads: 522 us, 1.05 PFLOP/s of causal pairs; 1024
-// tokens late in two 16K contexts with a window of 2048: 103 us (256 CTAs in two waves). Q K^T over 128 keys reads less
+// pipe for 1024; measured are about 1800 a step. 8192 tokens of 32/8 heads: 516 us, 1.07 PFLOP/s of causal pairs; 1024
+// tokens late in two 16K contexts with a window of 2048: 101 us (256 CTAs in two waves). Q K^T over 128 keys reads less
 // but leaves one score buffer: 614 us.
 //
 // V codes that are NaN would reach rows that do not see them (0 * NaN in the MMA): they are replaced by zero on the way
@@ -34,7 +34,10 @@ constexpr int kQpKeys = 128;                           // tokens per key tile: t
 constexpr int kQpThreads = 512;
 constexpr uint32_t kQpTile = kQpKeys * kHeadDim * 2;   // 32 KB: a tile of 128 x 128 f16, two 64-wide halves of 16 KB
 constexpr uint32_t kQpHalf = kQpTile / 2;
-constexpr size_t kQpSmem = 1024 + 6 * kQpTile;         // 2 Q + 2 K + 2 V tiles, or 4 Q (high, low) + K + V
+constexpr int kQpPitch = 256 + 16;                     // output rows on their way out, 256 bytes at a time: no bank twice
+constexpr uint32_t kQpStage = kQpRows * kQpPitch;      // 34 KB
+static_assert(kQpStage % 1024 == 0, "tiles start on 1 KB");
+constexpr size_t kQpSmem = 1024 + 4 * kQpTile + 2 * kQpStage;   // 2 Q + 2 K + 2 V tiles; 4 Q (high, low) + K + V are less
 constexpr int kQpNanList = 64;
 constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8)
 // Registers a thread after the split: 2 x 128 softmax threads, 128 converting threads, the MMA warp's group.
@@ -113,6 +116,13 @@ __device__ __forceinline__ void qp_tmem_ld64(uint32_t taddr, uint32_t (&v)[64]) 
 #pragma unroll
   for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));
 }
+// Asynchronous copy of `bytes` (a multiple of 16) from shared to global memory, both on 16-byte boundaries, and the wait
+// until the sources of this thread's copies are read.
+__device__ __forceinline__ void qp_bulk_store(const void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n cp.async.bulk.commit_group;\n"
+               ::"l"(__cvta_generic_to_global(dst)), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void qp_bulk_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
 // Named barriers of a pair of warps: one waits, the other only arrives.
 __device__ __forceinline__ void qp_bar_sync(int id) { asm volatile("bar.sync %0, 64;\n" ::"r"(id) : "memory"); }
 __device__ __forceinline__ void qp_bar_arrive(int id) { asm volatile("bar.arrive %0, 64;\n" ::"r"(id) : "memory"); }
@@ -127,6 +137,9 @@ __device__ __forceinline__ float qp_max3(float a, float b, float c) {
 __device__ __forceinline__ void qp_st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ void qp_st_shared8(uint32_t a, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ uint4 qp_ld_shared16(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -139,6 +152,7 @@ __device__ __forceinline__ uint32_t qp_chunk(uint32_t tile, int r, int c) {
 }
 
 template <bool B> struct QpFlag { static constexpr bool value = B; };
+template <int I> struct QpInt { static constexpr int value = I; };
 
 // r / h for a query row.
 __device__ __forceinline__ int qp_row_token(int r, const Q8AttendParams& p) {
@@ -150,6 +164,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
   constexpr int QP = SPLIT ? 2 : 1;                    // f16 terms per query row
+  constexpr uint32_t QS = SPLIT ? 2 * kQpTile : kQpStage;   // bytes of a query tile, later of its output rows
   extern __shared__ __align__(1024) unsigned char qp_raw[];
   __shared__ uint64_t s_qfull[2], s_full[2][NS], s_empty[2][NS], s_sfull[2][2], s_pfull[2][2], s_pv[2][2];
   __shared__ uint32_t s_taddr;
@@ -161,30 +176,17 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   // descriptors and branches in the uniform datapath (otherwise every MMA takes some 45 instructions).
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t base = (smem_addr(qp_raw) + 1023u) & ~1023u;
-  const uint32_t s_q = base, s_k = base + 2 * QP * kQpTile, s_v = s_k + NS * kQpTile;
+  const uint32_t s_q = base, s_k = base + 2 * QS, s_v = s_k + NS * kQpTile;
 
   // the longest row tiles first; all (batch, group) pairs of a row tile together
   const int BG = p.B * p.G, R = p.h * p.T;
   const int split = blockIdx.y;
   const int tile = p.row_tiles - 1 - (int)(blockIdx.x / (unsigned)BG), bg = (int)(blockIdx.x % (unsigned)BG);
   const int b = (int)((unsigned)bg / (unsigned)p.G), g = bg - b * p.G;
-  int n = __shfl_sync(0xffffffffu, q8_length(p.len, b), 0);
-  if (n < 0 || n > p.C) {
-    if (tid == 0) atomicOr(p.err, kErrQ8Range);
-    n = max(0, min(n, p.C));
-  }
+  const int length = q8_length(p.len, b);               // used after the set-up, which hides its latency
   const int r0 = tile * 2 * kQpRows;
   const int ntile = r0 + kQpRows < R ? 2 : 1;
-  const int pbase = n - p.T;
-  const int plo = pbase + qp_row_token(r0, p), phi = pbase + qp_row_token(min(r0 + 2 * kQpRows - 1, R - 1), p);
-  const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQpKeys);
-  // (total < 2^24 and nsplit <= 148: the products fit 32 bits)
-  const int it0 = (int)((unsigned)rg.total * (unsigned)split / (unsigned)p.nsplit);
-  const int it1 = (int)((unsigned)rg.total * (unsigned)(split + 1) / (unsigned)p.nsplit);
-  const int nt = it1 - it0;
-  auto tile_token = [&](int it) { return (it < rg.ns ? it : rg.first + (it - rg.ns)) * kQpKeys; };
-
-  if (tid == 0) {
+  if (tid == 13 * 32) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_qfull[i], kQpRows);
       for (int k = 0; k < 2; ++k) {
@@ -201,96 +203,142 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     s_abort = 0;
   }
   if (warp == 12) { tmem_alloc(&s_taddr, 512); tmem_relinquish(); }
+
+  // Query rows of warps 0-7, 16 pieces of 16 bytes a lane: LPR lanes a row, PER rows at a time. Asked for first, so
+  // that they arrive while barriers and TMEM are set up.
+  constexpr int LPR = kHeadDim * (int)sizeof(T) / 16, PER = 32 / LPR;
+  const int qt = (warp >> 2) & 1, wrow0 = (warp & 3) * 32;   // warps 0-7: the query tile and the warp's first row in it
+  uint4 raw[16];                                       // of these warps and of the converting ones
+  auto load_rows = [&](int round) {
+    const int rq = r0 + qt * kQpRows + wrow0 + 16 * PER * round + lane / LPR, left = R - rq;   // rows from this one on
+    // rows PER apart: PER / h tokens and PER % h heads further, one token more where the head wraps
+    const int t0 = qp_row_token(rq, p), dt = p.h == 1 ? PER : p.h == PER ? 1 : 0, dh = PER - dt * p.h;
+    int head = rq - t0 * p.h;
+    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t0 * p.q_st + V16<T>::n * (lane % LPR);
+    const long long hop = dt * p.q_st + dh * p.q_sh, wrap = p.q_st - p.h * p.q_sh;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);               // rows past the last are zeros and are not stored
+      if (i * PER < left) raw[i] = __ldg(reinterpret_cast<const uint4*>(src));
+      src += hop;
+      head += dh;
+      if (head >= p.h) { head -= p.h; src += wrap; }
+    }
+  };
+  if (warp < 8 && qt < ntile) load_rows(0);
   tmem_fence_before_sync();
   __syncthreads();
   tmem_fence_after_sync();
-  const uint32_t tm = __shfl_sync(0xffffffffu, s_taddr, 0);                          // S0 | S1 | O0 | O1, 128 columns each
+  const uint32_t tm = __shfl_sync(0xffffffffu, s_taddr, 0);   // S0 | S1 | O0 | O1, 128 columns each
+
+  int n = __shfl_sync(0xffffffffu, length, 0);
+  if (n < 0 || n > p.C) {
+    if (tid == 0) atomicOr(p.err, kErrQ8Range);
+    n = max(0, min(n, p.C));
+  }
+  const int pbase = n - p.T;
+  const int plo = pbase + qp_row_token(r0, p), phi = pbase + qp_row_token(min(r0 + 2 * kQpRows - 1, R - 1), p);
+  const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQpKeys);
+  // (total < 2^24 and nsplit <= 148: the products fit 32 bits)
+  const int it0 = (int)((unsigned)rg.total * (unsigned)split / (unsigned)p.nsplit);
+  const int it1 = (int)((unsigned)rg.total * (unsigned)(split + 1) / (unsigned)p.nsplit);
+  const int nt = it1 - it0;
+  auto tile_token = [&](int it) { return (it < rg.ns ? it : rg.first + (it - rg.ns)) * kQpKeys; };
+
+  // Converting warps: a tile is converted in two halves of 64 tokens, K's then V's; four halves are in flight in
+  // registers (with two the loads' latency showed: 545 us for 8192 tokens of 32/8 heads against 526). A thread takes 8
+  // codes of each 64-wide half of a row: 8 lanes read 64 contiguous bytes, and store the 8 chunks of one row of a swizzled
+  // half, each in its own banks.
+  const int rw = (warp & 3) * 4 + (lane >> 3), c8 = lane & 7;   // row within a group of 16, 8-code piece
+  const long long off = (long long)bg * p.C * kHeadDim + 8 * c8;
+  // half u of the walk: tile u / 4, K for u % 4 < 2, V after; into pieces 4 slot ...: rows rw + 16 i, dimensions 8 c8 ...
+  // and 64 + 8 c8 ... . Rows past the length repeat the last one (their weights are zero; what matters is that they are
+  // finite, see `store`).
+  auto load = [&](int u, auto slot) {
+    constexpr int at = 4 * decltype(slot)::value;
+    if (u >= 4 * nt) return;
+    const int t0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1), j0 = t0 + rw;
+    const uint8_t* src = ((u & 2) ? p.vc : p.kc) + off;
+    auto piece = [&](int i, const uint8_t* row) {
+      const uint2 a = __ldg(reinterpret_cast<const uint2*>(row)), c = __ldg(reinterpret_cast<const uint2*>(row + 64));
+      raw[at + i] = make_uint4(a.x, a.y, c.x, c.y);
+    };
+    if (t0 + kQ8Block <= n) {
+      src += (long long)j0 * kHeadDim;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) piece(i, src + 16 * i * kHeadDim);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) piece(i, src + (long long)min(j0 + 16 * i, n - 1) * kHeadDim);
+    }
+  };
 
   if (warp < 8) {
     // ---------------------------------------------------------------------------------------------- query rows
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kQpRegsSoftmax));
-    const int qt = warp >> 2, row = tid & 127;
+    const int row = tid & 127;
     if (qt < ntile && nt > 0) {
       const int r = min(r0 + qt * kQpRows + row, R - 1);
       const int pos = pbase + qp_row_token(r, p);
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t tS = tm + lanes + (uint32_t)qt * 128u, tO = tm + lanes + 256u + (uint32_t)qt * 128u;
-      const int wrow0 = (warp & 3) * 32;               // the warp's first row of the tile
-      const uint32_t qtile = s_q + (uint32_t)(qt * QP) * kQpTile;
-      // The warp's 32 query rows come straight into their places in the query tile (full lines, all copies in flight;
-      // 32-bit rows fill the places of both terms), then every thread scales its row by a power of two and splits it.
-      {
-        constexpr int CH = kHeadDim * (int)sizeof(T) / 16, PER = 32 / CH;   // 16-byte chunks a row, rows at a time
-        const int c = lane % CH;
-        const uint32_t chunk_tile = qtile + (uint32_t)(c >> 4) * kQpTile;
-        // rows PER apart: PER / h tokens and PER % h heads further, one token more where the head wraps
-        const int lr0 = wrow0 + lane / CH, left = R - (r0 + qt * kQpRows + lr0);   // rows from this one on
-        const int t0 = qp_row_token(r0 + qt * kQpRows + lr0, p), dt = PER / p.h, dh = PER - dt * p.h;
-        int head = r0 + qt * kQpRows + lr0 - t0 * p.h;
-        const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t0 * p.q_st + V16<T>::n * c;
-        const long long hop = dt * p.q_st + dh * p.q_sh, wrap = p.q_st - p.h * p.q_sh;
-#pragma unroll 4
-        for (int i = 0; i < 32 / PER; ++i) {
-          const bool in = i * PER < left;                // rows past the last are zeros and are not stored
-          qd_copy16(qp_chunk(chunk_tile, lr0 + i * PER, c & 15), in ? src : static_cast<const T*>(p.q), in);
-          src += hop;
-          head += dh;
-          if (head >= p.h) { head -= p.h; src += wrap; }
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        __syncwarp();
-        uint32_t amax = 0;                               // of the bits without the sign: fp32's, or two bf16's
-#pragma unroll 4
-        for (int i = 0; i < CH; ++i) {
-          const uint4 x = qp_ld_shared16(qp_chunk(qtile + (uint32_t)(i >> 4) * kQpTile, row, i & 15));
+      const uint32_t qtile = s_q + (uint32_t)qt * QS;
+      // Every row is scaled by a power of two into f16 (32-bit rows: two f16 terms) and goes to its places in the query
+      // tile. Row maxima: each lane's over its pieces, then a transposing reduction that leaves piece i's row to lane i.
+#pragma unroll 1
+      for (int round = 0; round < 2 / PER; ++round) {
+        if (round > 0) load_rows(round);
+        uint32_t amax[16];                               // of the bits without the sign
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint4 x = raw[i];
           if constexpr (SPLIT) {
-            amax = max(amax, max(max(x.x & 0x7fffffffu, x.y & 0x7fffffffu), max(x.z & 0x7fffffffu, x.w & 0x7fffffffu)));
+            amax[i] = max(max(x.x & 0x7fffffffu, x.y & 0x7fffffffu), max(x.z & 0x7fffffffu, x.w & 0x7fffffffu));
           } else {
-            amax = __vmaxu2(amax, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                           __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+            const uint32_t y = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                        __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+            amax[i] = max(y << 16, y & 0xffff0000u);
           }
         }
-        if constexpr (!SPLIT) amax = max(amax << 16, amax & 0xffff0000u);
-        const int eq = q8_row_exponent(amax);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+          for (int i = 0; i < o; ++i) {
+            const bool up = (lane & o) != 0;
+            const uint32_t send = up ? amax[i] : amax[i + o], keep = up ? amax[i + o] : amax[i];
+            amax[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, o));
+          }
+        if constexpr (SPLIT) amax[0] = max(amax[0], __shfl_xor_sync(0xffffffffu, amax[0], 16));
+        const int eq = q8_row_exponent(amax[0]);
         const float inv = q8_exp2i(-eq) * p.qsign;
-        s_frow[qt * kQpRows + row] = p.scale * q8_exp2i(eq);
-        if constexpr (SPLIT) {
-          // 8 dimensions: two raw chunks in, one chunk of each term out. Raw chunks 2i, 2i + 1 of the first half lie where
-          // the high term's chunks 2i, 2i + 1 go, of the second half where the low term's do: read 64 dimensions of raw
-          // data ahead of the writes that take their places.
-          uint4 raw[32];
+        const int lr = wrow0 + 16 * PER * round + lane / LPR;   // row of piece 0
+        s_frow[qt * kQpRows + lr + (lane & 15) * PER] = p.scale * q8_exp2i(eq);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) raw[i] = qp_ld_shared16(qp_chunk(qtile + (uint32_t)(i >> 4) * kQpTile, row, i & 15));
+        for (int i = 0; i < 16; ++i) {
+          const float z = __shfl_sync(0xffffffffu, inv, i, 16);
+          float y[V16<T>::n];
+          unpack(raw[i], y, static_cast<const T*>(nullptr));
+          if constexpr (SPLIT) {
+            uint32_t hi[2], lo[2];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float y[8];
-            unpack(raw[2 * i], y, static_cast<const float*>(nullptr));
-            unpack(raw[2 * i + 1], y + 4, static_cast<const float*>(nullptr));
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float u = y[2 * k] * inv, w = y[2 * k + 1] * inv;
+            for (int k = 0; k < 2; ++k) {
+              const float u = y[2 * k] * z, w = y[2 * k + 1] * z;
               hi[k] = q8_pack_half2(u, w);
-              const float2 z = q8_half2_floats(hi[k]);
-              lo[k] = q8_pack_half2(u - z.x, w - z.y);
+              const float2 x = q8_half2_floats(hi[k]);
+              lo[k] = q8_pack_half2(u - x.x, w - x.y);
             }
-            qp_st_shared16(qp_chunk(qtile, row, i), hi[0], hi[1], hi[2], hi[3]);
-            qp_st_shared16(qp_chunk(qtile + kQpTile, row, i), lo[0], lo[1], lo[2], lo[3]);
-          }
-        } else {
-#pragma unroll 4
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t at = qp_chunk(qtile, row, i);
-            float y[8];
-            unpack(qp_ld_shared16(at), y, static_cast<const __nv_bfloat16*>(nullptr));
-            qp_st_shared16(at, q8_pack_half2(y[0] * inv, y[1] * inv), q8_pack_half2(y[2] * inv, y[3] * inv),
-                           q8_pack_half2(y[4] * inv, y[5] * inv), q8_pack_half2(y[6] * inv, y[7] * inv));
+            const uint32_t at = qp_chunk(qtile, lr + i, lane >> 1) + 8u * (uint32_t)(lane & 1);
+            qp_st_shared8(at, hi[0], hi[1]);
+            qp_st_shared8(at + kQpTile, lo[0], lo[1]);
+          } else {
+            qp_st_shared16(qp_chunk(qtile, lr + 2 * i, lane & 15), q8_pack_half2(y[0] * z, y[1] * z),
+                           q8_pack_half2(y[2] * z, y[3] * z), q8_pack_half2(y[4] * z, y[5] * z), q8_pack_half2(y[6] * z, y[7] * z));
           }
         }
-        qp_fence_async();
-        pf_arrive(&s_qfull[qt]);
       }
+      qp_fence_async();
+      pf_arrive(&s_qfull[qt]);
+      __syncwarp();
       const float f_row = s_frow[qt * kQpRows + row];
       // positions of the warp's rows, for the test that a step needs no mask
       const int rw0 = r0 + qt * kQpRows + wrow0;
@@ -423,14 +471,18 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       qp_wait(&s_pv[qt][1], (uint32_t)(nt - 1) & 1u, &s_abort, p.err);
       tmem_fence_after_sync();
       __syncwarp();
-      // O through shared memory (the query tile's, now free) so that rows go out as full lines, 256 bytes of
-      // each of the warp's 32 rows at a time
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      // O through shared memory (the query tile's, now free): every thread puts its row there and hands it to the copy
+      // engine, 256 bytes at a time (a CTA's epilogue takes 3900 cycles; with 16 lanes storing a row 4400)
       const int bad = s_nan_count;
       const uint8_t* vbase = p.vc + (long long)bg * p.C * kHeadDim;
       const bool part = p.part != nullptr;
       const bool wide = part || SPLIT;                   // 32-bit rows: 64 dimensions at a time
       const int rr = r0 + qt * kQpRows + row;
+      const float z = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+      const uint32_t stage = qtile + (uint32_t)(row * kQpPitch);
+      const int head = r - (pos - pbase) * p.h;          // row r of a group is token r / h, head r % h; partial results keep r
+      char* dst = part ? reinterpret_cast<char*>(p.part + (((long long)split * BG + bg) * R + r) * kHeadDim)
+                       : reinterpret_cast<char*>(static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + (pos - pbase)) * kHeadDim);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -453,14 +505,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           }
           __syncwarp();
         }
-        if (!part) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
-        }
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * z);
         if (wide) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            qp_st_shared16(qp_chunk(qtile, row, 8 * (c & 1) + i), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            qp_st_shared16(stage + 128u * (uint32_t)(c & 1) + 16u * (uint32_t)i, o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -468,29 +518,13 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               h4[k] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]), __uint_as_float(o[8 * i + 2 * k + 1]));
-            qp_st_shared16(qp_chunk(qtile, row, 4 * c + i), h4[0], h4[1], h4[2], h4[3]);
+            qp_st_shared16(stage + 64u * (uint32_t)c + 16u * (uint32_t)i, h4[0], h4[1], h4[2], h4[3]);
           }
         }
         if (c == 3 || (wide && (c & 1))) {
-          // 16 lanes a row, 2 rows at a time; row r of a group is token r / h, head r % h (partial results keep r)
-          __syncwarp();
-          const int lr0 = wrow0 + (lane >> 4), ro0 = r0 + qt * kQpRows + lr0, to = qp_row_token(ro0, p);
-          int ho = ro0 - to * p.h;
-          const int dt = 2 / p.h, dh = 2 - dt * p.h;
-          const long long row_bytes = kHeadDim * (part ? 4 : (int)sizeof(T));
-          char* dst = part ? reinterpret_cast<char*>(p.part + (((long long)split * BG + bg) * R + ro0) * kHeadDim)
-                           : reinterpret_cast<char*>(static_cast<T*>(p.out) + (((long long)bg * p.h + ho) * p.T + to) * kHeadDim);
-          dst += (wide ? 128 * (c - 1) : 0) + 16 * (lane & 15);
-          const long long hop = part ? 2 * row_bytes : (dh * (long long)p.T + dt) * row_bytes;
-          const long long wrap = part ? 0 : (1 - p.h * (long long)p.T) * row_bytes;
-#pragma unroll 4
-          for (int i = 0; i < 16; ++i) {
-            if (ro0 + 2 * i < R) *reinterpret_cast<uint4*>(dst) = qp_ld_shared16(qp_chunk(qtile, lr0 + 2 * i, lane & 15));
-            dst += hop;
-            ho += dh;
-            if (ho >= p.h) { ho -= p.h; dst += wrap; }
-          }
-          __syncwarp();
+          qp_fence_async();
+          if (rr < R) qp_bulk_store(dst + (wide ? 128 * (c - 1) : 0), stage, 256u);
+          qp_bulk_read_wait();                           // the place is used again, or the CTA ends
         }
       }
       if (part && rr < R) {
@@ -517,45 +551,22 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   } else if (warp < 12) {
     // ---------------------------------------------------------------------------------------------- codes -> f16 tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kQpRegsConvert));
-    // A tile is converted in two halves of 64 tokens, K's then V's; four halves are in flight in registers (with two the
-    // loads' latency showed: 545 us for 8192 tokens of 32/8 heads against 526). A thread takes 8 codes of each 64-wide half of a row: 8 lanes read 64 contiguous bytes, and store
-    // the 8 chunks of one row of a swizzled half, each in its own banks.
-    const int rw = (warp - 8) * 4 + (lane >> 3), c8 = lane & 7;     // row within a group of 16, 8-code piece
-    const long long off = (long long)bg * p.C * kHeadDim + 8 * c8;
-    const uint32_t at = qp_chunk(0, rw, c8);
-    struct Half { uint2 a[4], b[4]; };                              // rows rw + 16 i: dimensions 8 c8 ..., 64 + 8 c8 ...
-    // half u of the walk: tile u / 4, K for u % 4 < 2, V after. Rows past the length repeat the last one (their weights
-    // are zero; what matters is that they are finite, see `store`).
-    auto load = [&](int u, Half& x) {
-      if (u >= 4 * nt) return;
-      const int t0 = tile_token(it0 + (u >> 2)) + kQ8Block * (u & 1), j0 = t0 + rw;
-      const uint8_t* src = ((u & 2) ? p.vc : p.kc) + off;
-      if (t0 + kQ8Block <= n) {
-        src += (long long)j0 * kHeadDim;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x.a[i] = __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim));
-          x.b[i] = __ldg(reinterpret_cast<const uint2*>(src + 16 * i * kHeadDim + 64));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t* row = src + (long long)min(j0 + 16 * i, n - 1) * kHeadDim;
-          x.a[i] = __ldg(reinterpret_cast<const uint2*>(row));
-          x.b[i] = __ldg(reinterpret_cast<const uint2*>(row + 64));
-        }
-      }
-    };
     // Stores a half. For V, `nan` collects 0 * value (screening the codes took half again as many instructions): NaN
     // when there is a NaN code, and then the half is read again, the codes replaced by zeros and their tokens listed.
-    auto store = [&](uint32_t dst, const Half& x, int u, auto is_v) {
+    load(0, QpInt<0>());
+    load(1, QpInt<1>());
+    load(2, QpInt<2>());
+    load(3, QpInt<3>());
+    const uint32_t at = qp_chunk(0, rw, c8);
+    auto store = [&](uint32_t dst, auto slot, int u, auto is_v) {
       __half2 nan = __floats2half2_rn(0.0f, 0.0f);
       const __half2 zero = nan;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint2 w = k ? x.b[i] : x.a[i];
+          const uint4 x = raw[4 * decltype(slot)::value + i];
+          const uint2 w = k ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y);
           const uint32_t h[4] = {q8_decode_lo(w.x), q8_decode_hi(w.x), q8_decode_lo(w.y), q8_decode_hi(w.y)};
           qp_st_shared16(dst + at + (uint32_t)k * kQpHalf + (uint32_t)i * 2048u, h[0], h[1], h[2], h[3]);
           if (decltype(is_v)::value) {
@@ -579,28 +590,25 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
                        q8_decode_hi(w.x), q8_decode_lo(w.y), q8_decode_hi(w.y));
       }
     };
-    Half x0, x1, x2, x3;
-    load(0, x0);
-    load(1, x1);
-    load(2, x2);
-    load(3, x3);
     // two halves into one tile: wait for its place, convert, ask for what comes four halves later, hand over
-    auto fill = [&](Half& a, Half& c, int u, auto is_v) {
+    auto fill = [&](int u, auto is_v) {
       constexpr int kv = decltype(is_v)::value ? 1 : 0;
+      const QpInt<2 * kv> first;
+      const QpInt<2 * kv + 1> second;
       const int it = u >> 2, st = it % NS;
       const uint32_t tile = (kv ? s_v : s_k) + (uint32_t)st * kQpTile;
       qp_wait(&s_empty[kv][st], ((uint32_t)(it / NS) & 1u) ^ 1u, &s_abort, p.err);
-      store(tile, a, u, is_v);
-      load(u + 4, a);
-      store(tile + kQ8Block * 128u, c, u + 1, is_v);
-      load(u + 5, c);
+      store(tile, first, u, is_v);
+      load(u + 4, first);
+      store(tile + kQ8Block * 128u, second, u + 1, is_v);
+      load(u + 5, second);
       qp_fence_async();
       pf_arrive(&s_full[kv][st]);
     };
 #pragma unroll 1
     for (int u = 0; u < 4 * nt; u += 4) {
-      fill(x0, x1, u, QpFlag<false>());
-      fill(x2, x3, u + 2, QpFlag<true>());
+      fill(u, QpFlag<false>());
+      fill(u + 2, QpFlag<true>());
     }
   } else {
     // ---------------------------------------------------------------------------------------------- MMAs
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       uint32_t lead;
       asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
       // low descriptor words: address / 16, leading offset / 16 (1 where the K-major layout does not use it)
-      const uint32_t dq = ((s_q + (uint32_t)(qt * QP) * kQpTile) >> 4) | (1u << 16), dk = (s_k >> 4) | (1u << 16),
+      const uint32_t dq = ((s_q + (uint32_t)qt * QS) >> 4) | (1u << 16), dk = (s_k >> 4) | (1u << 16),
                      dv = (s_v >> 4) | ((kQpHalf >> 4) << 16);
       const uint32_t tS = tm + (uint32_t)qt * 128u, tO = tm + 256u + (uint32_t)qt * 128u;
       auto scores = [&](int step) {                     // S = Q K^T for one block of the key tile
