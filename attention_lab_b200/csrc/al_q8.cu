@@ -53,7 +53,7 @@ void append_launch(int mode, unsigned grid, cudaStream_t st, const Q8AppendParam
 struct Q8Plan {
   bool token;                       // the few-column kernel (mma.sync); else the prompt kernel (tcgen05)
   int cs, chunk;                    // token: CTAs per cluster; steps per CTA of a split
-  int row_tiles;                    // prompt: tiles of 256 rows
+  int row_tiles, tile_rows;         // prompt: CTAs along a group's query rows, rows a CTA (128 or 256)
   int nsplit;                       // key splits merged through the workspace
   size_t ml_off, bytes;             // nsplit > 1: workspace layout
 };
@@ -66,9 +66,9 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
   // tokens a query tile can see, as far as the host knows
   const long long span = window > 0 ? std::min<long long>(len, (long long)window + sinks) : len;
   // The few-column kernel reads the cache once per 8 query rows, the prompt kernel once per 256 but fills 128 x 128 tiles
-  // and takes 11 us for the least work. Up to 16 rows the first wins throughout (16 heads over 32 x 8192 tokens: 180 us
+  // and takes 8 us for the least work. Up to 16 rows the first wins throughout (16 heads over 32 x 8192 tokens: 180 us
   // against 212); up to 128 while everything it reads is small (one request, 8 groups: 64 rows over 512 tokens 9.0 us
-  // against 15.0, over 4096 tokens 18.1 against 18.8; 32 rows over 32 x 8192 tokens 326 against 216).
+  // against 13.6, over 4096 tokens 18.1 against 14.9; 32 rows over 32 x 8192 tokens 326 against 216).
   const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
   if (R <= kQ8TokenCols || (R <= kQ8FewCols && units * span <= kQ8FewTokens)) {
     pl.token = true;
@@ -90,10 +90,26 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
       pl.nsplit = (int)((steps + pl.chunk - 1) / pl.chunk);
     }
   } else {
-    pl.row_tiles = (int)((R + 2 * kQpRows - 1) / (2 * kQpRows));
-    const long long ctas = segs * pl.row_tiles;
-    const long long tiles = (span + T + kQpKeys - 1) / kQpKeys + 1;
-    if (ctas < sms) pl.nsplit = (int)std::max<long long>(1, std::min<long long>(sms / ctas, tiles / 4));
+    // A CTA takes 128 or 256 query rows, and with few CTAs the keys are split and the splits merged. What a call's time
+    // measured as, in tenths of a microsecond for bf16 (fp32: all about 1.4 times that): 70 and 16 a key tile with 128
+    // rows, 80 and 21 with 256, 50 for the splits' partial results and their merge; the least is taken. 32/8 heads: a
+    // prompt of 512 tokens 14.9 us (128 rows; 256 rows, keys split, 20.4), 64 rows late in 2048 tokens 15.3 (128 rows in
+    // 8 splits; 256 rows in 4, 20.8), 256 tokens late in 4096 34.5 (256 rows in 4 splits; 128 rows in 2, 41.6).
+    long long best = 0;
+    for (int rows = kQpRows; rows <= 2 * kQpRows; rows += kQpRows) {
+      const long long ctas = segs * ((R + rows - 1) / rows);
+      if (rows == kQpRows && ctas > sms) continue;
+      const long long seen = window > 0 ? std::min<long long>(len, (long long)window + sinks + rows / h + kQpKeys) : len;
+      const long long tiles = (seen + kQpKeys - 1) / kQpKeys, most = std::max<long long>(1, std::min<long long>(sms / ctas, tiles / 2));
+      for (long long ns = 1; ns <= most; ns += std::max<long long>(1, most - 1)) {
+        const long long t = (tiles + ns - 1) / ns, cost = (rows == kQpRows ? 70 + 16 * t : 80 + 21 * t) + (ns > 1 ? 50 : 0);
+        if (best > 0 && cost >= best) continue;
+        best = cost;
+        pl.tile_rows = rows;
+        pl.row_tiles = (int)((R + rows - 1) / rows);
+        pl.nsplit = (int)ns;
+      }
+    }
   }
   if (pl.nsplit > 1) {
     const size_t rows = (size_t)segs * (size_t)R;
@@ -137,9 +153,10 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
     const cudaError_t e = cudaLaunchKernelEx(&cfg, q8_decode_kernel<T>, p);
     if (e != cudaSuccess) return cuda_fail(e, "q8_decode_kernel");
   } else {
-    if ((rc = prepare_kernel(q8_prompt_kernel<T>, kQpSmem))) return rc;
+    const auto kernel = pl.tile_rows > kQpRows ? q8_prompt_kernel<T, 2> : q8_prompt_kernel<T, 1>;
+    if ((rc = prepare_kernel(kernel, kQpSmem))) return rc;
     const dim3 grid((unsigned)(p.B * p.G * pl.row_tiles), (unsigned)pl.nsplit);
-    q8_prompt_kernel<T><<<grid, kQpThreads, kQpSmem, st>>>(p);
+    kernel<<<grid, kQpThreads, kQpSmem, st>>>(p);
     if ((rc = plain_launch_check("q8_prompt_kernel"))) return rc;
   }
   if (pl.nsplit > 1) {

@@ -2,7 +2,7 @@
 // sliding window and sinks (the rule of al_q8_decode.cuh).
 //
 // The T x h query rows of a KV group are one list (row r = t * h + head), so all heads of a group share every key tile.
-// A CTA takes 256 of them as two tiles of 128 rows (TMEM lanes) and walks the key tiles (128 tokens) that any of its
+// A CTA takes 256 of them as two tiles of 128 rows (TMEM lanes; one tile where there are few) and walks the key tiles (128 tokens) that any of its
 // rows can see, in steps of one block of the cache (64 tokens). Per step and query tile: S = Q K^T (tcgen05.mma, f16
 // operands from shared memory, fp32 in TMEM), the softmax weights P go back into S's columns as f16, and O += P V (P
 // from TMEM, V from shared memory). S has two buffers per query tile, so the next step's scores are there before this
@@ -159,7 +159,8 @@ __device__ __forceinline__ int qp_row_token(int r, const Q8AttendParams& p) {
   return p.h == 1 ? r : (int)__umulhi((uint32_t)r, p.h_magic);
 }
 
-template <typename T>
+// TILES: query tiles of 128 rows a CTA takes, 2, or 1 where that spreads few rows over more CTAs.
+template <typename T, int TILES>
 __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8AttendParams p) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
@@ -184,8 +185,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   const int tile = p.row_tiles - 1 - (int)(blockIdx.x / (unsigned)BG), bg = (int)(blockIdx.x % (unsigned)BG);
   const int b = (int)((unsigned)bg / (unsigned)p.G), g = bg - b * p.G;
   const int length = q8_length(p.len, b);               // used after the set-up, which hides its latency
-  const int r0 = tile * 2 * kQpRows;
-  const int ntile = r0 + kQpRows < R ? 2 : 1;
+  const int r0 = tile * TILES * kQpRows;
+  const int ntile = TILES == 2 && r0 + kQpRows < R ? 2 : 1;
   if (tid == 13 * 32) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_qfull[i], kQpRows);
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     n = max(0, min(n, p.C));
   }
   const int pbase = n - p.T;
-  const int plo = pbase + qp_row_token(r0, p), phi = pbase + qp_row_token(min(r0 + 2 * kQpRows - 1, R - 1), p);
+  const int plo = pbase + qp_row_token(r0, p), phi = pbase + qp_row_token(min(r0 + TILES * kQpRows - 1, R - 1), p);
   const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQpKeys);
   // (total < 2^24 and nsplit <= 148: the products fit 32 bits)
   const int it0 = (int)((unsigned)rg.total * (unsigned)split / (unsigned)p.nsplit);
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
         ml[0] = m;
         ml[1] = l;
       }
-    } else if (nt == 0) {
+    } else if (qt < ntile && nt == 0) {
       // nothing to see for any row of this CTA: zeros, or an empty partial
       const int rr = r0 + qt * kQpRows + row;
       if (rr < R) {

@@ -485,6 +485,31 @@ def test_prompts_alone_and_back_to_back(dtype):
         assert torch.equal(got, want) and status() == 0
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,G,h,T,C,window,lengths", [
+    (5, 2, 3, 333, 700, 0, [641, 201, 311, 531, 421]),     # CTAs of 128 rows, some of padding alone
+    (3, 4, 5, 200, 1500, 0, [37, 1500, 0]),
+    (2, 2, 1, 300, 900, 100, [900, 129]),
+    (1, 8, 4, 64, 2048, 0, [2048]),                        # CTAs of 128 rows, keys split
+    (2, 4, 2, 130, 1000, 0, [5, 1000]),
+    (1, 4, 4, 256, 3000, 0, [2987]),                       # CTAs of 256 rows, keys split
+    (1, 1, 8, 520, 3000, 0, [701])])
+def test_prompts_of_few_rows(dtype, B, G, h, T, C, window, lengths):
+    """Every way a prompt over few rows is spread over the GPU, into memory that held NaN, with rows of padding: each row
+    is written once, by the CTA that owns it."""
+    cache = random_cache(23, B, G, C)
+    q = make_q(24, B, G, h, T, dtype)
+    on_gpu = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    want = None
+    for _ in range(20):
+        junk = torch.full((B, G, h, T, 128), float("nan"), device=DEV, dtype=q.dtype)
+        del junk
+        got = al().attend_q8(q, cache, on_gpu, window=window)
+        want = got.clone() if want is None else want
+        assert torch.equal(got, want) and status() == 0
+    check_attend(cache, q, lengths, window, 0, want)
+
+
 def test_misaligned_queries_are_copied():
     cache = random_cache(5, 1, 2, 100)
     wide = torch.randn(1, 2, 3, 1, 131, device=DEV)
