@@ -134,6 +134,11 @@ __device__ __forceinline__ float q8_factor(float f_row, int ek) {
   return fminf(fmaxf(f_row * q8_exp2i(ek), 1.17549435e-38f), 3.0e38f);
 }
 
+// r / h for a query row.
+__device__ __forceinline__ int q8_row_token(int r, const Q8AttendParams& p) {
+  return p.h == 1 ? r : (int)__umulhi((uint32_t)r, p.h_magic);
+}
+
 // 16 bytes global -> shared, zeros when !in (nothing is read then).
 __device__ __forceinline__ void qd_copy16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
@@ -149,24 +154,35 @@ __device__ __forceinline__ uint4 qd_lds16(uint32_t a) {
 template <typename T>
 __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8AttendParams p) {
   extern __shared__ __align__(1024) unsigned char qd_raw[];
-  float (*s_o)[kQdCols][kHeadDim] = reinterpret_cast<float (*)[kQdCols][kHeadDim]>(qd_raw);   // after the loop
+  float4 (*s_o)[kQdCols][kHeadDim / 4] = reinterpret_cast<float4 (*)[kQdCols][kHeadDim / 4]>(qd_raw);   // after the loop
   __shared__ float s_m[kQdWarps][kQdCols], s_l[kQdWarps][kQdCols];
-  __shared__ float s_cm[kQdCols], s_cl[kQdCols];
+  __shared__ __align__(16) float4 s_in[kMaxCluster][kHeadDim / 4];   // partials that the cluster's CTAs send to this one
+  __shared__ float2 s_in_ml[kMaxCluster];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
-  const int bg = blockIdx.y, b = bg / p.G, g = bg - b * p.G;
+  const int bg = blockIdx.y, b = (int)((unsigned)bg / (unsigned)p.G), g = bg - b * p.G;
   const int cs = gridDim.x, rank = blockIdx.x;
+  const bool clustered = !p.part && cs > 1;
+  if (clustered) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");   // this CTA runs; waited for below
   const int R = p.h * p.T;
   int n = q8_length(p.len, b);
+  // the query row, asked for before anything waits for the length
+  const int col0 = blockIdx.z * kQdCols;
+  const int col_last = min(col0 + kQdCols, R) - 1;
+  const int mycol = min(col0 + g8, R - 1);               // columns past the end repeat the last one and are not stored
+  const int mytok = q8_row_token(mycol, p);
+  Raw8<T> raw[4];
+  {
+    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + (mycol - mytok * p.h) * p.q_sh + mytok * p.q_st;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i].load(src + 64 * (i >> 1) + 16 * t4 + 8 * (i & 1));
+  }
   if (n < 0 || n > p.C) {
     if (tid == 0) atomicOr(p.err, kErrQ8Range);
     n = max(0, min(n, p.C));
   }
-  const int col0 = blockIdx.z * kQdCols;
-  const int col_last = min(col0 + kQdCols, R) - 1;
-  const int mycol = min(col0 + g8, R - 1);               // columns past the end repeat the last one and are not stored
-  const int myp = n - p.T + mycol / p.h;                 // this thread's column: position
-  const int plo = n - p.T + col0 / p.h, phi = n - p.T + col_last / p.h;
+  const int myp = n - p.T + mytok;                       // this thread's column: position
+  const int plo = n - p.T + q8_row_token(col0, p), phi = n - p.T + q8_row_token(col_last, p);
   const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQdStep);
 
   const uint8_t* kbase = p.kc + (long long)bg * p.C * kHeadDim;
@@ -220,17 +236,14 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   uint32_t qa[8][4];
   float f_row;                                           // 2^eq * scale: raw score -> log2 units (before 2^ek)
   {
-    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + (mycol % p.h) * p.q_sh + (mycol / p.h) * p.q_st;
     float x[32];
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int i = 0; i < 4; ++i) {
+      float y[8];
+      raw[i].floats(y);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float y[8];
-        q8_load8(src + 64 * half + 16 * t4 + 8 * i, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[16 * half + 8 * i + j] = y[j] * p.qsign;
-      }
+      for (int j = 0; j < 8; ++j) x[8 * i + j] = y[j] * p.qsign;
+    }
     uint32_t amax = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
@@ -392,114 +405,93 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   cp_async_wait<0>();
   __syncthreads();                                          // the rings give way to the partial results
 
-  // the CTA's partial: thread holds column g8, dimensions 16 t + j (o[j][0] + o[j][2]) and 64 + 16 t + j
+  // The warps' partials in shared memory: thread holds column g8, dimensions 16 t + j (o[j][0] + o[j][2]) and 64 + 16 t + j.
+  // Piece x (4 dimensions) of column c lies at x ^ (x >> 3 & 1) ^ 2 (c & 1): no bank twice.
+  auto place = [](int c, int x) { return x ^ ((x >> 3) & 1) ^ ((c & 1) << 1); };
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
-    *reinterpret_cast<float4*>(&s_o[warp][g8][16 * t4 + j]) =
+    s_o[warp][g8][place(g8, 4 * t4 + j / 4)] =
         make_float4(o[j][0] + o[j][2], o[j + 1][0] + o[j + 1][2], o[j + 2][0] + o[j + 2][2], o[j + 3][0] + o[j + 3][2]);
-    *reinterpret_cast<float4*>(&s_o[warp][g8][64 + 16 * t4 + j]) =
+    s_o[warp][g8][place(g8, 16 + 4 * t4 + j / 4)] =
         make_float4(o[j][1] + o[j][3], o[j + 1][1] + o[j + 1][3], o[j + 2][1] + o[j + 2][3], o[j + 3][1] + o[j + 3][3]);
   }
   if (t4 == 0) { s_m[warp][g8] = m; s_l[warp][g8] = l; }
+  __syncwarp();
+  if (clustered) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");   // every CTA of the cluster runs
   __syncthreads();
-  // merge the warps into s_o[0]: a thread takes one dimension of every NT-th column
-  {
-    constexpr int NT = kQdThreads / kHeadDim, NC = kQdCols / NT;
-    const int d = tid % kHeadDim, c0 = tid / kHeadDim;
-    float acc[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = c0 + i * NT;
-      float M = s_m[0][c];
-#pragma unroll
-      for (int w = 1; w < kQdWarps; ++w) M = fmaxf(M, s_m[w][c]);
-      float a = 0.0f, L = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kQdWarps; ++w) {
-        const float e = q8_merge_weight(s_l[w][c], s_m[w][c], M);
-        a += e != 0.0f ? e * s_o[w][c][d] : 0.0f;
-        L += q8_merge_l(s_l[w][c], s_m[w][c], M);
-      }
-      acc[i] = a;
-      if (d == 0) { s_cm[c] = M; s_cl[c] = L; }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NC; ++i) s_o[0][c0 + i * NT][d] = acc[i];
-  }
+  auto emit = [&](int c, float4 a, float L) {              // 4 dimensions of a finished column
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    if (L == 0.0f) a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int t = q8_row_token(col0 + c, p), hd = col0 + c - t * p.h;
+    T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + hd) * p.T + t) * kHeadDim + 4 * lane;
+    a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = a;
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+  };
+  // Merge. Every warp has all 32 (warp, column) weights, one a lane, and takes columns warp, warp + kQdWarps: a lane 4
+  // dimensions. (With the weights worked out by every thread for itself, in 32 copies of the code, this took 4600 cycles.)
   const int ncol = col_last - col0 + 1;
-  if (p.part) {
-    __syncthreads();
-    const long long row0 = ((long long)rank * gridDim.y + bg) * R + col0;
-    for (int i = tid; i < ncol * (kHeadDim / 4); i += kQdThreads) {
-      const int c = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4));
-      *reinterpret_cast<float4*>(p.part + (row0 + c) * kHeadDim + d) = *reinterpret_cast<const float4*>(&s_o[0][c][d]);
-    }
-    if (tid < ncol) {
-      p.part_ml[(row0 + tid) * 2] = s_cm[tid];
-      p.part_ml[(row0 + tid) * 2 + 1] = s_cl[tid];
-    }
-  } else if (cs > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    // Every CTA's (m, l), one remote load a thread, into a table of weights; then rank r sums every cs-th (column,
-    // 4 dimensions) piece over the CTAs with its remote loads in flight together. (Read one after the other in two
-    // loops these loads took about 3 us.)
-    __shared__ float s_gm[kMaxCluster][kQdCols], s_gl[kMaxCluster][kQdCols];
-    const int gr = tid >> 3, gc = tid & 7;                 // kMaxCluster * kQdCols = kQdThreads
-    static_assert(kMaxCluster * kQdCols == kQdThreads && kQdCols == 8, "one thread per (CTA, column)");
-    float mr = -INFINITY, lr = 0.0f;
-    if (gr < cs) {
-      mr = *cluster.map_shared_rank(&s_cm[gc], gr);
-      lr = *cluster.map_shared_rank(&s_cl[gc], gr);
-    }
-    s_gm[gr][gc] = mr;
-    __syncthreads();
-    float M = s_gm[0][gc];
+  float M, L, e;
+  {
+    static_assert(kQdWarps * kQdCols == 32, "a lane per (warp, column)");
+    const float mw = s_m[lane >> 3][lane & 7], lw = s_l[lane >> 3][lane & 7];
+    M = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, 8));
+    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+    e = q8_merge_weight(lw, mw, M);
+    L = q8_merge_l(lw, mw, M);
+    L += __shfl_xor_sync(0xffffffffu, L, 8);
+    L += __shfl_xor_sync(0xffffffffu, L, 16);
+  }
+#pragma unroll 1
+  for (int c = warp; c < ncol; c += kQdWarps) {
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int r = 1; r < kMaxCluster; ++r) M = fmaxf(M, s_gm[r][gc]);
-    s_gl[gr][gc] = q8_merge_l(lr, mr, M);
-    __syncthreads();
-    s_gm[gr][gc] = q8_merge_weight(lr, mr, M);             // the weight takes the maximum's place
-    __syncthreads();
-    for (int i = rank * kQdThreads + tid; i < ncol * (kHeadDim / 4); i += cs * kQdThreads) {
-      const int c = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4));
-      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float L = 0.0f;
-#pragma unroll
-      for (int r0 = 0; r0 < kMaxCluster; r0 += 8) {
-        if (r0 >= cs) break;
-        float4 v[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r0 + r < cs) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s_o[0][c][d], r0 + r));
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          if (r0 + r >= cs) break;
-          const float e = s_gm[r0 + r][c];
-          L += s_gl[r0 + r][c];
-          if (e == 0.0f) continue;
-          a.x += e * v[r].x; a.y += e * v[r].y; a.z += e * v[r].z; a.w += e * v[r].w;
-        }
-      }
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      const int cc = col0 + c, hd = cc % p.h, t = cc / p.h;
-      T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + hd) * p.T + t) * kHeadDim + d;
-      if (L == 0.0f) a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      dst[0] = fromf<T>(a.x * inv); dst[1] = fromf<T>(a.y * inv); dst[2] = fromf<T>(a.z * inv); dst[3] = fromf<T>(a.w * inv);
+    for (int w = 0; w < kQdWarps; ++w) {
+      const float ew = __shfl_sync(0xffffffffu, e, 8 * w + c);
+      const float4 v = s_o[w][c][place(c, lane)];
+      if (ew != 0.0f) { a.x += ew * v.x; a.y += ew * v.y; a.z += ew * v.z; a.w += ew * v.w; }
     }
-    cluster.sync();                                       // peers' shared memory stays until every rank has read it
-  } else {
-    __syncthreads();
-    for (int i = tid; i < ncol * kHeadDim; i += kQdThreads) {
-      const int c = i / kHeadDim, d = i % kHeadDim;
-      const float L = s_cl[c];
-      const int cc = col0 + c, hd = cc % p.h, t = cc / p.h;
-      static_cast<T*>(p.out)[(((long long)bg * p.h + hd) * p.T + t) * kHeadDim + d] =
-          fromf<T>(L == 0.0f ? 0.0f : s_o[0][c][d] / L);
+    const float Mc = __shfl_sync(0xffffffffu, M, c), Lc = __shfl_sync(0xffffffffu, L, c);
+    if (p.part) {
+      const long long row = ((long long)rank * gridDim.y + bg) * R + col0 + c;
+      *reinterpret_cast<float4*>(p.part + row * kHeadDim + 4 * lane) = a;
+      if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + row * 2) = make_float2(Mc, Lc);
+    } else if (cs == 1) {
+      emit(c, a, Lc);
+    } else {
+      // to the CTA that finishes the column: rank c mod cs (cs is a power of two)
+      const int owner = c & (cs - 1), slot = (c - owner) + rank;
+      cg::cluster_group cluster = cg::this_cluster();
+      *cluster.map_shared_rank(&s_in[slot][lane], owner) = a;
+      if (lane == 0) *cluster.map_shared_rank(&s_in_ml[slot], owner) = make_float2(Mc, Lc);
     }
+  }
+  __syncwarp();
+  if (!clustered) return;
+  // One barrier, and every CTA finishes its columns from its own shared memory. (Reading the others' partials instead takes
+  // a remote round trip and a second barrier.)
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+#pragma unroll 1
+  for (int c = rank + cs * warp; c < ncol; c += cs * kQdWarps) {
+    const float2 ml = lane < cs ? s_in_ml[c - rank + lane] : make_float2(-INFINITY, 0.0f);
+    M = ml.x;
+#pragma unroll
+    for (int o2 = 8; o2 > 0; o2 >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o2));
+    e = q8_merge_weight(ml.y, ml.x, M);
+    L = q8_merge_l(ml.y, ml.x, M);
+#pragma unroll
+    for (int o2 = 8; o2 > 0; o2 >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o2);
+    L = __shfl_sync(0xffffffffu, L, 0);
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int r = 0; r < cs; ++r) {
+      const float er = __shfl_sync(0xffffffffu, e, r);
+      const float4 v = s_in[c - rank + r][lane];
+      if (er != 0.0f) { a.x += er * v.x; a.y += er * v.y; a.z += er * v.z; a.w += er * v.w; }
+    }
+    emit(c, a, L);
   }
 }
 

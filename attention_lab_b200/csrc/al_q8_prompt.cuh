@@ -154,11 +154,6 @@ __device__ __forceinline__ uint32_t qp_chunk(uint32_t tile, int r, int c) {
 template <bool B> struct QpFlag { static constexpr bool value = B; };
 template <int I> struct QpInt { static constexpr int value = I; };
 
-// r / h for a query row.
-__device__ __forceinline__ int qp_row_token(int r, const Q8AttendParams& p) {
-  return p.h == 1 ? r : (int)__umulhi((uint32_t)r, p.h_magic);
-}
-
 // TILES: query tiles of 128 rows a CTA takes, 2, or 1 where that spreads few rows over more CTAs.
 template <typename T, int TILES>
 __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8AttendParams p) {
@@ -213,7 +208,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   auto load_rows = [&](int round) {
     const int rq = r0 + qt * kQpRows + wrow0 + 16 * PER * round + lane / LPR, left = R - rq;   // rows from this one on
     // rows PER apart: PER / h tokens and PER % h heads further, one token more where the head wraps
-    const int t0 = qp_row_token(rq, p), dt = p.h == 1 ? PER : p.h == PER ? 1 : 0, dh = PER - dt * p.h;
+    const int t0 = q8_row_token(rq, p), dt = p.h == 1 ? PER : p.h == PER ? 1 : 0, dh = PER - dt * p.h;
     int head = rq - t0 * p.h;
     const T* src = static_cast<const T*>(p.q) + b * p.q_sb + g * p.q_sg + head * p.q_sh + t0 * p.q_st + V16<T>::n * (lane % LPR);
     const long long hop = dt * p.q_st + dh * p.q_sh, wrap = p.q_st - p.h * p.q_sh;
@@ -238,7 +233,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     n = max(0, min(n, p.C));
   }
   const int pbase = n - p.T;
-  const int plo = pbase + qp_row_token(r0, p), phi = pbase + qp_row_token(min(r0 + TILES * kQpRows - 1, R - 1), p);
+  const int plo = pbase + q8_row_token(r0, p), phi = pbase + q8_row_token(min(r0 + TILES * kQpRows - 1, R - 1), p);
   const Q8Range rg = q8_range(plo, phi, p.window, p.sinks, kQpKeys);
   // (total < 2^24 and nsplit <= 148: the products fit 32 bits)
   const int it0 = (int)((unsigned)rg.total * (unsigned)split / (unsigned)p.nsplit);
@@ -280,7 +275,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
     const int row = tid & 127;
     if (qt < ntile && nt > 0) {
       const int r = min(r0 + qt * kQpRows + row, R - 1);
-      const int pos = pbase + qp_row_token(r, p);
+      const int pos = pbase + q8_row_token(r, p);
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t tS = tm + lanes + (uint32_t)qt * 128u, tO = tm + lanes + 256u + (uint32_t)qt * 128u;
       const uint32_t qtile = s_q + (uint32_t)qt * QS;
@@ -343,7 +338,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       const float f_row = s_frow[qt * kQpRows + row];
       // positions of the warp's rows, for the test that a step needs no mask
       const int rw0 = r0 + qt * kQpRows + wrow0;
-      const int wlo = pbase + qp_row_token(min(rw0, R - 1), p), whi = pbase + qp_row_token(min(rw0 + 31, R - 1), p);
+      const int wlo = pbase + q8_row_token(min(rw0, R - 1), p), whi = pbase + q8_row_token(min(rw0 + 31, R - 1), p);
       const signed char* keb = p.ke + (long long)bg * p.NB;
       const signed char* veb = p.ve + (long long)bg * p.NB;
       float m = -INFINITY, l = 0.0f;
@@ -542,7 +537,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
           ml[0] = -INFINITY;
           ml[1] = 0.0f;
         } else {
-          const int t = qp_row_token(rr, p), head = rr - t * p.h;
+          const int t = q8_row_token(rr, p), head = rr - t * p.h;
           T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim;
           const float z[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
           for (int c = 0; c < 16; ++c) q8_store8(dst + 8 * c, z);
