@@ -66,20 +66,22 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
   // tokens a query tile can see, as far as the host knows
   const long long span = window > 0 ? std::min<long long>(len, (long long)window + sinks) : len;
   // The few-column kernel reads the cache once per 8 query rows, the prompt kernel once per 256 but fills 128 x 128 tiles
-  // and takes 8 us for the least work. Up to 16 rows the first wins throughout (16 heads over 32 x 8192 tokens: 180 us
-  // against 212); up to 128 while everything it reads is small (one request, 8 groups: 64 rows over 512 tokens 9.0 us
-  // against 13.6, over 4096 tokens 18.1 against 14.9; 32 rows over 32 x 8192 tokens 326 against 216).
+  // and takes 8 us for the least work. Up to 16 rows the first wins throughout (16 heads over 32 x 8192 tokens: 175 us
+  // against 211); up to 128 while everything it reads is small (one request, 8 groups: 64 rows over 512 tokens 5.8 us
+  // against 13.6, over 4096 tokens 15.4 against 15.1; 32 rows over 32 x 8192 tokens 317 against 215).
   const long long ngrp = (R + kQdCols - 1) / kQdCols, units = segs * ngrp;
   if (R <= kQ8TokenCols || (R <= kQ8FewCols && units * span <= kQ8FewTokens)) {
     pl.token = true;
-    // One wave: clusters grow while the CTAs (two an SM) still fit at once and every warp keeps two steps. 8 segments of
-    // 2048 tokens: 8 CTAs 8.6 us, 16 10.5; 6 x 8 segments of 4100 tokens: 4 CTAs 19.4 us, 6 21.6, 8 27.9.
+    // One wave: clusters grow while the CTAs (two an SM) still fit at once and every warp keeps a step (two before the
+    // first doubling, which brings the exchange). 8 segments of 2048 tokens: 8 CTAs each 5.4 us, 16 5.2; 128 of 256
+    // tokens: one CTA each 4.9, two 5.8.
     pl.cs = 1;
-    while (pl.cs < kMaxCluster && units * pl.cs * 2 <= 2LL * sms && span >= pl.cs * 4LL * kQdWarps * kQdStep) pl.cs <<= 1;
-    // Splits merged by a second kernel: more CTAs a segment than clusters spread over the SMs (one request of 128K: 50 us
-    // against 92), and for requests of their own lengths runs of 4096 tokens, so that the load evens out whatever the
-    // lengths are: 256 segments of 16K to 32K tokens 272 us against 282 with clusters of 4 (runs of 2048: 290), 64 of 100
-    // to 32K 54 against 76; 64 segments that all have 32K lose, 102 against 92.
+    while (pl.cs < kMaxCluster && units * pl.cs * 2 <= 2LL * sms && span >= pl.cs * (pl.cs == 1 ? 4LL : 2LL) * kQdWarps * kQdStep)
+      pl.cs <<= 1;
+    // Splits merged by a second kernel: more CTAs a segment than clusters spread over the SMs (one request of 128K: 48 us
+    // against 89; 6 x 8 segments of 4100 tokens: 13.8 against 16.4), and for requests of their own lengths runs of 4096
+    // tokens, so that the load evens out whatever the lengths are: 256 segments of 16K to 32K tokens 259 us against 316
+    // with clusters, 64 of 100 to 32K 54 against 72; 64 segments that all have 32K lose, 97 against 91.
     long long fill = std::min<long long>(2LL * sms / units, span / (2 * kQdWarps * kQdStep));
     if (ragged) fill = std::max<long long>(fill, span / kQdChunk);
     fill = std::min<long long>(fill, 32 * kQmWarps);

@@ -28,7 +28,7 @@ namespace al {
 
 constexpr int kQ8TokenCols = 16;           // up to this many query rows per group always take this kernel
 constexpr int kQ8FewCols = 128;            // up to this many do while (segments x groups of 8 rows x tokens) is at most
-constexpr long long kQ8FewTokens = 1 << 17;   // this; the rest take the prompt kernel
+constexpr long long kQ8FewTokens = 1 << 18;   // this; the rest take the prompt kernel
 constexpr int kQdWarps = 4;
 constexpr int kQdThreads = 32 * kQdWarps;
 constexpr int kQdCols = 8;                 // columns (query, head) per CTA
@@ -134,6 +134,10 @@ __device__ __forceinline__ float q8_factor(float f_row, int ek) {
   return fminf(fmaxf(f_row * q8_exp2i(ek), 1.17549435e-38f), 3.0e38f);
 }
 
+__device__ __forceinline__ void q8_store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void q8_store4(__nv_bfloat16* p, float4 v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+}
 // r / h for a query row.
 __device__ __forceinline__ int q8_row_token(int r, const Q8AttendParams& p) {
   return p.h == 1 ? r : (int)__umulhi((uint32_t)r, p.h_magic);
@@ -163,6 +167,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   const int bg = blockIdx.y, b = (int)((unsigned)bg / (unsigned)p.G), g = bg - b * p.G;
   const int cs = gridDim.x, rank = blockIdx.x;
   const bool clustered = !p.part && cs > 1;
+  if (p.part) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the merge, which waits for the end of this grid
   if (clustered) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");   // this CTA runs; waited for below
   const int R = p.h * p.T;
   int n = q8_length(p.len, b);
@@ -426,9 +431,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
     if (L == 0.0f) a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int t = q8_row_token(col0 + c, p), hd = col0 + c - t * p.h;
     T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + hd) * p.T + t) * kHeadDim + 4 * lane;
-    a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = a;
-    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+    q8_store4(dst, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
   };
   // Merge. Every warp has all 32 (warp, column) weights, one a lane, and takes columns warp, warp + kQdWarps: a lane 4
   // dimensions. (With the weights worked out by every thread for itself, in 32 copies of the code, this took 4600 cycles.)

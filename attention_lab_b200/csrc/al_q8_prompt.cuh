@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   const int split = blockIdx.y;
   const int tile = p.row_tiles - 1 - (int)(blockIdx.x / (unsigned)BG), bg = (int)(blockIdx.x % (unsigned)BG);
   const int b = (int)((unsigned)bg / (unsigned)p.G), g = bg - b * p.G;
+  if (p.part) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the merge, which waits for the end of this grid
   const int length = q8_length(p.len, b);               // used after the set-up, which hides its latency
   const int r0 = tile * TILES * kQpRows;
   const int ntile = TILES == 2 && r0 + kQpRows < R ? 2 : 1;
@@ -691,6 +692,17 @@ __global__ void __launch_bounds__(32 * kQmWarps) q8_merge_kernel(const Q8AttendP
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   // the common maximum: a lane per split (nsplit <= 32 * WPR)
   const int mine = part + WPR * lane;
+  // the first partial rows are asked for together with their maxima
+  constexpr int kAhead = 8;
+  float4 v[kAhead];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int s = part + WPR * (i + k);
+      if (s < p.nsplit) v[k] = *reinterpret_cast<const float4*>(p.part + ((long long)s * rows + row) * kHeadDim + d);
+    }
+  };
+  fetch(0);
   float2 ml = make_float2(-INFINITY, 0.0f);
   if (mine < p.nsplit) ml = *reinterpret_cast<const float2*>(p.part_ml + ((long long)mine * rows + row) * 2);
   float M = ml.x;
@@ -707,28 +719,33 @@ __global__ void __launch_bounds__(32 * kQmWarps) q8_merge_kernel(const Q8AttendP
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-  for (int i = 0; part + WPR * i < p.nsplit; ++i) {
-    const float e = __shfl_sync(0xffffffffu, wgt, i);
-    if (e == 0.0f) continue;                             // also an empty split, whose O was not written
-    const float4 v = *reinterpret_cast<const float4*>(p.part + ((long long)(part + WPR * i) * rows + row) * kHeadDim + d);
-    a.x += e * v.x; a.y += e * v.y; a.z += e * v.z; a.w += e * v.w;
+#pragma unroll 1
+  for (int i = 0; part + WPR * i < p.nsplit; i += kAhead) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float e = __shfl_sync(0xffffffffu, wgt, (i + k) & 31);
+      // (weight zero: also an empty split, whose O was not written)
+      if (part + WPR * (i + k) < p.nsplit && e != 0.0f) { a.x += e * v[k].x; a.y += e * v[k].y; a.z += e * v[k].z; a.w += e * v[k].w; }
+    }
+    fetch(i + kAhead);
   }
   if (WPR > 1) {
     *reinterpret_cast<float4*>(&s_o[warp][d]) = a;
     if (lane == 0) s_l[warp] = L;
     __syncthreads();
     if (part > 0) return;
+#pragma unroll
     for (int w = 1; w < WPR; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(&s_o[first + w][d]);
-      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+      const float4 x = *reinterpret_cast<const float4*>(&s_o[first + w][d]);
+      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
       L += s_l[first + w];
     }
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  const int bg = (int)(row / R), r = (int)(row - (long long)bg * R), t = r / p.h, head = r - t * p.h;
+  // (B G R < 2^31)
+  const int bg = (int)((unsigned)row / (unsigned)R), r = (int)row - bg * R, t = q8_row_token(r, p), head = r - t * p.h;
   T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + head) * p.T + t) * kHeadDim + d;
-  dst[0] = fromf<T>(a.x * inv); dst[1] = fromf<T>(a.y * inv); dst[2] = fromf<T>(a.z * inv); dst[3] = fromf<T>(a.w * inv);
+  q8_store4(dst, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
 }
 
 }  // namespace al
