@@ -179,7 +179,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   const int split = blockIdx.y;
   const int tile = p.row_tiles - 1 - (int)(blockIdx.x / (unsigned)BG), bg = (int)(blockIdx.x % (unsigned)BG);
   const int b = (int)((unsigned)bg / (unsigned)p.G), g = bg - b * p.G;
-  if (p.part) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the merge, which waits for the end of this grid
   const int length = q8_length(p.len, b);               // used after the set-up, which hides its latency
   const int r0 = tile * TILES * kQpRows;
   const int ntile = TILES == 2 && r0 + kQpRows < R ? 2 : 1;
