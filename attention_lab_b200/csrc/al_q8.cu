@@ -58,7 +58,7 @@ struct Q8Plan {
   size_t ml_off, bytes;             // nsplit > 1: workspace layout
 };
 
-int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_length, bool ragged, int sms, Q8Plan* out) {
+int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_length, bool ragged, bool wide, int sms, Q8Plan* out) {
   Q8Plan pl = {};
   pl.nsplit = 1;
   const long long R = (long long)h * T, segs = (long long)B * G;
@@ -92,7 +92,7 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
       pl.nsplit = (int)((steps + pl.chunk - 1) / pl.chunk);
     }
   } else {
-    // A CTA takes 128 or 256 query rows, and with few CTAs the keys are split and the splits merged. What a call's time
+    // A CTA takes 128 or 256 query rows (32-bit queries 128), and with few CTAs the keys are split and the splits merged. What a call's time
     // measured as, in tenths of a microsecond for bf16 (fp32: all about 1.4 times that): 70 and 16 a key tile with 128
     // rows, 80 and 21 with 256, 50 for the splits' partial results and their merge; the least is taken. 32/8 heads: a
     // prompt of 512 tokens 14.9 us (128 rows; 256 rows, keys split, 20.4), 64 rows late in 2048 tokens 15.3 (128 rows in
@@ -100,7 +100,7 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
     long long best = 0;
     for (int rows = kQpRows; rows <= 2 * kQpRows; rows += kQpRows) {
       const long long ctas = segs * ((R + rows - 1) / rows);
-      if (rows == kQpRows && ctas > sms) continue;
+      if (wide ? rows > kQpRows : rows == kQpRows && ctas > sms) continue;   // 32-bit queries: always 128 (kQpFlush)
       const long long seen = window > 0 ? std::min<long long>(len, (long long)window + sinks + rows / h + kQpKeys) : len;
       const long long tiles = (seen + kQpKeys - 1) / kQpKeys, most = std::max<long long>(1, std::min<long long>(sms / ctas, tiles / 2));
       for (long long ns = 1; ns <= most; ns += std::max<long long>(1, most - 1)) {
@@ -155,7 +155,10 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
     const cudaError_t e = cudaLaunchKernelEx(&cfg, q8_decode_kernel<T>, p);
     if (e != cudaSuccess) return cuda_fail(e, "q8_decode_kernel");
   } else {
-    const auto kernel = pl.tile_rows > kQpRows ? q8_prompt_kernel<T, 2> : q8_prompt_kernel<T, 1>;
+    auto kernel = q8_prompt_kernel<T, 1>;
+    if constexpr (sizeof(T) == 2) {
+      if (pl.tile_rows > kQpRows) kernel = q8_prompt_kernel<T, 2>;
+    }
     if ((rc = prepare_kernel(kernel, kQpSmem))) return rc;
     const dim3 grid((unsigned)(p.B * p.G * pl.row_tiles), (unsigned)pl.nsplit);
     kernel<<<grid, kQpThreads, kQpSmem, st>>>(p);
@@ -319,9 +322,10 @@ int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int si
   if (B == 0 || T == 0) return AL_OK;
   DeviceInfo* di = nullptr;
   if ((rc = device_info(&di))) return rc;
-  Q8Plan pl;
-  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, true, di->sms, &pl))) return rc;
-  *bytes = pl.bytes;
+  Q8Plan pl, pl32;
+  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, true, false, di->sms, &pl))) return rc;
+  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, true, true, di->sms, &pl32))) return rc;
+  *bytes = std::max(pl.bytes, pl32.bytes);               // enough for either type
   return AL_OK;
 }
 
@@ -341,7 +345,7 @@ int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_
   DeviceInfo* di = nullptr;
   if ((rc = device_info(&di))) return rc;
   Q8Plan pl;
-  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, lengths != nullptr, di->sms, &pl))) return rc;
+  if ((rc = q8_plan(B, G, h, T, C, window, sinks, max_length, lengths != nullptr, dtype == AL_F32, di->sms, &pl))) return rc;
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)))
     return fail(AL_EINVAL, "this call needs a 16-byte aligned workspace of %zu bytes, got %zu", pl.bytes, workspace_bytes);
   Q8AttendParams p = {};

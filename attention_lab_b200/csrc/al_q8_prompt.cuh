@@ -13,7 +13,7 @@
 //                   swizzled layout both contractions read; the next tile's codes are in registers meanwhile
 //   warps 12, 13    issue the MMAs, one per query tile
 // 16-bit queries are one f16 operand (scaled by a power of two per row, exact). 32-bit queries and their weights are
-// split into two f16 terms (SPLIT): twice the MMAs, about 21 bits, single-buffered key tiles.
+// split into two f16 terms (SPLIT): twice the MMAs, about 21 bits, one query tile a CTA (see kQpFlush).
 //
 // Bound: shared memory and the MUFU together. A step's MMAs read their operands for 1280 cycles of an SM's shared-memory
 // bandwidth (Q again for every 64 keys), the converting warps store 32 KB (256 cycles), and its exponentials hold the MUFU
@@ -37,8 +37,12 @@ constexpr uint32_t kQpHalf = kQpTile / 2;
 constexpr int kQpPitch = 256 + 16;                     // output rows on their way out, 256 bytes at a time: no bank twice
 constexpr uint32_t kQpStage = kQpRows * kQpPitch;      // 34 KB
 static_assert(kQpStage % 1024 == 0, "tiles start on 1 KB");
-constexpr size_t kQpSmem = 1024 + 4 * kQpTile + 2 * kQpStage;   // 2 Q + 2 K + 2 V tiles; 4 Q (high, low) + K + V are less
+constexpr size_t kQpSmem = 1024 + 4 * kQpTile + 2 * kQpStage;   // 2 Q + 2 K + 2 V tiles (a 32-bit tile's two terms are less)
 constexpr int kQpNanList = 64;
+// 32-bit queries: steps that O accumulates before it is added to the sum in TMEM's free half, in fp32 with rounding. The
+// tensor cores cut each of their sums off towards zero: without this the output loses 2.3e-6 over 1024 tokens, 1.8e-5 over
+// 16384 (elementary operations in fp32: 0.7e-6, 2.3e-6). 16-bit outputs are rounded to 2e-3 in any case.
+constexpr int kQpFlush = 4;
 constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8)
 // Registers a thread after the split: 2 x 128 softmax threads, 128 converting threads, the MMA warp's group.
 // 184 + 184 + 104 + 40 = 512 = 4 x the 128 of the launch.
@@ -158,7 +162,8 @@ template <int I> struct QpInt { static constexpr int value = I; };
 template <typename T, int TILES>
 __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8AttendParams p) {
   constexpr bool SPLIT = sizeof(T) == 4;
-  constexpr int NS = SPLIT ? 1 : 2;                    // key tiles in flight
+  static_assert(!SPLIT || TILES == 1, "the second tile's TMEM holds the sums of 32-bit queries");
+  constexpr int NS = 2;                                // key tiles in flight
   constexpr int QP = SPLIT ? 2 : 1;                    // f16 terms per query row
   constexpr uint32_t QS = SPLIT ? 2 * kQpTile : kQpStage;   // bytes of a query tile, later of its output rows
   extern __shared__ __align__(1024) unsigned char qp_raw[];
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
   // descriptors and branches in the uniform datapath (otherwise every MMA takes some 45 instructions).
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t base = (smem_addr(qp_raw) + 1023u) & ~1023u;
-  const uint32_t s_q = base, s_k = base + 2 * QS, s_v = s_k + NS * kQpTile;
+  const uint32_t s_q = base, s_k = base + TILES * QS, s_v = s_k + NS * kQpTile;
 
   // the longest row tiles first; all (batch, group) pairs of a row tile together
   const int BG = p.B * p.G, R = p.h * p.T;
@@ -278,6 +283,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       const int pos = pbase + q8_row_token(r, p);
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t tS = tm + lanes + (uint32_t)qt * 128u, tO = tm + lanes + 256u + (uint32_t)qt * 128u;
+      const uint32_t tA = tm + lanes + 384u;           // the sum of 32-bit queries
       const uint32_t qtile = s_q + (uint32_t)qt * QS;
       // Every row is scaled by a power of two into f16 (32-bit rows: two f16 terms) and goes to its places in the query
       // tile. Row maxima: each lane's over its pieces, then a transposing reduction that leaves piece i's row to lane i.
@@ -342,6 +348,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       const signed char* keb = p.ke + (long long)bg * p.NB;
       const signed char* veb = p.ve + (long long)bg * p.NB;
       float m = -INFINITY, l = 0.0f;
+      float m_sum = -INFINITY;                         // the maximum that the sum in TMEM is relative to
       int ev_top = -128;                               // largest V exponent met so far
       const int nsteps = 2 * nt;
       auto step_token = [&](int step) { return tile_token(it0 + (step >> 1)) + kQ8Block * (step & 1); };
@@ -422,6 +429,29 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
             }
           }
         }
+        if (SPLIT && step > 0 && step % kQpFlush == 0) {
+          // O's share so far joins the sum; this step's P V starts O anew (the wait is the one above)
+          qp_wait(&s_pv[qt][1 - buf], (uint32_t)((step - 1) >> 1) & 1u, &s_abort, p.err);
+          tmem_fence_after_sync();
+          __syncwarp();
+          tmem_wait_st();
+          const float fa = m_sum == m ? 1.0f : q8_ex2(m_sum - m);
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16], a[16];
+            tmem_ld16(tO + 16u * (uint32_t)c, o);
+            tmem_ld16(tA + 16u * (uint32_t)c, a);        // (what it holds before the first time is not used)
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              asm volatile("" : "+r"(o[i]), "+r"(a[i]));
+              if (step > kQpFlush) o[i] = __float_as_uint(fmaf(__uint_as_float(a[i]), fa, __uint_as_float(o[i])));
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) tmem_st2(tA + 16u * (uint32_t)c + (uint32_t)i, o[i], o[i + 1]);
+          }
+          m_sum = m;
+        }
         const float mref = (m == -INFINITY ? 0.0f : m) - kQpBias, add = fev - mref;
         ev_top = max(ev_top, ev_now);
         float far = 0.0f;
@@ -475,6 +505,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
       const bool wide = part || SPLIT;                   // 32-bit rows: 64 dimensions at a time
       const int rr = r0 + qt * kQpRows + row;
       const float z = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+      const float fa = m_sum == m ? 1.0f : q8_ex2(m_sum - m);
       const uint32_t stage = qtile + (uint32_t)(row * kQpPitch);
       const int head = r - (pos - pbase) * p.h;          // row r of a group is token r / h, head r % h; partial results keep r
       char* dst = part ? reinterpret_cast<char*>(p.part + (((long long)split * BG + bg) * R + r) * kHeadDim)
@@ -484,6 +515,13 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
         uint32_t o[32];
         pf_tmem_ld32(tO + 32u * (uint32_t)c, o);
         pf_tmem_wait(o);
+        if (SPLIT && nsteps > kQpFlush) {
+          uint32_t a[32];
+          pf_tmem_ld32(tA + 32u * (uint32_t)c, a);
+          pf_tmem_wait(a);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(a[i]), fa, __uint_as_float(o[i])));
+        }
         if (bad > 0) {
           // tokens with a NaN code in V: the listed ones, or all of this CTA's when the list ran over
           const int cnt = bad <= kQpNanList ? bad : nt * kQpKeys;
@@ -636,7 +674,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prompt_kernel(const Q8Attend
 #pragma unroll
           for (uint32_t ks = 0; ks < 4; ++ks)
             qp_mma_ts(lead, tO, tS + (uint32_t)(step & 1) * 64u + (uint32_t)term * 32u + ks * 8u,
-                      dv + ((vb + ks * 2048u) >> 4), (step | term | (int)ks) > 0 ? 1u : 0u);
+                      dv + ((vb + ks * 2048u) >> 4), ((SPLIT ? step % kQpFlush : step) | term | (int)ks) > 0 ? 1u : 0u);
         qp_commit(lead, &s_pv[qt][step & 1]);
       };
       qp_wait(&s_full[0][0], 0, &s_abort, p.err);

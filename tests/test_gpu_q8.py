@@ -510,6 +510,21 @@ def test_prompts_of_few_rows(dtype, B, G, h, T, C, window, lengths):
     check_attend(cache, q, lengths, window, 0, want)
 
 
+def test_fp32_prompts_do_not_drift():
+    """The tensor cores cut sums off towards zero; over a long context that must not add up. With every value one the output
+    is one: O loses at most 2^-23 of itself in each of the 32 sums between two additions to the fp32 sum, and the errors of
+    those additions and of the denominator, rounded to nearest, average out over the rows."""
+    n = 12000
+    cache = random_cache(31, 2, 8, n)
+    cache.v.copy_(torch.full((2, 8, n, 128), 256.0, device=DEV).to(torch.float8_e4m3fn))
+    cache.v_exp.fill_(-8)
+    q = make_q(32, 2, 8, 8, 80, "f32")
+    out = al().attend_q8(q, cache, torch.tensor([n, n - 77], dtype=torch.int32, device=DEV))
+    drift = float((out.double() - 1).mean())
+    assert abs(drift) <= 32 * 2 ** -23, drift
+    assert status() == 0
+
+
 def test_misaligned_queries_are_copied():
     cache = random_cache(5, 1, 2, 100)
     wide = torch.randn(1, 2, 3, 1, 131, device=DEV)
