@@ -16,8 +16,8 @@
 // Bound: HBM reads of 256 bytes per visible token and group. The work of a segment is split over a cluster of CTAs
 // whose partial (m, l, O) are merged through distributed shared memory, so one launch does the whole step; with so few
 // segments that clusters of 16 leave SMs idle, or with requests of their own lengths, over runs of steps whose partials go
-// through global memory to q8_merge_kernel. 32 requests of 16K to 32K tokens, 32/8 heads: 272 us, 5.9 TB/s; 32 of 32K: 338
-// us, 6.4 TB/s; one of 128K: 50 us, 5.4 TB/s; one of 2048: 8.6 us, all latency (launch, length, rows, two steps, merge).
+// through global memory to q8_merge_kernel. 32 requests of 16K to 32K tokens, 32/8 heads: 259 us, 6.2 TB/s; 32 of 32K: 322
+// us, 6.7 TB/s; one of 128K: 47 us, 5.7 TB/s; one of 2048: 5.1 us, all latency (launch, length, rows, a step, merge).
 // Registers fed from global memory without the ring ran the first at 417 us: two CTAs of four warps an SM held too few
 // bytes in flight.
 #pragma once
