@@ -43,7 +43,7 @@ constexpr int kQpNanList = 64;
 // tensor cores cut each of their sums off towards zero: without this the output loses 2.3e-6 over 1024 tokens, 1.8e-5 over
 // 16384 (elementary operations in fp32: 0.7e-6, 2.3e-6). 16-bit outputs are rounded to 2e-3 in any case.
 constexpr int kQpFlush = 4;
-constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8)
+constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8); f16 ends them 2^-30 below a row's largest
 // Registers a thread after the split: 2 x 128 softmax threads, 128 converting threads, the MMA warp's group.
 // 184 + 184 + 104 + 40 = 512 = 4 x the 128 of the launch.
 constexpr int kQpRegsSoftmax = 184, kQpRegsConvert = 104, kQpRegsMma = 40;
