@@ -122,14 +122,20 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
   return AL_OK;
 }
 
-int q8_attend_check(int B, int G, int h, int T, int C, int window, int sinks) {
+// A window or sinks as large as the cache hide nothing, and are passed on as none: the kernels subtract the window from
+// positions down to -T (at least -2^25, below) in 32 bits, which holds for a window smaller than a cache that fits memory.
+void q8_visible(int C, int* window, int* sinks) {
+  if (*window >= C || *sinks >= C) *window = 0;
+  if (*window == 0) *sinks = 0;
+}
+
+int q8_attend_check(int B, int G, int h, int T, int window, int sinks) {
   if (h < 1 || T < 0) return fail(AL_EINVAL, "h must be positive and T not negative, got h=%d T=%d", h, T);
   if (window < 0 || sinks < 0) return fail(AL_EINVAL, "window and sinks must not be negative, got %d and %d", window, sinks);
   if (h > 64) return fail(AL_EUNSUPPORTED, "heads per group must be in [1, 64], got %d", h);
   if ((long long)h * T > (1 << 25)) return fail(AL_EUNSUPPORTED, "h*T = %lld exceeds 2^25 query rows per group", (long long)h * T);
   if (B * (long long)G * (((long long)h * T + 255) / 256) > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query tiles");
   if (B * (long long)G * h * T > 0x7fffffffLL) return fail(AL_EUNSUPPORTED, "too many query rows");
-  (void)C;
   return AL_OK;
 }
 
@@ -317,8 +323,9 @@ int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int si
   if (!bytes) return fail(AL_EINVAL, "null bytes");
   *bytes = 0;
   if (B < 0 || G <= 0 || C <= 0) return fail(AL_EINVAL, "G and C must be positive and B not negative");
-  int rc = q8_attend_check(B, G, h, T, C, window, sinks);
+  int rc = q8_attend_check(B, G, h, T, window, sinks);
   if (rc) return rc;
+  q8_visible(C, &window, &sinks);
   if (B == 0 || T == 0) return AL_OK;
   DeviceInfo* di = nullptr;
   if ((rc = device_info(&di))) return rc;
@@ -336,7 +343,8 @@ int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_
   if (!dtype_ok(dtype)) return fail(AL_EINVAL, "unknown dtype code");
   int rc = q8_shape(B, G, C, d, k_codes, v_codes, k_exp, v_exp);
   if (rc) return rc;
-  if ((rc = q8_attend_check(B, G, h, T, C, window, sinks))) return rc;
+  if ((rc = q8_attend_check(B, G, h, T, window, sinks))) return rc;
+  q8_visible(C, &window, &sinks);
   if (!lengths && (length < 0 || length > C)) return fail(AL_EINVAL, "length=%d must be in [0, capacity=%d]", length, C);
   if (!(scale == scale) || scale > 3.0e38f || scale < -3.0e38f) return fail(AL_EINVAL, "scale must be finite");
   if (B == 0 || T == 0) return AL_OK;
@@ -354,7 +362,7 @@ int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_
   p.ke = static_cast<const signed char*>(k_exp); p.ve = static_cast<const signed char*>(v_exp);
   p.len.per_batch = lengths; p.len.all = length;
   p.B = B; p.G = G; p.h = h; p.T = T; p.C = C; p.NB = q8_blocks(C);
-  p.window = window; p.sinks = window > 0 ? sinks : 0;
+  p.window = window; p.sinks = sinks;
   p.scale = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
   p.qsign = scale < 0 ? -1.0f : 1.0f;
   p.out = out; p.nsplit = pl.nsplit; p.row_tiles = pl.row_tiles; p.chunk = pl.chunk; p.err = di->err;
