@@ -122,9 +122,15 @@ __device__ __forceinline__ float q8_rescale(float x, float d) {
 }
 
 // Merging partials (m, l, O): the weight of one with maximum m under the common maximum M, and its share of the
-// denominator. An empty partial has m = -inf and l = 0; one whose every score was NaN has m = -inf and l NaN.
+// denominator. An empty partial has m = -inf and l = 0; one whose every score was NaN has m = -inf and l NaN. Only empty
+// partials, whose O may not have been written, are left out (a negative weight): one whose weight underflows still brings
+// the NaN of a V code that it saw, so that the result's NaN do not depend on how the tokens were split.
+constexpr float kQ8Skip = -1.0f;
 __device__ __forceinline__ float q8_merge_weight(float l, float m, float M) {
-  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : q8_ex2(m - M);
+  return m == -INFINITY ? (l == 0.0f ? kQ8Skip : 1.0f) : q8_ex2(m - M);
+}
+__device__ __forceinline__ void q8_merge_add(float4& a, float weight, const float4& v) {
+  if (weight != kQ8Skip) { a.x += weight * v.x; a.y += weight * v.y; a.z += weight * v.z; a.w += weight * v.w; }
 }
 __device__ __forceinline__ float q8_merge_l(float l, float m, float M) { return m == -INFINITY ? l : q8_rescale(l, m - M); }
 
@@ -453,8 +459,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
 #pragma unroll
     for (int w = 0; w < kQdWarps; ++w) {
       const float ew = __shfl_sync(0xffffffffu, e, 8 * w + c);
-      const float4 v = s_o[w][c][place(c, lane)];
-      if (ew != 0.0f) { a.x += ew * v.x; a.y += ew * v.y; a.z += ew * v.z; a.w += ew * v.w; }
+      q8_merge_add(a, ew, s_o[w][c][place(c, lane)]);
     }
     const float Mc = __shfl_sync(0xffffffffu, M, c), Lc = __shfl_sync(0xffffffffu, L, c);
     if (p.part) {
@@ -491,8 +496,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
 #pragma unroll 4
     for (int r = 0; r < cs; ++r) {
       const float er = __shfl_sync(0xffffffffu, e, r);
-      const float4 v = s_in[c - rank + r][lane];
-      if (er != 0.0f) { a.x += er * v.x; a.y += er * v.y; a.z += er * v.z; a.w += er * v.w; }
+      q8_merge_add(a, er, s_in[c - rank + r][lane]);
     }
     emit(c, a, L);
   }

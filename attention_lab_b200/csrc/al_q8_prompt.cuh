@@ -762,8 +762,7 @@ __global__ void __launch_bounds__(32 * kQmWarps) q8_merge_kernel(const Q8AttendP
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const float e = __shfl_sync(0xffffffffu, wgt, (i + k) & 31);
-      // (weight zero: also an empty split, whose O was not written)
-      if (part + WPR * (i + k) < p.nsplit && e != 0.0f) { a.x += e * v[k].x; a.y += e * v[k].y; a.z += e * v[k].z; a.w += e * v[k].w; }
+      if (part + WPR * (i + k) < p.nsplit) q8_merge_add(a, e, v[k]);
     }
     fetch(i + kAhead);
   }

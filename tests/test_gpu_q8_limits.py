@@ -1,10 +1,11 @@
 """The 8-bit cache's operators on the GPU at their limits."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_q8 import DEV, al, check_attend, make_q, random_cache, status
+from test_gpu_q8 import DEV, TYPES, al, check_attend, host, make_q, random_cache, status
 
 pytestmark = pytest.mark.gpu
 
@@ -25,4 +26,30 @@ def test_a_window_past_the_capacity_hides_nothing(dtype, h, T):
             assert torch.equal(al().attend_q8(q, cache, on_gpu, window=window, sinks=sinks), want), (window, sinks)
     check_attend(cache, q, lengths, 7, 2 ** 31 - 1, al().attend_q8(q, cache, on_gpu, window=7, sinks=2 ** 31 - 1))
     check_attend(cache, q, lengths, C - 1, 3, al().attend_q8(q, cache, on_gpu, window=C - 1, sinks=3))
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h, T", [(1, 1), (4, 2), (1, 60), (2, 90), (1, 300)])
+def test_nan_in_a_split_without_weight(dtype, h, T):
+    """A visible NaN code in V makes its dimension NaN however far its token's score lies below the row's maximum (0 times
+    NaN is NaN), so also where warps, CTAs or key splits that hold it have no weight left; nothing else changes. Every
+    score is 0 but the first token's, about 600 binades above."""
+    C = 9000
+    cache = random_cache(7, 1, 1, C)
+    cache.k.view(torch.uint8).zero_()
+    cache.k.view(torch.uint8)[0, 0, 0, 0] = 0x7E                       # 448
+    cache.k_exp.zero_()
+    q = torch.zeros(1, 1, h, T, 128, device=DEV, dtype=TYPES[dtype])
+    q[..., 0] = 1.0
+    on_gpu = torch.tensor([C], dtype=torch.int32, device=DEV)
+    for j in (1, 31, 40, 130, 700, 4100, C - T - 1, C - T):
+        bad = cache._replace(v=cache.v.clone())
+        bad.v.view(torch.uint8)[0, 0, j, 5] = 0x7F
+        for lengths, hint in ((on_gpu, None), (on_gpu, C), (on_gpu, 3000), (on_gpu, 1), (C, None)):
+            got = host(al().attend_q8(q, bad, lengths, scale=1.0, max_length=hint))
+            base = host(al().attend_q8(q, cache, lengths, scale=1.0, max_length=hint))
+            assert np.isnan(got[..., 5]).all(), (j, hint)
+            keep = [i for i in range(128) if i != 5]
+            assert np.array_equal(got[..., keep], base[..., keep]), (j, hint)
     assert status() == 0
