@@ -145,11 +145,11 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
   const long long R = (long long)p.h * p.T;
   int rc;
   if (pl.token) {
-    if ((rc = prepare_kernel(q8_decode_kernel<T>, kQdSmem))) return rc;
+    if ((rc = prepare_kernel(q8_decode_kernel<T>, kQdSmemOf<T>))) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(pl.nsplit > 1 ? pl.nsplit : pl.cs), (unsigned)(p.B * p.G), (unsigned)((R + kQdCols - 1) / kQdCols));
     cfg.blockDim = dim3(kQdThreads, 1, 1);
-    cfg.dynamicSmemBytes = kQdSmem;
+    cfg.dynamicSmemBytes = kQdSmemOf<T>;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;

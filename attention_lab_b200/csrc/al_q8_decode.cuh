@@ -37,6 +37,12 @@ constexpr int kQdChunk = 4096;             // tokens per CTA where requests have
 constexpr int kQdStages = 2;               // ring stages per warp
 constexpr uint32_t kQdStageBytes = 2 * kQdStep * kHeadDim;           // 8 KB: K rows, then V rows
 constexpr size_t kQdSmem = kQdWarps * kQdStages * kQdStageBytes;     // 64 KB
+// 32-bit queries: steps of a warp that O accumulates before it is added to a sum in shared memory, in fp32 with rounding
+// (its lanes' own places, 4 KB a warp). The tensor cores cut each of their sums off towards zero: over 131072 tokens that
+// one CTA walks alone the output lost 2.7e-5 without this (which costs 2 %: 32 fp32 requests of 16K to 32K tokens 261 us to
+// 267). 16-bit outputs are rounded to 2e-3 in any case.
+constexpr int kQdFlush = 8;
+template <typename T> constexpr size_t kQdSmemOf = kQdSmem + (sizeof(T) == 4 ? kQdWarps * kQdCols * kHeadDim * sizeof(float) : 0);
 constexpr float kQdBias = 10.0f;           // weights run up to 2^10, so f16's normal range starts 2^-24 below the largest
 
 struct Q8AttendParams {
@@ -152,6 +158,9 @@ __device__ __forceinline__ int q8_row_token(int r, const Q8AttendParams& p) {
 // 16 bytes global -> shared, zeros when !in (nothing is read then).
 __device__ __forceinline__ void qd_copy16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void qd_sts16(uint32_t a, float4 v) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ uint4 qd_lds16(uint32_t a) {
   uint4 v;
@@ -282,6 +291,26 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
   for (int j = 0; j < 16; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f; }
   float m = -INFINITY, l = 0.0f;
   int ev_top = -128;                                     // largest V exponent met so far
+  // 32-bit queries: the sum O joins every kQdFlush steps, relative to m_sum; piece i of the lane is O's columns 4 (i & 3) ...
+  // of the row halves (i < 4: [0] and [2], else [1] and [3])
+  constexpr bool WIDE = sizeof(T) == 4;
+  const uint32_t sums = smem_addr(qd_raw) + (uint32_t)kQdSmem + (uint32_t)(warp * kQdCols * kHeadDim * 4 + lane * 16);
+  float m_sum = -INFINITY;
+  int since = 0;
+  bool summed = false;
+  auto piece = [&](int i) {
+    const int j = 4 * (i & 3), r = i >> 2;
+    return make_float4(o[j][r] + o[j][r + 2], o[j + 1][r] + o[j + 1][r + 2], o[j + 2][r] + o[j + 2][r + 2], o[j + 3][r] + o[j + 3][r + 2]);
+  };
+  auto plus_sum = [&](int i, float fa) {                 // piece i and what the sum holds of it
+    float4 v = piece(i);
+    if (summed) {
+      const uint4 x = qd_lds16(sums + (uint32_t)i * 512u);
+      v.x = fmaf(__uint_as_float(x.x), fa, v.x); v.y = fmaf(__uint_as_float(x.y), fa, v.y);
+      v.z = fmaf(__uint_as_float(x.z), fa, v.z); v.w = fmaf(__uint_as_float(x.w), fa, v.w);
+    }
+    return v;
+  };
 
   // Fragment addresses: K row of n index g8 is (g8 >> 1) + 4 (g8 & 1), its chunks t4 and t4 + 4; V row of k-slot 2t + u
   // is t4 + 4u, its chunk (the n index g8) (g8 >> 1) + 4 (g8 & 1).
@@ -412,22 +441,31 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
         mma_f16_16816(o[4 * w + 3], pa[ks][0], pa[ks][1], pa[ks][2], pa[ks][3], q8_decode_hi(xh), q8_decode_hi(yh));
       }
     }
+    if (WIDE && ++since == kQdFlush) {
+      const float fa = m_sum == m ? 1.0f : q8_ex2(m_sum - m);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 v = plus_sum(i, fa);
+        qd_sts16(sums + (uint32_t)i * 512u, v);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f; }
+      m_sum = m;
+      since = 0;
+      summed = true;
+    }
   }
   cp_async_wait<0>();
   __syncthreads();                                          // the rings give way to the partial results
 
-  // The warps' partials in shared memory: thread holds column g8, dimensions 16 t + j (o[j][0] + o[j][2]) and 64 + 16 t + j.
-  // Piece x (4 dimensions) of column c lies at x ^ (x >> 3 & 1) ^ 2 (c & 1): no bank twice.
+  // The warps' partials in shared memory: thread holds column g8, dimensions 16 t + j (o[j][0] + o[j][2]: pieces 0-3) and
+  // 64 + 16 t + j (pieces 4-7). Piece x (4 dimensions) of column c lies at x ^ (x >> 3 & 1) ^ 2 (c & 1): no bank twice.
   auto place = [](int c, int x) { return x ^ ((x >> 3) & 1) ^ ((c & 1) << 1); };
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
+  const float fa = m_sum == m ? 1.0f : q8_ex2(m_sum - m);
 #pragma unroll
-  for (int j = 0; j < 16; j += 4) {
-    s_o[warp][g8][place(g8, 4 * t4 + j / 4)] =
-        make_float4(o[j][0] + o[j][2], o[j + 1][0] + o[j + 1][2], o[j + 2][0] + o[j + 2][2], o[j + 3][0] + o[j + 3][2]);
-    s_o[warp][g8][place(g8, 16 + 4 * t4 + j / 4)] =
-        make_float4(o[j][1] + o[j][3], o[j + 1][1] + o[j + 1][3], o[j + 2][1] + o[j + 2][3], o[j + 3][1] + o[j + 3][3]);
-  }
+  for (int i = 0; i < 8; ++i) s_o[warp][g8][place(g8, 16 * (i >> 2) + 4 * t4 + (i & 3))] = WIDE ? plus_sum(i, fa) : piece(i);
   if (t4 == 0) { s_m[warp][g8] = m; s_l[warp][g8] = l; }
   __syncwarp();
   if (clustered) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");   // every CTA of the cluster runs

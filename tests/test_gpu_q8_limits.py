@@ -53,3 +53,22 @@ def test_nan_in_a_split_without_weight(dtype, h, T):
             keep = [i for i in range(128) if i != 5]
             assert np.array_equal(got[..., keep], base[..., keep]), (j, hint)
     assert status() == 0
+
+
+def test_fp32_single_tokens_do_not_drift():
+    """As for prompts: with every value one the output is one, and what the tensor cores cut off must not add up over a long
+    context that one CTA walks alone (as many segments as SMs, so no split). Between two additions to the fp32 sum a warp
+    takes 16 tensor-core sums, each cutting off at most 2^-23 of what it holds; rounded additions average out."""
+    B, G, n = 19, 8, 131072
+    cache = al().Q8Cache.empty(B, G, n, DEV)
+    for b in range(B):
+        x = torch.randint(0, 127, (G, n, 128), device=DEV, dtype=torch.uint8, generator=torch.Generator(DEV).manual_seed(b))
+        cache.k.view(torch.uint8)[b] = x | (x << 7)                     # any finite code, the lowest bit as its sign
+    cache.k_exp.fill_(-14)                                              # scores of the order of one
+    cache.v.view(torch.uint8).fill_(0x78)                               # 256
+    cache.v_exp.fill_(-8)
+    q = make_q(33, B, G, 2, 1, "f32")
+    out = al().attend_q8(q, cache, n)
+    drift = float((out.double() - 1).mean())
+    assert abs(drift) <= 16 * 2 ** -23, drift
+    assert status() == 0
