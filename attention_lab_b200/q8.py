@@ -77,8 +77,10 @@ def rotary_table(length: int, rotary_dim: int = HEAD_DIM, *, base: float = 10000
         {"type": "linear", "factor": s}      every position divided by s
         {"type": "ntk", "factor": s}         base times s^(rotary_dim / (rotary_dim - 2))
         {"type": "yarn", "factor": s, "original": n}   frequencies that turn more than `fast` (32) times in the original
-            context of n positions kept, those that turn less than `slow` (1) times divided by s, a ramp between; table
-            entries times `amplitude` (default 0.1 ln s + 1)
+            context of n positions kept, those that turn less than `slow` (1) times divided by s, between them a ramp that
+            is linear in the pair's index, from the whole index below the one of `fast` turns to the one above that of
+            `slow` (checkpoints trained with YaRN run with this ramp, not with the one linear in turns); table entries
+            times `amplitude` (default 0.1 ln s + 1, and 1 for s <= 1)
     """
     length, rot = int(length), int(rotary_dim)
     if length < 1 or rot < 2 or rot % 2:
@@ -106,12 +108,15 @@ def rotary_table(length: int, rotary_dim: int = HEAD_DIM, *, base: float = 10000
         if "original" not in scaling:
             raise ValueError("yarn scaling needs the original context length")
         fast, slow = float(scaling.pop("fast", 32.0)), float(scaling.pop("slow", 1.0))
-        if not fast > slow:
-            raise ValueError("yarn scaling needs fast > slow")
-        turns = freq * float(scaling.pop("original")) / (2 * math.pi)
-        keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
+        original = float(scaling.pop("original"))
+        if not (fast > slow > 0 and original > 0 and base > 1):
+            raise ValueError("yarn scaling needs fast > slow > 0, original > 0 and base > 1")
+        # pair i turns original base^(-2i/rot) / (2 pi) times: the index of so many turns, not rounded
+        index = lambda turns: rot * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))
+        first, last = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rot - 1)
+        keep = 1.0 - ((i - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
         freq = freq * keep + freq / s * (1.0 - keep)
-        amp *= float(scaling.pop("amplitude", 0.1 * math.log(s) + 1.0))
+        amp *= float(scaling.pop("amplitude", 0.1 * math.log(s) + 1.0 if s > 1 else 1.0))
     elif kind not in ("none", "ntk"):
         raise ValueError(f"unknown scaling type {kind!r}")
     if scaling:

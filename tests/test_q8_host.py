@@ -1,0 +1,48 @@
+"""The 8-bit cache's host side without a GPU: rotary tables as checkpoints use them."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from attention_lab_b200 import q8
+
+transformers = pytest.importorskip("transformers")
+
+
+def model_rotary(head_dim, length, base, **rope):
+    """The rotary module of a Qwen3 configuration."""
+    from transformers.models.qwen3.modeling_qwen3 import Qwen3RotaryEmbedding
+    cfg = transformers.Qwen3Config(hidden_size=4 * head_dim, num_attention_heads=4, num_key_value_heads=2,
+                                   head_dim=head_dim, max_position_embeddings=length)
+    cfg.rope_parameters = dict(rope_theta=base, **rope)
+    return Qwen3RotaryEmbedding(cfg)
+
+
+@pytest.mark.parametrize("base, rot, factor, original, turns", [
+    (1e6, 128, 4.0, 32768, {}), (1e4, 64, 8.0, 2048, {}), (1e6, 96, 2.0, 4096, {}), (5e5, 128, 16.0, 8192, {}),
+    (1e6, 128, 40.0, 4096, {"fast": 48.0, "slow": 2.0}), (1e4, 128, 4.0, 20, {})])
+def test_yarn_is_the_table_checkpoints_use(base, rot, factor, original, turns):
+    """Every pair, the ramp's middle among them. transformers computes its frequencies in 32 bits (a power and two
+    products: 2^-20 relative is ample), so tables are compared where that moves an angle by less than 1e-4."""
+    names = {"fast": "beta_fast", "slow": "beta_slow"}
+    theirs = model_rotary(rot, int(factor * original), base, rope_type="yarn", factor=factor,
+                          original_max_position_embeddings=original, **{names[k]: v for k, v in turns.items()})
+    ours = q8.rotary_table(100, rot, base=base, device="cpu",
+                           scaling=dict(type="yarn", factor=factor, original=original, **turns)).double()
+    ang = torch.arange(100, dtype=torch.float64)[:, None] * theirs.inv_freq.double()
+    amp = theirs.attention_scaling
+    assert amp == pytest.approx(0.1 * math.log(factor) + 1)
+    assert (ours[:, :rot // 2] - amp * ang.cos()).abs().max() < 2e-4
+    assert (ours[:, rot // 2:] - amp * ang.sin()).abs().max() < 2e-4
+    freq = torch.atan2(ours[1, rot // 2:], ours[1, :rot // 2])           # of position 1: the frequencies themselves
+    assert ((freq - theirs.inv_freq.double()) / theirs.inv_freq.double()).abs()[freq > 1e-3].max() < 1e-3
+
+
+@pytest.mark.parametrize("bad", [dict(original=0), dict(original=-5), dict(slow=0.0), dict(base=1.0)])
+def test_yarn_refuses(bad):
+    bad = dict(bad)
+    base = bad.pop("base", 1e4)
+    with pytest.raises(ValueError):
+        q8.rotary_table(8, 16, base=base, scaling={"type": "yarn", "factor": 2, "original": 64, **bad}, device="cpu")
