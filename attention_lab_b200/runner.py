@@ -513,8 +513,12 @@ def make_cache(model, capacity: int, *, with_index: bool, index_dim: int = 32, b
 
 
 def model_rotary_table(model, length: int, device=None) -> torch.Tensor:
-    """The model's own rotary frequencies and scaling as a q8 rotary table [length, head_dim] (half layout)."""
+    """The model's own rotary frequencies and scaling as a q8 rotary table [length, head_dim] (half layout). Rope types
+    whose frequencies change with the length a forward has reached have no one table and are refused."""
     rot = model.model.rotary_emb
+    kind = getattr(rot, "rope_type", "default")
+    if kind in ("dynamic", "longrope"):
+        raise ValueError(f"rope type {kind!r}: its frequencies change with the length, a rotary table holds one set")
     device = rot.inv_freq.device if device is None else device
     return q8.rotary_table(length, 2 * rot.inv_freq.numel(), frequencies=rot.inv_freq,
                            amplitude=float(getattr(rot, "attention_scaling", 1.0)), device=device)

@@ -46,3 +46,27 @@ def test_yarn_refuses(bad):
     base = bad.pop("base", 1e4)
     with pytest.raises(ValueError):
         q8.rotary_table(8, 16, base=base, scaling={"type": "yarn", "factor": 2, "original": 64, **bad}, device="cpu")
+
+
+@pytest.mark.parametrize("rope", [dict(rope_type="dynamic", factor=2.0),
+                                  dict(rope_type="longrope", factor=4.0, short_factor=[1.0] * 64, long_factor=[2.0] * 64,
+                                       original_max_position_embeddings=64)])
+def test_frequencies_that_change_with_the_length_are_refused(rope):
+    from types import SimpleNamespace
+    from attention_lab_b200 import runner
+    model = SimpleNamespace(model=SimpleNamespace(rotary_emb=model_rotary(128, 256, 1e6, **rope)))
+    with pytest.raises(ValueError, match=rope["rope_type"]):
+        runner.model_rotary_table(model, 100)
+
+
+@pytest.mark.parametrize("rope", [dict(rope_type="default"), dict(rope_type="linear", factor=2.0),
+                                  dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64),
+                                  dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                                       original_max_position_embeddings=64)])
+def test_a_models_fixed_frequencies_become_its_table(rope):
+    from types import SimpleNamespace
+    from attention_lab_b200 import runner
+    rot = model_rotary(128, 256, 1e6, **rope)
+    table = runner.model_rotary_table(SimpleNamespace(model=SimpleNamespace(rotary_emb=rot)), 100).double()
+    ang = torch.arange(100, dtype=torch.float64)[:, None] * rot.inv_freq.double()
+    assert (table - torch.cat([ang.cos(), ang.sin()], 1) * rot.attention_scaling).abs().max() < 2 ** -23
