@@ -25,18 +25,27 @@ from typing import NamedTuple
 
 import torch
 
-try:
-    from . import _q8_bind as _bind   # argument checks, outputs and the C-ABI call (csrc/bind_q8.cpp)
-except ImportError as _e:
-    class _NotBuilt:
-        def __init__(self, why):
-            self.why = why
 
-        def __getattr__(self, name):
-            raise RuntimeError(f"the 8-bit cache's binding is not built ({self.why}): run `python -m "
-                               "attention_lab_b200.build` (these operators have no fallback)")
+class _Binding:
+    """The operators' compiled binding (csrc/bind_q8.cpp: argument checks, outputs and the C-ABI call), loaded with the
+    CUDA library it is linked to at the first call of an operator: importing this module maps neither."""
 
-    _bind = _NotBuilt(_e)
+    NAMES = ("rotary_embed", "append_q8", "read_q8", "attend_q8")
+
+    def __getattr__(self, name):                 # reached until the functions below are attributes
+        if name not in self.NAMES:
+            raise AttributeError(name)
+        try:
+            from . import _q8_bind
+        except ImportError as e:
+            raise RuntimeError(f"the 8-bit cache's binding is not built ({e}): run `python -m attention_lab_b200.build` "
+                               "(these operators have no fallback)") from e
+        for n in self.NAMES:
+            setattr(self, n, getattr(_q8_bind, n))
+        return getattr(self, name)
+
+
+_bind = _Binding()
 
 BLOCK = 64                     # tokens that share one exponent
 HEAD_DIM = 128

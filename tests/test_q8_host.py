@@ -70,3 +70,27 @@ def test_a_models_fixed_frequencies_become_its_table(rope):
     table = runner.model_rotary_table(SimpleNamespace(model=SimpleNamespace(rotary_emb=rot)), 100).double()
     ang = torch.arange(100, dtype=torch.float64)[:, None] * rot.inv_freq.double()
     assert (table - torch.cat([ang.cos(), ang.sin()], 1) * rot.attention_scaling).abs().max() < 2 ** -23
+
+
+def test_importing_the_package_maps_no_native_library():
+    """Host-side users of the package (selection rules, tables, a CPU measurement) do not load the CUDA library; the first
+    operator does."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+import attention_lab_b200 as al
+from attention_lab_b200 import q8, runner, selection
+al.rotary_table(8, 128, device="cpu"), al.Q8Cache.empty(1, 1, 8, "cpu")
+maps = lambda: [l for l in open("/proc/self/maps") if "attention_lab_b200" in l and ".so" in l]
+assert not maps(), maps()[:2]
+x = torch.zeros(1, 1, 3, 128)
+try:
+    al.rotary_embed(x, None, torch.zeros(8, 128), 0)
+except ValueError as e:
+    assert "CUDA" in str(e)
+assert maps()
+"""
+    res = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
