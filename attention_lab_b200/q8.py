@@ -16,7 +16,8 @@ ragged batch of prompts is padded on the left). A device length outside [0, C] i
 (`_lib.device_status()`); an int is checked here.
 
 As in `ops`: tensors live on one CUDA device, float32 or bfloat16, head_dim 128, work goes to the current stream,
-nothing synchronises, ValueError for shapes, dtypes and ranges.
+nothing synchronises, ValueError for shapes, dtypes and ranges. rotary_embed takes part in autograd; the cache holds
+codes, through which no gradient passes: append_q8 and attend_q8 return tensors without one.
 """
 from __future__ import annotations
 
@@ -134,12 +135,40 @@ def rotary_table(length: int, rotary_dim: int = HEAD_DIM, *, base: float = 10000
     return torch.cat([ang.cos() * amp, ang.sin() * amp], dim=1).float().contiguous()
 
 
+class _Rotation(torch.autograd.Function):
+    """The rotation as an operation of autograd: a pair's gradient is the output's, turned the other way."""
+
+    @staticmethod
+    def forward(ctx, q, k, table, positions, layout, inverse):
+        at = positions if isinstance(positions, torch.Tensor) else None
+        ctx.save_for_backward(table, at)
+        ctx.start, ctx.layout, ctx.inverse = (positions if at is None else None), layout, inverse
+        return _bind.rotary_embed(q, k, table, positions, layout, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        table, at = ctx.saved_tensors
+        turn = lambda x, y: _rotate(x, y, table, ctx.start if at is None else at, ctx.layout, not ctx.inverse)
+        if ctx.needs_input_grad[0]:
+            gq, gk = turn(dq, dk if ctx.needs_input_grad[1] else None)
+        else:
+            gq, gk = None, turn(dk, None)[0]
+        return gq, gk, None, None, None, None
+
+
+def _rotate(q, k, table, positions, layout, inverse):
+    if torch.is_grad_enabled() and (getattr(q, "requires_grad", False) or getattr(k, "requires_grad", False)):
+        return _Rotation.apply(q, k, table, positions, layout, inverse)
+    return _bind.rotary_embed(q, k, table, positions, layout, inverse)
+
+
 def rotary_embed(q: torch.Tensor, k, table: torch.Tensor, positions, *, layout: str = "half", inverse: bool = False):
     """q [B,H,T,d] and k [B,G,T,d] (or None) rotated to their positions, in one launch: pairs (a, b) become
     (a c - b s, b c + a s) in float32, rounded once; dimensions past the table's rotary_dim are copied. `positions` is
     an int (row t at positions + t) or int64 [B,T] (or [T]); negative ones are padding (zeros), one past the table gives
-    zeros and error bit 4. `inverse` rotates back: the gradient of the forward rotation. Returns (q', k')."""
-    return _bind.rotary_embed(q, k, table, positions, _layout(layout), inverse)
+    zeros and error bit 4. `inverse` turns the other way (s becomes -s): the gradient of the forward rotation, which
+    autograd takes through q and k by itself (the table has none). Returns (q', k')."""
+    return _rotate(q, k, table, positions, _layout(layout), bool(inverse))
 
 
 def append_q8(cache, lengths, k_new: torch.Tensor, v_new: torch.Tensor, *, q=None, table=None, layout: str = "half"):

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_q8 import DEV, TYPES, al, check_attend, host, make_q, random_cache, status
+from test_gpu_q8 import DEV, TYPES, al, check_attend, gen, host, make_q, random_cache, status
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,50 @@ def test_fp32_single_tokens_do_not_drift():
     drift = float((out.double() - 1).mean())
     assert abs(drift) <= 16 * 2 ** -23, drift
     assert status() == 0
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_takes_part_in_autograd(layout, dtype, inverse):
+    """Gradients through the operator are its other direction applied to the outputs' gradients, for q and k, alone or
+    together, strided or expanded; where neither asks for one, nothing is recorded."""
+    g = gen(12)
+    table = al().rotary_table(60, 64, device=DEV, scaling={"type": "yarn", "factor": 2, "original": 30})
+    pos = torch.randint(0, 60, (2, 7), generator=g).to(DEV)
+    pos[0, 0] = -1
+    q = torch.randn(2, 7, 5, 128, generator=g).to(TYPES[dtype]).to(DEV).transpose(1, 2).requires_grad_()
+    k = torch.randn(2, 3, 7, 128, generator=g).to(TYPES[dtype]).to(DEV).requires_grad_()
+    wq, wk = torch.randn(2, 5, 7, 128, generator=g).to(DEV), torch.randn(2, 3, 7, 128, generator=g).to(DEV)
+    wq, wk = wq.to(TYPES[dtype]), wk.to(TYPES[dtype])
+    kw = dict(layout=layout, inverse=inverse)
+    back = dict(layout=layout, inverse=not inverse)
+    plain = al().rotary_embed(q.detach(), k.detach(), table, pos, **kw)
+    qo, ko = al().rotary_embed(q, k, table, pos, **kw)
+    assert torch.equal(qo, plain[0]) and torch.equal(ko, plain[1])
+    gq, gk = torch.autograd.grad([qo, ko], [q, k], [wq, wk])
+    want = al().rotary_embed(wq, wk, table, pos, **back)
+    assert torch.equal(gq, want[0]) and torch.equal(gk, want[1])
+    assert torch.all(gq[0, :, 0] == 0)
+    # one of the two; an expanded gradient (that of a sum); q alone
+    only = torch.autograd.grad(al().rotary_embed(q.detach(), k, table, pos, **kw)[1].sum(), k)[0]
+    assert torch.equal(only, al().rotary_embed(torch.ones_like(wk), None, table, pos, **back)[0])
+    alone, none = al().rotary_embed(q, None, table, pos, **kw)
+    assert none is None and torch.equal(torch.autograd.grad(alone, q, wq)[0], want[0])
+    with torch.no_grad():
+        assert not al().rotary_embed(q, k, table, pos, **kw)[0].requires_grad
+    assert not plain[0].requires_grad and status() == 0
+
+
+def test_rotary_gradient_against_differences_through_autograd():
+    """Central differences of a loss through the operator; the map is linear, so a step of one has no truncation error."""
+    g = gen(3)
+    table = al().rotary_table(40, 96, device=DEV)
+    x = torch.randn(1, 2, 2, 128, generator=g).to(DEV).requires_grad_()
+    w = torch.randn(1, 2, 2, 128, generator=g).to(DEV)
+    loss = lambda y: (al().rotary_embed(y, None, table, 9)[0].double() * w.double()).sum(dim=(1, 2, 3))
+    loss(x).sum().backward()
+    probe = torch.eye(512, device=DEV).view(512, 1, 2, 2, 128)
+    with torch.no_grad():
+        diff = torch.stack([(loss(x + p) - loss(x - p))[0] / 2 for p in probe])
+    assert float((diff - x.grad.double().view(-1)).abs().max()) < 64 * 2 ** -23
