@@ -172,13 +172,17 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p = THPVariable_Unpack(a[3]);
     TORCH_CHECK_VALUE(p.scalar_type() == at::kLong, "positions must be int64");
     on_device(p, dev);
-    if (p.dim() < 2 || (p.dim() == 2 && p.size(0) == 1 && B != 1)) p = p.expand({B, T});
-    TORCH_CHECK_VALUE(p.dim() == 2 && p.size(0) == B && p.size(1) == T, "positions must be [B,T] = [", B, ",", T, "], got ", p.sizes());
+    // [B,T], [T] or [1,T], or a single position for every row
+    const int64_t pd = p.dim();
+    TORCH_CHECK_VALUE(p.numel() == 1 || ((pd == 1 || (pd == 2 && (p.size(0) == B || p.size(0) == 1))) && p.size(pd - 1) == T),
+                      "positions must be [B,T] = [", B, ",", T, "], got ", p.sizes());
+    if (p.numel() == 1) p = p.reshape({});
+    p = p.expand({B, T});
     pos = p.data_ptr<int64_t>();
     pst[0] = p.stride(0); pst[1] = p.stride(1);
   } else {
     start = integer(a[3], "positions");
-    TORCH_CHECK_VALUE(start >= 0 && start + T <= t.rows, "positions [", start, ", ", start + T, ") outside the table's ", t.rows, " rows");
+    TORCH_CHECK_VALUE(start >= 0 && start <= (int64_t)t.rows - T, T, " positions from ", start, " on lie outside the table's ", t.rows, " rows");
   }
   at::Tensor out = at::empty({B, H, T, d}, q.options());
   check(al_rotary(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), H, Hk ? k.data_ptr() : nullptr, ks[0], ks[1], ks[2],

@@ -119,3 +119,15 @@ def test_rotary_gradient_against_differences_through_autograd():
     with torch.no_grad():
         diff = torch.stack([(loss(x + p) - loss(x - p))[0] / 2 for p in probe])
     assert float((diff - x.grad.double().view(-1)).abs().max()) < 64 * 2 ** -23
+
+
+def test_rotary_positions_are_checked():
+    table = al().rotary_table(10, 128, device=DEV)
+    q = torch.randn(2, 2, 3, 128, device=DEV)
+    for at in (2 ** 63 - 1, 2 ** 63 - 3, 2 ** 62, 8, -1):
+        with pytest.raises(ValueError, match="positions"):
+            al().rotary_embed(q, None, table, at)
+    for shape in ((4,), (2, 4), (3, 3), (2, 3, 1), (3, 1), (2, 1), (0,)):
+        with pytest.raises(ValueError, match="positions"):
+            al().rotary_embed(q, None, table, torch.zeros(shape, dtype=torch.int64, device=DEV))
+    assert al().rotary_embed(q, None, table, 7)[0].shape == q.shape and status() == 0
