@@ -32,17 +32,14 @@ const at::Tensor& tensor(PyObject* o, const char* what) {
   return THPVariable_Unpack(o);
 }
 int64_t integer(PyObject* o, const char* what) {
-  if (PyLong_CheckExact(o)) {
-    const long long v = PyLong_AsLongLong(o);
-    if (v == -1 && PyErr_Occurred()) throw python_error();
-    return v;
-  }
+  TORCH_CHECK_TYPE(PyIndex_Check(o), what, " must be an integer, got ", Py_TYPE(o)->tp_name);
   PyObject* i = PyNumber_Index(o);
   if (!i) throw python_error();
-  const long long v = PyLong_AsLongLong(i);
+  int overflow = 0;
+  const long long v = PyLong_AsLongLongAndOverflow(i, &overflow);
   Py_DECREF(i);
   if (v == -1 && PyErr_Occurred()) throw python_error();
-  (void)what;
+  TORCH_CHECK_VALUE(overflow == 0, what, " is out of range");
   return v;
 }
 // An integer that the C ABI takes as int: out of its range is out of every range.
@@ -273,6 +270,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int most = !len.ptr ? len.all : a[6] == Py_None ? c.C : small(a[6], "max_length");
   double scale = 1.0 / std::sqrt((double)c.d);
   if (a[5] != Py_None) {
+    TORCH_CHECK_TYPE(PyNumber_Check(a[5]), "scale must be a number, got ", Py_TYPE(a[5])->tp_name);
     scale = PyFloat_AsDouble(a[5]);
     if (scale == -1.0 && PyErr_Occurred()) throw python_error();
   }

@@ -131,3 +131,21 @@ def test_rotary_positions_are_checked():
         with pytest.raises(ValueError, match="positions"):
             al().rotary_embed(q, None, table, torch.zeros(shape, dtype=torch.int64, device=DEV))
     assert al().rotary_embed(q, None, table, 7)[0].shape == q.shape and status() == 0
+
+
+def test_a_wrong_type_is_reported_by_name():
+    c = al().Q8Cache.empty(1, 1, 64, DEV)
+    x = torch.randn(1, 1, 3, 128, device=DEV)
+    q = x[:, :, None]
+    for call, name in ((lambda: al().append_q8(c, 3.5, x, x), "lengths"), (lambda: al().read_q8(c, "0", 3), "lo"),
+                       (lambda: al().read_q8(c, 0, None), "hi"), (lambda: al().attend_q8(q, c, 3, window=1.5), "window"),
+                       (lambda: al().attend_q8(q, c, 3, sinks=[]), "sinks"),
+                       (lambda: al().attend_q8(q, c, torch.tensor([3], dtype=torch.int32, device=DEV), max_length="x"), "max_length"),
+                       (lambda: al().attend_q8(q, c, 3, scale="x"), "scale"),
+                       (lambda: al().rotary_embed(x, None, al().rotary_table(8, device=DEV), 0.5), "positions")):
+        with pytest.raises(TypeError, match=name):
+            call()
+    for call, name in ((lambda: al().append_q8(c, 2 ** 70, x, x), "lengths"), (lambda: al().read_q8(c, -2 ** 70, 3), "lo"),
+                       (lambda: al().attend_q8(q, c, 3, window=2 ** 31), "window"), (lambda: al().attend_q8(q, c, 3, sinks=2 ** 64), "sinks")):
+        with pytest.raises(ValueError, match=name):
+            call()
