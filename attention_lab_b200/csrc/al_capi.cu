@@ -4,7 +4,9 @@
 #include <cstdio>
 #include <cstring>
 #include <algorithm>
+#include <map>
 #include <mutex>
+#include <tuple>
 #include <unordered_map>
 
 #include "al_context.cuh"
@@ -23,6 +25,7 @@ thread_local char g_msg[1024] = "";
 std::mutex g_mu;
 DeviceInfo g_dev[64];
 std::unordered_map<unsigned long long, int> g_smem_set;   // (kernel, device) -> dynamic smem bytes allowed
+std::map<std::tuple<const void*, int, size_t, int>, bool> g_cluster_ok;   // kernel, cluster size, smem, device -> schedulable
 }  // namespace
 
 namespace al {
@@ -77,13 +80,29 @@ int prepare_kernel_ptr(const void* kernel, size_t smem) {
   return AL_OK;
 }
 
+int cluster_schedulable(const void* kernel, const cudaLaunchConfig_t& cfg, int cs, bool* ok) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const auto key = std::make_tuple(kernel, cs, cfg.dynamicSmemBytes, dev);
+  {
+    std::lock_guard<std::mutex> lk(g_mu);
+    auto it = g_cluster_ok.find(key);
+    if (it != g_cluster_ok.end()) { *ok = it->second; return AL_OK; }
+  }
+  int n = 0;
+  cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
+  *ok = n > 0;
+  std::lock_guard<std::mutex> lk(g_mu);
+  g_cluster_ok[key] = *ok;
+  return AL_OK;
+}
+
 }  // namespace al
 
 namespace {
 
 constexpr int kMaxRanks = 64;   // ranks of one exchange (the flag array of a channel holds one word each)
-
-std::unordered_map<unsigned long long, int> g_cluster_ok;   // (kernel, cs, smem, device) -> schedulable
 
 template <typename K, typename... P>
 int launch(K kernel, dim3 grid, int cs, size_t smem, void* stream, const P&... p) {
@@ -102,24 +121,8 @@ int launch(K kernel, dim3 grid, int cs, size_t smem, void* stream, const P&... p
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cs > 1) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const unsigned long long key = (reinterpret_cast<unsigned long long>(reinterpret_cast<const void*>(kernel)) << 16) ^
-                                   ((unsigned long long)cs << 40) ^ ((unsigned long long)smem << 8) ^ (unsigned long long)dev;
-    int ok = -1;
-    {
-      std::lock_guard<std::mutex> lk(g_mu);
-      auto it = g_cluster_ok.find(key);
-      if (it != g_cluster_ok.end()) ok = it->second;
-    }
-    if (ok < 0) {
-      int n = 0;
-      cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
-      ok = n > 0 ? 1 : 0;
-      std::lock_guard<std::mutex> lk(g_mu);
-      g_cluster_ok[key] = ok;
-    }
+    bool ok = false;
+    if ((rc = cluster_schedulable(reinterpret_cast<const void*>(kernel), cfg, cs, &ok))) return rc;
     if (!ok) return fail(AL_EUNSUPPORTED, "a cluster of %d CTAs with %zu bytes of shared memory cannot be scheduled", cs, smem);
   }
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p...);

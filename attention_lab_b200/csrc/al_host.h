@@ -20,11 +20,28 @@ int cuda_fail(cudaError_t e, const char* where);
 int device_info(DeviceInfo** out);
 // Allow `smem` bytes of dynamic shared memory and non-portable cluster sizes (set once per kernel and device).
 int prepare_kernel_ptr(const void* kernel, size_t smem);
+// Whether the current device can schedule a cluster of `cs` CTAs of the kernel as cfg launches it (asked once per kernel,
+// size, shared memory and device).
+int cluster_schedulable(const void* kernel, const cudaLaunchConfig_t& cfg, int cs, bool* ok);
 #pragma GCC visibility pop
 
 template <typename K>
 int prepare_kernel(K kernel, size_t smem) {
   return prepare_kernel_ptr(reinterpret_cast<const void*>(kernel), smem);
+}
+
+// The largest cluster size of cs, cs / 2, ..., 1 (cs a power of two) for which fits(size, &ok) says ok, into *out; a size
+// of one needs no asking. fits returns a status code, and a failing one ends the search.
+template <typename F>
+int fitting_cluster(int cs, F&& fits, int* out) {
+  for (; cs > 1; cs >>= 1) {
+    bool ok = false;
+    const int rc = fits(cs, &ok);
+    if (rc != AL_OK) return rc;
+    if (ok) break;
+  }
+  *out = cs;
+  return AL_OK;
 }
 
 inline int plain_launch_check(const char* what) {

@@ -147,17 +147,23 @@ int q8_launch_attend(const Q8AttendParams& p, const Q8Plan& pl, void* stream) {
   if (pl.token) {
     if ((rc = prepare_kernel(q8_decode_kernel<T>, kQdSmemOf<T>))) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(pl.nsplit > 1 ? pl.nsplit : pl.cs), (unsigned)(p.B * p.G), (unsigned)((R + kQdCols - 1) / kQdCols));
     cfg.blockDim = dim3(kQdThreads, 1, 1);
     cfg.dynamicSmemBytes = kQdSmemOf<T>;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)pl.cs;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pl.cs > 1 ? 1 : 0;
+    auto shape = [&](int cs) {                         // any power of two will do: the CTAs of a cluster interleave
+      cfg.gridDim = dim3((unsigned)(pl.nsplit > 1 ? pl.nsplit : cs), (unsigned)(p.B * p.G), (unsigned)((R + kQdCols - 1) / kQdCols));
+      attr[0].val.clusterDim = {(unsigned)cs, 1, 1};
+      cfg.numAttrs = cs > 1 ? 1 : 0;
+    };
+    int cs = 1;
+    if ((rc = fitting_cluster(pl.cs, [&](int n, bool* ok) {
+           shape(n);
+           return cluster_schedulable(reinterpret_cast<const void*>(q8_decode_kernel<T>), cfg, n, ok);
+         }, &cs))) return rc;
+    shape(cs);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, q8_decode_kernel<T>, p);
     if (e != cudaSuccess) return cuda_fail(e, "q8_decode_kernel");
   } else {

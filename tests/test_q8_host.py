@@ -94,3 +94,33 @@ assert maps()
 """
     res = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True)
     assert res.returncode == 0, res.stderr
+
+
+def test_a_cluster_that_cannot_be_scheduled_is_halved(tmp_path):
+    """The token kernel's launch asks for clusters of up to 16; where the device schedules smaller ones only, the largest of
+    those is taken, and a failing question ends the launch with its status."""
+    import os
+    import subprocess
+    from pathlib import Path
+    from attention_lab_b200 import build
+    src = tmp_path / "clusters.cpp"
+    src.write_text('''
+#include <cstdio>
+#include "al_host.h"
+int main() {
+  for (int want = 1; want <= 16; want *= 2)
+    for (int most = 1; most <= 16; most *= 2) {
+      int out = -1, asked = 0;
+      const int rc = al::fitting_cluster(want, [&](int cs, bool* ok) { ++asked; *ok = cs <= most; return AL_OK; }, &out);
+      if (rc != AL_OK || out != (want < most ? want : most)) return std::printf("%d of %d: %d\\n", want, most, out), 1;
+      if (want == 1 && asked) return 2;
+    }
+  int out = -1;
+  return al::fitting_cluster(8, [](int, bool*) { return AL_ECUDA; }, &out) == AL_ECUDA && out == -1 ? 0 : 3;
+}
+''')
+    cuda = Path(os.path.realpath(build.nvcc())).parents[1]
+    exe = tmp_path / "clusters"
+    subprocess.run(["g++", "-std=c++17", "-I", str(build.SRC), "-I", str(cuda / "include"), str(src), "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stdout
