@@ -5,12 +5,15 @@
 
 One nvcc compilation per csrc/*.cu (al_capi.cu: the sparse-decode path, al_q8.cu: the 8-bit cache; each includes its
 kernel headers), run side by side, then one link; static CUDA runtime, position independent code. An object is compiled
-again when its source, a header or this file is newer. `--verbose` adds `-Xptxas -v` (registers, spills and shared memory per kernel).
+again when its source, a header or this file is newer, or when its compiler line, torch or the Python ABI is another than
+it was built with (kept beside it, and for the whole in _built.stamp). `--verbose` adds `-Xptxas -v` (registers, spills and shared memory per kernel).
 """
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
 import importlib.util
+import json
 import os
 import re
 import shutil
@@ -24,6 +27,7 @@ SRC = PKG / "csrc"
 LIB = PKG / "libattention_lab_b200.so"
 BIND = PKG / "_q8_bind.so"
 OBJ = PKG / "_build"
+STAMP = PKG / "_built.stamp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -35,11 +39,24 @@ def nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(SRC.glob("*.cu")) + sorted(SRC.glob("*.cpp")) + sorted(SRC.glob("*.cuh")) + sorted(SRC.glob("*.h")) + [PKG.parent / "include" / "attention_lab_b200.h"]
+    return [*sorted(f for pattern in ("*.cu", "*.cpp", "*.cuh", "*.h") for f in SRC.glob(pattern)),
+            PKG.parent / "include" / "attention_lab_b200.h", PKG / "build.py"]
+
+
+def made_with(commands) -> str:
+    """What built files depend on besides their sources, wherever the tree lies."""
+    return json.dumps({"torch": importlib.metadata.version("torch"), "abi": sysconfig.get_config_var("SOABI"),
+                       "commands": commands}, indent=0).replace(str(PKG.parent), ".")
+
+
+def stamp() -> str:
+    return made_with([command(OBJ / (src.stem + ".o")) for src, command in compilations().items()]
+                     + [link_library([]), link_bind(OBJ / "bind_q8.o")])
 
 
 def up_to_date() -> bool:
-    return all(out.exists() and all(out.stat().st_mtime >= s.stat().st_mtime for s in sources()) for out in (LIB, BIND))
+    return (all(out.exists() and all(out.stat().st_mtime >= s.stat().st_mtime for s in sources()) for out in (LIB, BIND))
+            and STAMP.exists() and STAMP.read_text() == stamp())
 
 
 def included(src: Path) -> set[Path]:
@@ -72,27 +89,38 @@ def link_bind(obj: Path) -> list[str]:
             "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-o", str(BIND) + ".tmp"]
 
 
+def compilations() -> dict:
+    """Source -> the compiler line that makes its object."""
+    flags = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
+             "-I", str(PKG.parent / "include")]
+    lines = {src: lambda obj, src=src: [*flags, "-c", str(src), "-o", str(obj) + ".tmp"] for src in sorted(SRC.glob("*.cu"))}
+    lines[SRC / "bind_q8.cpp"] = bind_command
+    return lines
+
+
+def link_library(objects) -> list[str]:
+    return [nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", *objects, "-o", str(LIB) + ".tmp"]
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
     if up_to_date() and not force:
         return LIB
     OBJ.mkdir(exist_ok=True)
-    flags = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
-             "-I", str(PKG.parent / "include")]
-    if verbose:
-        flags.insert(1, "-Xptxas=-v")
-    commands = {src: lambda obj, src=src: [*flags, "-c", str(src), "-o", str(obj) + ".tmp"] for src in sorted(SRC.glob("*.cu"))}
-    commands[SRC / "bind_q8.cpp"] = bind_command
     jobs, objects = [], []
-    for src, command in commands.items():
+    for src, command in compilations().items():
         obj = OBJ / (src.stem + ".o")
         if src.suffix == ".cu":
             objects.append(str(obj))
-        if not force and obj.exists() and all(obj.stat().st_mtime >= f.stat().st_mtime
-                                              for f in included(src) | {Path(__file__).resolve()}):
+        line = command(obj)
+        made, note = made_with(line), obj.with_suffix(".made")
+        if not force and obj.exists() and note.exists() and note.read_text() == made and all(
+                obj.stat().st_mtime >= f.stat().st_mtime for f in included(src) | {Path(__file__).resolve()}):
             continue
-        jobs.append((obj, subprocess.Popen(command(obj), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+        if verbose and src.suffix == ".cu":
+            line.insert(1, "-Xptxas=-v")
+        jobs.append((obj, note, made, subprocess.Popen(line, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = False
-    for obj, job in jobs:
+    for obj, note, made, job in jobs:
         out = job.communicate()[0]
         if job.returncode != 0 or verbose:
             sys.stderr.write(out)
@@ -100,15 +128,16 @@ def build(verbose: bool = False, force: bool = False) -> Path:
             failed = True
         else:
             os.replace(str(obj) + ".tmp", obj)
+            note.write_text(made)
     if failed:
         raise RuntimeError("compilation failed")
-    for out, command in ((LIB, [nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", *objects,
-                                "-o", str(LIB) + ".tmp"]), (BIND, link_bind(OBJ / "bind_q8.o"))):
+    for out, command in ((LIB, link_library(objects)), (BIND, link_bind(OBJ / "bind_q8.o"))):
         res = subprocess.run(command, capture_output=True, text=True)
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError(f"linking {out.name} failed with exit code {res.returncode}")
         os.replace(str(out) + ".tmp", out)
+    STAMP.write_text(stamp())
     return LIB
 
 

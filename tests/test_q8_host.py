@@ -124,3 +124,30 @@ int main() {
     subprocess.run(["g++", "-std=c++17", "-I", str(build.SRC), "-I", str(cuda / "include"), str(src), "-o", str(exe)], check=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True)
     assert res.returncode == 0, res.stdout
+
+
+def test_the_build_notices_what_it_was_built_with(monkeypatch, tmp_path):
+    """Built files are stale when a source, the build rules, a compiler line, torch or the Python ABI is another."""
+    import os
+    from attention_lab_b200 import build
+    assert build.PKG / "build.py" in build.sources()
+    for name in ("LIB", "BIND", "STAMP"):
+        monkeypatch.setattr(build, name, tmp_path / name)
+    assert not build.up_to_date()
+    build.LIB.touch(), build.BIND.touch()
+    assert not build.up_to_date()                                     # nothing says what they were built with
+    build.STAMP.write_text(build.stamp())
+    assert build.up_to_date()
+    with monkeypatch.context() as m:
+        m.setattr(build, "ARCH", [*build.ARCH, "-DSOMETHING"])
+        assert not build.up_to_date()
+    with monkeypatch.context() as m:
+        m.setattr(build.importlib.metadata, "version", lambda name: "0.0")
+        assert not build.up_to_date()
+    with monkeypatch.context() as m:
+        m.setattr(build.sysconfig, "get_config_var", lambda name: "other")
+        assert not build.up_to_date()
+    assert build.up_to_date()
+    newest = max(s.stat().st_mtime for s in build.sources())
+    os.utime(build.BIND, (newest - 10, newest - 10))
+    assert not build.up_to_date()
