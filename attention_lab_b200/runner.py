@@ -298,6 +298,8 @@ class LabState:
         self.eight_bit = isinstance(cache, Q8LabCache)
         if self.eight_bit and (mode != "full" or decode_backend != "kernel"):
             raise ValueError("an 8-bit cache is read in full mode by its own kernels")
+        if self.eight_bit and (indexers is not None or selector != "index" or sparse_layers is not None or canonical_order):
+            raise ValueError("an 8-bit cache has no sparse step: no indexers, selector, sparse_layers or canonical_order")
         if not self.eight_bit and (window or sinks):
             raise ValueError("window and sinks need an 8-bit cache (cache_format='q8')")
         if int(window) < 0 or int(sinks) < 0:

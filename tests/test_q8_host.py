@@ -151,3 +151,13 @@ def test_the_build_notices_what_it_was_built_with(monkeypatch, tmp_path):
     newest = max(s.stat().st_mtime for s in build.sources())
     os.utime(build.BIND, (newest - 10, newest - 10))
     assert not build.up_to_date()
+
+
+def test_a_state_over_an_8_bit_cache_refuses_what_it_cannot_use():
+    from attention_lab_b200 import runner
+    cache = runner.Q8LabCache(layers=2, batch=1, groups=1, capacity=64, head_dim=128, table=torch.zeros(64, 128), device="cpu")
+    assert runner.LabState(cache, window=8, sinks=1).eight_bit
+    for kw in (dict(sparse_layers=[0]), dict(selector="recent"), dict(selector="uniform"), dict(indexers=[None, None]),
+               dict(canonical_order=True)):
+        with pytest.raises(ValueError, match="8-bit"):
+            runner.LabState(cache, **kw)
