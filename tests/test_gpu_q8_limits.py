@@ -1,10 +1,14 @@
 """The 8-bit cache's operators on the GPU at their limits."""
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 import torch
 
+import q8_bounds
+from oracle import q8 as ref
 from test_gpu_q8 import DEV, TYPES, al, check_attend, gen, host, make_q, random_cache, status
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +153,43 @@ def test_a_wrong_type_is_reported_by_name():
                        (lambda: al().attend_q8(q, c, 3, window=2 ** 31), "window"), (lambda: al().attend_q8(q, c, 3, sinks=2 ** 64), "sinks")):
         with pytest.raises(ValueError, match=name):
             call()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h, T", [(4, 1), (2, 90)])
+@pytest.mark.parametrize("gap", [0, 10, 16, 20, 28, 40, 100])
+def test_quiet_blocks_under_a_loud_one(dtype, h, T, gap):
+    """One block whose V is 2^gap louder than the others but zero in half of the dimensions: in those an output comes from
+    the quiet blocks alone, and holds what the weights' lower end leaves of them (an absolute bound, relative to the row's
+    loudest visible term), while the denominator counts every block in full."""
+    n = 300
+    cache = random_cache(gap, 1, 2, n)
+    cache.v_exp.fill_(-50)
+    cache.v_exp[..., 2] = gap - 50
+    cache.v.view(torch.uint8)[:, :, 128:192, 64:] = 0
+    q = make_q(gap + 1, 1, 2, h, T, dtype)
+    out = host(al().attend_q8(q, cache, n)).astype(np.float64)
+    one_term = dtype == "bf16" and T > 1
+    for g in range(2):
+        want, tol = q8_bounds.attend(host(q)[0, g].astype(np.float64), ref.values(host(cache.k), cache.k_exp.cpu().numpy())[0, g],
+                                     host(cache.v)[0, g], cache.v_exp.cpu().numpy()[0, g], n, 0, 0, 1 / math.sqrt(128),
+                                     terms=1 if one_term else 2, out_half_ulp=2 ** -8 if dtype == "bf16" else 2 ** -24)
+        err = np.abs(out[0, g] - want)
+        assert np.all(err <= tol), float((err / np.maximum(tol, 1e-300)).max())
+        if gap <= 10:                                                  # and there something of them is left
+            assert np.abs(out[0, g][..., 64:] - want[..., 64:]).max() < 2 ** -6 * np.abs(want[..., 64:]).max()
+
+
+@pytest.mark.parametrize("h, T", [(17, 1), (1, 40), (5, 4), (64, 2), (9, 3)])
+def test_16_bit_queries_over_few_tokens_keep_two_terms(h, T):
+    """Up to 128 rows over few tokens take the single tokens' kernel, whose weights are two f16 terms in either type: scores
+    small enough that a lost low term shows (q8_bounds plants one on the CPU)."""
+    n = 24
+    cache = random_cache(h * T, 2, 1, 64)
+    q = make_q(h, 2, 1, h, T, "bf16")
+    out = host(al().attend_q8(q, cache, n, scale=0.02)).astype(np.float64)
+    for b in range(2):
+        want, tol = q8_bounds.attend(host(q)[b, 0].astype(np.float64), ref.values(host(cache.k), cache.k_exp.cpu().numpy())[b, 0],
+                                     host(cache.v)[b, 0], cache.v_exp.cpu().numpy()[b, 0], n, 0, 0, 0.02, terms=2,
+                                     out_half_ulp=2 ** -8)
+        assert np.all(np.abs(out[b, 0] - want) <= tol)

@@ -161,3 +161,39 @@ def test_a_state_over_an_8_bit_cache_refuses_what_it_cannot_use():
                dict(canonical_order=True)):
         with pytest.raises(ValueError, match="8-bit"):
             runner.LabState(cache, **kw)
+
+
+def test_the_attention_bound_notices_a_lost_low_term():
+    """tests/q8_bounds.py against its own planted mistakes: two-term weights stay within the two-term bound, weights cut to
+    one f16 term do not, and the one-term bound holds those."""
+    import numpy as np
+    import q8_bounds
+    from oracle import q8 as ref
+    rng = np.random.default_rng(0)
+    n = 24
+    q = rng.normal(size=(17, 1, 128))
+    k = ref._VALUES[ref.encode(np.clip(rng.normal(size=(n, 128)) * 60, -440, 440))] * 2.0 ** -6
+    v, e = ref.encode(np.clip(rng.normal(size=(n, 128)) * 60, -440, 440)), np.array([-6], np.int8)
+
+    def one(w):
+        return w.astype(np.float16).astype(np.float64)
+
+    def two(w):
+        return one(w) + one(w - one(w))
+
+    def run(terms, weight=None, half_ulp=2 ** -8):
+        return q8_bounds.attend(q, k, v, e, n, 0, 0, 0.02, terms=terms, out_half_ulp=half_ulp, weight=weight)
+
+    want, tol = run(2)
+    assert (np.abs(run(2, two)[0] - want) <= tol).all()
+    assert not (np.abs(run(2, one)[0] - want) <= tol).all()
+    assert (np.abs(run(1, one)[0] - want) <= run(1)[1]).all()
+    # a quiet block under a loud one: two terms end 2^-31 below the row's loudest term, which the bound allows and needs
+    e = np.array([-50, 0], np.int8)
+    k, v = np.tile(k, (4, 1))[:80], np.tile(v, (4, 1))[:80]
+    v[64:, 64:] = 0
+    n = 80
+    biased = lambda w: two(w * 2.0 ** -4) * 2.0 ** 4
+    want, tol = run(2, half_ulp=2 ** -24)
+    err = np.abs(run(2, biased, 2 ** -24)[0] - want)
+    assert (err <= tol).all() and np.abs(want[..., 64:]).min() > 0 and (err[..., 64:] > 0.5 * np.abs(want[..., 64:])).all()
