@@ -127,6 +127,11 @@ __device__ __forceinline__ float q8_rescale(float x, float d) {
   return x * a * a;
 }
 
+// Denominators are held in units of 2^11: a token counts its weight (2^6 to 2^14) times 2^-ev, with ev in [-100, 120], so
+// 2^25 tokens stay below 2^128 (blocks of zeros have ev = -100, and a CTA may walk very many) and one above 2^-126. Outputs
+// take the unit back before they are divided; both steps are exact.
+constexpr float kQ8Unit = 1.0f / 2048.0f;
+
 // Merging partials (m, l, O): the weight of one with maximum m under the common maximum M, and its share of the
 // denominator. An empty partial has m = -inf and l = 0; one whose every score was NaN has m = -inf and l NaN. Only empty
 // partials, whose O may not have been written, are left out (a negative weight): one whose weight underflows still brings
@@ -134,6 +139,9 @@ __device__ __forceinline__ float q8_rescale(float x, float d) {
 constexpr float kQ8Skip = -1.0f;
 __device__ __forceinline__ float q8_merge_weight(float l, float m, float M) {
   return m == -INFINITY ? (l == 0.0f ? kQ8Skip : 1.0f) : q8_ex2(m - M);
+}
+__device__ __forceinline__ float4 q8_divided(float4 a, float inv) {
+  return make_float4(a.x * kQ8Unit * inv, a.y * kQ8Unit * inv, a.z * kQ8Unit * inv, a.w * kQ8Unit * inv);
 }
 __device__ __forceinline__ void q8_merge_add(float4& a, float weight, const float4& v) {
   if (weight != kQ8Skip) { a.x += weight * v.x; a.y += weight * v.y; a.z += weight * v.z; a.w += weight * v.w; }
@@ -386,9 +394,9 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
       sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += q8_ex2(s[i] - (ref + fev));
-      l += sum;
+      l += sum * kQ8Unit;
     } else {
-      l += sum * inv_ev;
+      l += sum * kQ8Unit * inv_ev;
     }
     uint4 vr[8];                                            // row 16 (i >> 2) + 8 (i >> 1 & 1) + 4 (i & 1) + t4
 #pragma unroll
@@ -475,7 +483,7 @@ __global__ void __launch_bounds__(kQdThreads, 2) q8_decode_kernel(const Q8Attend
     if (L == 0.0f) a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int t = q8_row_token(col0 + c, p), hd = col0 + c - t * p.h;
     T* dst = static_cast<T*>(p.out) + (((long long)bg * p.h + hd) * p.T + t) * kHeadDim + 4 * lane;
-    q8_store4(dst, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+    q8_store4(dst, q8_divided(a, inv));
   };
   // Merge. Every warp has all 32 (warp, column) weights, one a lane, and takes columns warp, warp + kQdWarps: a lane 4
   // dimensions. (With the weights worked out by every thread for itself, in 32 copies of the code, this took 4600 cycles.)

@@ -193,3 +193,27 @@ def test_16_bit_queries_over_few_tokens_keep_two_terms(h, T):
                                      host(cache.v)[b, 0], cache.v_exp.cpu().numpy()[b, 0], n, 0, 0, 0.02, terms=2,
                                      out_half_ulp=2 ** -8)
         assert np.all(np.abs(out[b, 0] - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_long_runs_of_zero_values(dtype):
+    """Blocks whose V is all zero have the lowest exponent, so each of their tokens counts 2^100 times its weight in the
+    denominator until a block with values comes: a CTA that walks 20000 of them alone, at weights just under the point
+    where the maximum would follow, must not overflow there. Scores are 0 but for the first 64 tokens, 7.8 binades below."""
+    B, G, h, T, n = 8, 19, 2, 80, 20000
+    cache = al().Q8Cache.empty(B, G, n, DEV)
+    cache.k.view(torch.uint8).zero_(), cache.v.view(torch.uint8).zero_()
+    cache.k.view(torch.uint8)[:, :, :64, 0] = 0xB8                     # -1
+    cache.k_exp.zero_(), cache.v_exp.fill_(-100)
+    cache.v.view(torch.uint8)[:, :, 19968:] = 0x38                     # 1
+    cache.v_exp[:, :, 19968 // 64:] = 0
+    q = torch.zeros(B, G, h, T, 128, device=DEV, dtype=TYPES[dtype])
+    q[..., 0] = 1.0
+    scale = 7.8 * math.log(2)
+    out = al().attend_q8(q, cache, n, scale=scale).double().cpu()
+    p = torch.arange(n - T, n, dtype=torch.float64)                    # a query sees p + 1 tokens, p - 19967 with values
+    want = (p - 19967).clamp(min=0) / (p + 1 - 64 + 64 * 2 ** -7.8)
+    assert status() == 0
+    # the weights are equal but for their rounding, which no sum here can hide: a part in 2^8 (16 bits) or 2^12
+    tol = want * (2 ** -8 + 2 ** -12 if dtype == "bf16" else 2 ** -12)
+    assert ((out - want[:, None]).abs() <= tol[:, None]).all()
