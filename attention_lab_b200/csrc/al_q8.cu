@@ -65,6 +65,8 @@ int q8_plan(int B, int G, int h, int T, int C, int window, int sinks, int max_le
   int len = max_length > 0 ? std::min(max_length, C) : C;
   // tokens a query tile can see, as far as the host knows
   const long long span = window > 0 ? std::min<long long>(len, (long long)window + sinks) : len;
+  // (Times in this function: graph replays in bursts at the full clock, 1965 MHz; longer runs of the large ones are 10 to
+  // 15 % slower under the power cap.)
   // The few-column kernel reads the cache once per 8 query rows, the prompt kernel once per 256 but fills 128 x 128 tiles
   // and takes 8 us for the least work. Up to 16 rows the first wins throughout (16 heads over 32 x 8192 tokens: 175 us
   // against 211); up to 128 while everything it reads is small (one request, 8 groups: 64 rows over 512 tokens 5.8 us

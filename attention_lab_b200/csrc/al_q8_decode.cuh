@@ -3,23 +3,26 @@
 //
 // A query at position p sees the tokens j <= p with window = 0, or j > p - window, or j < sinks. A CTA holds 8 columns
 // (query, head) of one (batch, group); its warps walk steps of 32 tokens and every warp keeps its own online softmax,
-// so no warp waits for another until the end. A warp streams its steps' K and V rows (8 KB a step) through a ring of its
-// own in shared memory with cp.async (16-byte chunks XOR-swizzled by row, rows past the end zero-filled) and reads them
-// as 16 bytes a lane straight into the tensor-core fragments: both contractions may permute their summed index, their
-// tokens and their dimensions freely, and the order is chosen so that no two lanes of a quarter warp share a bank. K and
-// V codes become f16 exactly; q and the softmax weights are split into two f16 terms that occupy the two halves of the
-// MMA's 16 rows (rows 0-7 high, 8-15 low), so 8 columns with about 21 bits each cost the same MMAs as 16 columns with
-// 11. The block's exponents enter as 2^(ek) on the scores and as an addend ev inside the weights' exponent: weights are
-// w = 2^(s + ev - m) with the running maximum m over s + ev, the output sums w * code, and the denominator sums
-// w * 2^-ev.
+// so no warp waits for another until the end. A warp streams its steps' K and V rows (8 KB a step) through a ring of
+// its own in shared memory with cp.async (16-byte chunks XOR-swizzled by row, rows past the end zero-filled) and reads
+// them as 16 bytes a lane straight into the tensor-core fragments: both contractions may permute their summed index,
+// their tokens and their dimensions freely, and the order is chosen so that no two lanes of a quarter warp share a
+// bank. K and V codes become f16 exactly; q and the softmax weights are split into two f16 terms that occupy the two
+// halves of the MMA's 16 rows (rows 0-7 high, 8-15 low), so 8 columns with about 21 bits each cost the same MMAs as 16
+// columns with 11. (f16 ends the weights 2^-35 below a row's largest: what lies lower is lost to the output, not to the
+// denominator, which is summed from the unrounded weights.) The block's exponents enter as 2^(ek) on the scores and as
+// an addend ev inside the weights' exponent: weights are w = 2^(s + ev - m) with the running maximum m over s + ev, the
+// output sums w * code, and the denominator sums w * 2^-ev.
 //
 // Bound: HBM reads of 256 bytes per visible token and group. The work of a segment is split over a cluster of CTAs
 // whose partial (m, l, O) are merged through distributed shared memory, so one launch does the whole step; with so few
-// segments that clusters of 16 leave SMs idle, or with requests of their own lengths, over runs of steps whose partials go
-// through global memory to q8_merge_kernel. 32 requests of 16K to 32K tokens, 32/8 heads: 259 us, 6.2 TB/s; 32 of 32K: 322
-// us, 6.7 TB/s; one of 128K: 47 us, 5.7 TB/s; one of 2048: 5.1 us, all latency (launch, length, rows, a step, merge).
-// Registers fed from global memory without the ring ran the first at 417 us: two CTAs of four warps an SM held too few
-// bytes in flight.
+// segments that clusters of 16 leave SMs idle, or with requests of their own lengths, over runs of steps whose partials
+// go through global memory to q8_merge_kernel. 32 requests of 16K to 32K tokens, 32/8 heads: 260 us, 6.2 TB/s, for the
+// first 50 ms at 1965 MHz; then the power cap holds the SMs near 1750 MHz and it takes 285 to 304 (the conversions and
+// MMAs are close behind the memory). 32 of 32K: 324 us, 6.6 TB/s, then 365 to 389; one of 128K: 50 us, 5.4 TB/s; one of
+// 2048: 5.1 us, all latency (launch, length, rows, a step, merge). (bf16; graph replays of ten calls. The figures
+// beside the other choices here and in q8_plan are such replays at the full clock.) Registers fed from global memory
+// without the ring ran the first at 417 us: two CTAs of four warps an SM held too few bytes in flight.
 #pragma once
 #include <cuda_fp16.h>
 #include "al_q8.cuh"

@@ -12,14 +12,18 @@
 //   warps 8-11      read the codes from global memory, convert them to f16 (exact) and store them in the 128-byte
 //                   swizzled layout both contractions read; the next tile's codes are in registers meanwhile
 //   warps 12, 13    issue the MMAs, one per query tile
-// 16-bit queries are one f16 operand (scaled by a power of two per row, exact). 32-bit queries and their weights are
-// split into two f16 terms (SPLIT): twice the MMAs, about 21 bits, one query tile a CTA (see kQpFlush).
+// 16-bit queries are one f16 operand (scaled by a power of two per row, exact), and so are their weights: 11 bits, where the
+// output is rounded to 8 (a second term would double the P V MMAs; against elementary fp32 operations rounded once, outputs
+// move by 6.5e-4 in the norm, one ulp at most, and the error against 64 bits stays 1.6e-3). Denominators are summed from
+// unrounded weights. 32-bit queries and their weights are split into two f16 terms (SPLIT): twice the MMAs, about 21 bits,
+// one query tile a CTA (see kQpFlush). f16 ends either kind 2^-31 below a row's largest weight (see kQpBias).
 //
-// Bound: shared memory and the MUFU together. A step's MMAs read their operands for 1280 cycles of an SM's shared-memory
-// bandwidth (Q again for every 64 keys), the converting warps store 32 KB (256 cycles), and its exponentials hold the MUFU
-// pipe for 1024; measured are about 1800 a step. 8192 tokens of 32/8 heads: 516 us, 1.07 PFLOP/s of causal pairs; 1024
-// tokens late in two 16K contexts with a window of 2048: 101 us (256 CTAs in two waves). Q K^T over 128 keys reads less
-// but leaves one score buffer: 614 us.
+// Bound: shared memory and the MUFU together. A step's MMAs read their operands for 1280 cycles of an SM's shared-
+// memory bandwidth (Q again for every 64 keys), the converting warps store 32 KB (256 cycles), and its exponentials
+// hold the MUFU pipe for 1024; measured are about 1800 a step. 8192 tokens of 32/8 heads: 520 us, 1.06 PFLOP/s of
+// causal pairs, for the first 50 ms; then 565 under the power cap (SMs near 1800 MHz). 1024 tokens late in two 16K
+// contexts with a window of 2048: 101 us (256 CTAs in two waves). Q K^T over 128 keys reads less but leaves one score
+// buffer: 614 us.
 //
 // V codes that are NaN would reach rows that do not see them (0 * NaN in the MMA): they are replaced by zero on the way
 // in, their tokens noted, and rows that do see one get their NaN in the epilogue.
@@ -41,9 +45,13 @@ constexpr size_t kQpSmem = 1024 + 4 * kQpTile + 2 * kQpStage;   // 2 Q + 2 K + 2
 constexpr int kQpNanList = 64;
 // 32-bit queries: steps that O accumulates before it is added to the sum in TMEM's free half, in fp32 with rounding. The
 // tensor cores cut each of their sums off towards zero: without this the output loses 2.3e-6 over 1024 tokens, 1.8e-5 over
-// 16384 (elementary operations in fp32: 0.7e-6, 2.3e-6). 16-bit outputs are rounded to 2e-3 in any case.
+// 16384 (elementary operations in fp32: 0.7e-6, 2.3e-6). 16-bit outputs are rounded to 2e-3 in any case (a sum cuts off
+// about 1.3e-8: with one term 1.3e-5 over 16384 tokens of one CTA, 1e-4 over 131072).
 constexpr int kQpFlush = 4;
-constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;        // weights run up to 2^(6 + 8); f16 ends them 2^-30 below a row's largest
+// Weights run up to 2^(6 + 8), and f16's smallest step is 2^-24: a weight is good to 2^-31 of the row's largest at the worst.
+// The largest is that of 2^(s + ev), so a block of V that is 2^31 quieter than a visible one leaves nothing in the output,
+// also in dimensions where the loud block's codes are zero.
+constexpr float kQpBias = 6.0f, kQpLazy = 8.0f;
 // Registers a thread after the split: 2 x 128 softmax threads, 128 converting threads, the MMA warp's group.
 // 184 + 184 + 104 + 40 = 512 = 4 x the 128 of the launch.
 constexpr int kQpRegsSoftmax = 184, kQpRegsConvert = 104, kQpRegsMma = 40;

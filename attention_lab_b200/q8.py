@@ -189,5 +189,13 @@ def attend_q8(q: torch.Tensor, cache, lengths, *, window: int = 0, sinks: int = 
     """Attention of q [B,G,h,T,d] over the cache, causal: the query at position p sees the tokens j <= p, with a
     `window` > 0 only those with j > p - window or j < sinks. A row that sees nothing is zero. `max_length` (default: the
     capacity) is what the caller knows of the largest length; it chooses how the work is split, never the result's rows.
-    Returns [B,G,h,T,d] of q's dtype."""
+    Returns [B,G,h,T,d] of q's dtype.
+
+    Precision: the cache's values are exact, q too (32-bit q to 2^-22 of its row's largest element); scores, maxima,
+    denominators and outputs are summed in 32 bits. A softmax weight meets V as f16 terms: two (2^-21 of the weight) for
+    32-bit q, and for 16-bit q up to 16 rows (T * h) a group, or 128 over few tokens; one (2^-11) for longer 16-bit chunks,
+    where the output is rounded to 2^-8 in any case. Either ends 2^-31 below the row's largest 2^(score + exponent of the
+    V block): values of V that are so much quieter than a visible block leave nothing in the output, though their tokens
+    count in the denominator in full. A NaN code in a visible token makes the row (K) or its dimension (V) NaN, whatever
+    the token's weight; hidden tokens' codes never show."""
     return _bind.attend_q8(q, cache, lengths, window, sinks, scale, max_length)

@@ -241,8 +241,8 @@ int al_read_q8(const void* k_codes, const void* v_codes, const void* k_exp, cons
                int lo, int hi, int out_dtype, void* k_out, void* v_out, void* stream);
 
 /* Attention of q [B,G,h,T,128] (strides for B, G, h, T) over the cache: the query at position p sees tokens j <= p with
- *   window = 0, or j > p - window, or j < sinks. out [B,G,h,T,128] (dtype, contiguous); a row that sees nothing is zero.
- *   max_length (0 = C) is what the caller knows of the largest length; it only chooses how the work is split. The
+ *   window = 0, or j > p - window, or j < sinks (either of at least C hides nothing). out [B,G,h,T,128]
+ *   (dtype, contiguous); a row that sees nothing is zero. max_length (0 = C) is what the caller knows of the largest length; it only chooses how the work is split. The
  *   workspace (al_attend_q8_workspace bytes, 16-byte aligned; NULL when that is 0) holds partial results of the call. */
 int al_attend_q8_workspace(int B, int G, int h, int T, int C, int window, int sinks, int max_length, size_t* bytes);
 int al_attend_q8(const void* q, int64_t q_sb, int64_t q_sg, int64_t q_sh, int64_t q_st, int dtype,
